@@ -21,9 +21,10 @@ __all__ = [
     "BdattnError", "lib", "lib_path", "F32", "F16", "BF16", "MASK_NONE", "MASK_CAUSAL",
     "ROPE_INTERLEAVED", "ROPE_HALF_SPLIT", "SdpaParams", "NormRopeJob", "sdpa_fwd",
     "rmsnorm_rope", "linear_attn_relu_fwd", "rope_tables_flux", "rope_tables_qwen", "RopeSegment", "device_status", "last_error",
+    "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd",
 ]
 
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 MASK_NONE, MASK_CAUSAL = 0, 1
 STATUS_WAIT_TIMEOUT, STATUS_BAD_ARGS = 1, 2
 ROPE_INTERLEAVED, ROPE_HALF_SPLIT = 0, 1
@@ -110,6 +111,18 @@ class QkvoParams(C.Structure):
     ]
 
 
+class AddRmsNormParams(C.Structure):
+    """Mirror of ``bdattn_add_rmsnorm_params`` (include/bdattn.h)."""
+    _fields_ = [
+        ("dtype", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("residual_out", C.c_void_p),
+        ("gain", C.c_void_p), ("gain_dtype", C.c_int),
+        ("out", C.c_void_p), ("out_dtype", C.c_int), ("out_scale", C.c_void_p),
+        ("x_ld", C.c_longlong), ("residual_ld", C.c_longlong), ("residual_out_ld", C.c_longlong),
+        ("out_ld", C.c_longlong), ("eps", C.c_float),
+    ]
+
+
 _FORMATS = {C.c_int: "i", C.c_longlong: "q", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
 
 
@@ -128,6 +141,7 @@ def _packer(cls):
 
 _pack_sdpa, _pack_qkv, _pack_qkvo = _packer(SdpaParams), _packer(QkvProjParams), _packer(QkvoParams)
 _pack_job = _packer(NormRopeJob)
+_pack_add_rmsnorm = _packer(AddRmsNormParams)
 _FLT_MAX = struct.unpack("f", b"\xff\xff\x7f\x7f")[0]
 
 
@@ -136,7 +150,7 @@ def _f32(x):
     return x if -_FLT_MAX <= x <= _FLT_MAX else C.c_float(x).value
 
 
-_STRUCTURES = [C.POINTER(t) for t in (SdpaParams, QkvProjParams, QkvoParams, NormRopeJob)]
+_STRUCTURES = [C.POINTER(t) for t in (SdpaParams, QkvProjParams, QkvoParams, NormRopeJob, AddRmsNormParams)]
 
 _lib = None
 
@@ -205,9 +219,11 @@ def lib():
                                            C.c_int, C.c_void_p]
         L.bdattn_add_row_bias.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_longlong,
                                           C.c_int, C.c_void_p]
+        L.bdattn_add_rmsnorm_fwd.argtypes = [C.POINTER(AddRmsNormParams), C.c_void_p]
         # The same entry points for this module's own calls, which pass packed structures (bytes) as pointers
         for name in ("sdpa_fwd", "sdpa_fwd_allgather", "sdpa_fwd_allgather_multicast", "mgpu_sdpa_fwd_headsharded",
-                     "sdpa_traced_fwd", "rmsnorm_rope", "qkvo_fwd", "qkvo_fwd_static", "qkv_norm_rope_fwd"):
+                     "sdpa_traced_fwd", "rmsnorm_rope", "qkvo_fwd", "qkvo_fwd_static", "qkv_norm_rope_fwd",
+                     "add_rmsnorm_fwd"):
             fn = L["bdattn_" + name]             # a function object of its own
             fn.argtypes = [C.c_void_p if t in _STRUCTURES else t for t in getattr(L, "bdattn_" + name).argtypes]
             setattr(L, "packed_" + name, fn)
@@ -233,7 +249,8 @@ _current_device = None   # set by the first call, when CUDA is up
 def _bind_torch():
     global _torch, _raw_stream
     import torch
-    _dtype_codes.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32})
+    _dtype_codes.update({torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32,
+                         torch.float8_e4m3fn: E4M3})
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     _torch = torch
 
@@ -606,3 +623,49 @@ def qkv_norm_rope_fwd(x, wq, wk, wv, q_out, k_out, v_out, num_heads, head_dim, *
     except struct.error as e:
         raise TypeError(str(e)) from None
     _check(lib().packed_qkv_norm_rope_fwd(p, _stream(stream)))
+
+
+def _matrix(t, what, shape=None):
+    """(pointer, ld) of a 2-D tensor with contiguous columns (a single row or column may have any stride)."""
+    sh, st = t.shape, t.stride()
+    if len(st) != 2 or (st[1] != 1 and sh[1] > 1):
+        raise BdattnError(f"{what} must be a 2-D tensor with contiguous columns")
+    if shape is not None and sh != shape:
+        raise BdattnError(f"{what} has shape {tuple(sh)}, expected {tuple(shape)}")
+    return t.data_ptr(), st[0] if sh[0] > 1 else sh[1]
+
+
+def _vector(t, n, what):
+    """Pointer of a dense 1-D tensor of n values, 0 for None."""
+    if t is None:
+        return 0
+    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride()[0] != 1):
+        raise BdattnError(f"{what} must be a dense tensor of {n} values")
+    return t.data_ptr()
+
+
+def add_rmsnorm_fwd(x, out, gain=None, *, residual=None, residual_out=None, out_scale=None, eps=1e-6, stream=None):
+    """``bdattn_add_rmsnorm_fwd``: h = x (+ residual), residual_out = h, out = rmsnorm(h) * gain; with a
+    ``torch.float8_e4m3fn`` out, out_scale (rows, FP32) receives the rows' scales."""
+    xp, x_ld = _matrix(x, "x")
+    shape = x.shape
+    op, o_ld = _matrix(out, "out", shape)
+    dtype, out_dtype = _dtype_code(x), _dtype_code(out)
+    rp = r_ld = rop = ro_ld = 0
+    if residual is not None:
+        rp, r_ld = _matrix(residual, "residual", shape)
+        if residual.dtype != x.dtype:
+            raise BdattnError("residual must have the dtype of x")
+    if residual_out is not None:
+        rop, ro_ld = _matrix(residual_out, "residual_out", shape)
+        if residual_out.dtype != x.dtype:
+            raise BdattnError("residual_out must have the dtype of x")
+    if out_scale is not None and _dtype_code(out_scale) != F32:
+        raise BdattnError("out_scale must be FP32")
+    try:
+        p = _pack_add_rmsnorm(dtype, shape[0], shape[1], xp, rp, rop, _vector(gain, shape[1], "gain"),
+                              _dtype_code(gain) if gain is not None else F32, op, out_dtype,
+                              _vector(out_scale, shape[0], "out_scale"), x_ld, r_ld, ro_ld, o_ld, _f32(eps))
+    except struct.error as e:
+        raise TypeError(str(e)) from None
+    _check(lib().packed_add_rmsnorm_fwd(p, _stream(stream)))

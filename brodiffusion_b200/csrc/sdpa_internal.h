@@ -201,6 +201,21 @@ cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream);
 // problem of the launch must have whole tiles of that width.
 cudaError_t launch_gemm_pair(const GemmLaunch& L, int tile_cols, cudaStream_t stream);
 
+// Residual addition + RMSNorm of rows (16-bit in; 16-bit or e4m3 out).
+struct AddRmsNormArgs {
+    const void* x;
+    const void* residual;      // or null
+    void* residual_out;        // or null
+    const void* gain;          // cols values, or null
+    int gain_is_f32;
+    void* out;
+    float* out_scale;          // e4m3 output: rows values
+    int rows, cols;
+    long long ldx, ldr, ldro, ldo;
+    float eps;
+};
+cudaError_t launch_add_rmsnorm(const AddRmsNormArgs& a, bool bf16, bool fp8, cudaStream_t stream);
+
 // Elementwise helpers.
 cudaError_t launch_add_inplace(void* y, const void* x, long long n, bool bf16, cudaStream_t stream);
 cudaError_t launch_axpby_inplace(void* y, const void* x, long long n, float a, float b, bool bf16,

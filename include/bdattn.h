@@ -33,7 +33,7 @@ typedef struct CUstream_st* bdattn_stream_t; /* == cudaStream_t */
 
 /* Element types; values follow brotensor::Dtype order as used by the callers
  * (FP32, FP16, BF16). */
-enum { BDATTN_F32 = 0, BDATTN_F16 = 1, BDATTN_BF16 = 2 };
+enum { BDATTN_F32 = 0, BDATTN_F16 = 1, BDATTN_BF16 = 2, BDATTN_E4M3 = 3 /* 8 bits, no infinity, largest 448 */ };
 
 /* Attention visibility rules. */
 enum {
@@ -524,6 +524,44 @@ int bdattn_add_inplace(void* y, const void* x, long long n, int dtype, bdattn_st
 
 int bdattn_add_row_bias(void* y, const void* bias, int rows, int cols, long long ld, int dtype,
                         bdattn_stream_t stream);
+
+/* ------------------------------------------- a pre-norm layer over a stream
+ * The operators around attention in a causal layer whose K and V are cached (the
+ * text layers ahead of a denoiser, a block-causal prefix): norm, projections with
+ * everything behind them, attention over the cache.  No counterpart in the
+ * reference, which leaves such layers to its language-model library.
+ *
+ * bdattn_add_rmsnorm_fwd: the residual stream's addition and the norm of the sum,
+ *   h = x (+ residual) in FP32,  residual_out = h rounded to dtype,
+ *   y = h * rsqrt(mean(h^2) + eps) * gain,
+ *   out = y rounded to dtype (out_dtype = dtype), or, with out_dtype E4M3,
+ *   out_scale[row] = max|y| / 448 and out = e4m3(y / out_scale[row]) (a row of zeros
+ *   has scale 0; a row with a value that is not finite has scale NaN).
+ * The norm is that of the unrounded sum.  x, residual, residual_out (rows, cols) of
+ * dtype BF16 / F16; residual, residual_out and gain may be NULL; gain_dtype F32 or
+ * dtype.  residual_out may be residual or x (same ld), out may be x or residual
+ * where its dtype is theirs.  Any cols >= 1, any alignment of the element type and any ld >= cols;
+ * rows of 16-byte alignment with cols and ld multiples of 8 are the fast ones. */
+typedef struct bdattn_add_rmsnorm_params {
+    int dtype;
+    int rows;              /* 0: nothing is done */
+    int cols;
+    const void* x;
+    const void* residual;
+    void* residual_out;
+    const void* gain;
+    int gain_dtype;
+    void* out;
+    int out_dtype;
+    float* out_scale;      /* rows values; E4M3 output only */
+    long long x_ld;        /* 0 => cols */
+    long long residual_ld;
+    long long residual_out_ld;
+    long long out_ld;
+    float eps;
+} bdattn_add_rmsnorm_params;
+
+int bdattn_add_rmsnorm_fwd(const bdattn_add_rmsnorm_params* p, bdattn_stream_t stream);
 
 /* Y = a*Y + b*X over n dense elements, in place: the device side of the
  * prefix KV cache operations QwenImage21PrefixCache::scale_kv (brotensor
