@@ -21,7 +21,7 @@ __all__ = [
     "BdattnError", "lib", "lib_path", "F32", "F16", "BF16", "MASK_NONE", "MASK_CAUSAL",
     "ROPE_INTERLEAVED", "ROPE_HALF_SPLIT", "SdpaParams", "NormRopeJob", "sdpa_fwd",
     "rmsnorm_rope", "linear_attn_relu_fwd", "rope_tables_flux", "rope_tables_qwen", "RopeSegment", "device_status", "last_error",
-    "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd",
+    "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd", "WindowParams", "sdpa_window_fwd",
 ]
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
@@ -123,6 +123,11 @@ class AddRmsNormParams(C.Structure):
     ]
 
 
+class WindowParams(C.Structure):
+    """Mirror of ``bdattn_window_params`` (include/bdattn.h)."""
+    _fields_ = [("window", C.c_int), ("sinks", C.c_int), ("kv_len", C.c_void_p)]
+
+
 _FORMATS = {C.c_int: "i", C.c_longlong: "q", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
 
 
@@ -141,7 +146,7 @@ def _packer(cls):
 
 _pack_sdpa, _pack_qkv, _pack_qkvo = _packer(SdpaParams), _packer(QkvProjParams), _packer(QkvoParams)
 _pack_job = _packer(NormRopeJob)
-_pack_add_rmsnorm = _packer(AddRmsNormParams)
+_pack_add_rmsnorm, _pack_window = _packer(AddRmsNormParams), _packer(WindowParams)
 _FLT_MAX = struct.unpack("f", b"\xff\xff\x7f\x7f")[0]
 
 
@@ -150,7 +155,7 @@ def _f32(x):
     return x if -_FLT_MAX <= x <= _FLT_MAX else C.c_float(x).value
 
 
-_STRUCTURES = [C.POINTER(t) for t in (SdpaParams, QkvProjParams, QkvoParams, NormRopeJob, AddRmsNormParams)]
+_STRUCTURES = [C.POINTER(t) for t in (SdpaParams, QkvProjParams, QkvoParams, NormRopeJob, AddRmsNormParams, WindowParams)]
 
 _lib = None
 
@@ -219,11 +224,12 @@ def lib():
                                            C.c_int, C.c_void_p]
         L.bdattn_add_row_bias.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_longlong,
                                           C.c_int, C.c_void_p]
+        L.bdattn_sdpa_window_fwd.argtypes = [C.POINTER(SdpaParams), C.POINTER(WindowParams), C.c_void_p]
         L.bdattn_add_rmsnorm_fwd.argtypes = [C.POINTER(AddRmsNormParams), C.c_void_p]
         # The same entry points for this module's own calls, which pass packed structures (bytes) as pointers
         for name in ("sdpa_fwd", "sdpa_fwd_allgather", "sdpa_fwd_allgather_multicast", "mgpu_sdpa_fwd_headsharded",
                      "sdpa_traced_fwd", "rmsnorm_rope", "qkvo_fwd", "qkvo_fwd_static", "qkv_norm_rope_fwd",
-                     "add_rmsnorm_fwd"):
+                     "add_rmsnorm_fwd", "sdpa_window_fwd"):
             fn = L["bdattn_" + name]             # a function object of its own
             fn.argtypes = [C.c_void_p if t in _STRUCTURES else t for t in getattr(L, "bdattn_" + name).argtypes]
             setattr(L, "packed_" + name, fn)
@@ -314,7 +320,7 @@ def device_status(clear: bool = True) -> int:
 
 def sdpa_fwd(q, k, v, out, num_heads, *, mask_mode=MASK_NONE, key_mask=None, key_scale=None,
              val_scale=None, softmax_scale=0.0, num_kv_heads=0, q_norm=None, stream=None,
-             peer_out_ptrs=None, multicast_out_ptrs=None, _trace=None, _mgpu=None):
+             peer_out_ptrs=None, multicast_out_ptrs=None, _trace=None, _mgpu=None, _window=None):
     """``bdattn_sdpa_fwd``.  q/out and k/v are a tensor or a list of one or two
     tensors (row segments attended as if concatenated); tensors are
     (rows, nh*hd) or (B, rows, nh*hd) torch CUDA tensors.
@@ -375,6 +381,9 @@ def sdpa_fwd(q, k, v, out, num_heads, *, mask_mode=MASK_NONE, key_mask=None, key
                        gain[0], gain[1], gain_dtype, eps, cos, sin, rope_row0)
     except struct.error as e:
         raise TypeError(str(e)) from None
+    if _window is not None:
+        _check(lib().packed_sdpa_window_fwd(p, _window, _stream(stream)))
+        return
     if _trace is not None:
         _check(lib().packed_sdpa_traced_fwd(p, C.byref(_trace), _stream(stream)))
         return
@@ -635,6 +644,12 @@ def _matrix(t, what, shape=None):
     return t.data_ptr(), st[0] if sh[0] > 1 else sh[1]
 
 
+def _torch_int32():
+    if _torch is None:
+        _bind_torch()
+    return _torch.int32
+
+
 def _vector(t, n, what):
     """Pointer of a dense 1-D tensor of n values, 0 for None."""
     if t is None:
@@ -669,3 +684,31 @@ def add_rmsnorm_fwd(x, out, gain=None, *, residual=None, residual_out=None, out_
     except struct.error as e:
         raise TypeError(str(e)) from None
     _check(lib().packed_add_rmsnorm_fwd(p, _stream(stream)))
+
+
+def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, num_kv_heads=0, key_mask=None,
+                    softmax_scale=0.0, stream=None):
+    """``bdattn_sdpa_window_fwd``: causal attention over a cache; query i of Lq sits at position P = n - Lq + i, where
+    n = kv_len[b] (INT32, one value per batch item) or all rows of k, and sees the last ``window`` keys up to P (0: all) and
+    the first ``sinks``.  Tensors and segments as for ``sdpa_fwd``."""
+    segments = [t for x in (q, k, v, out) for t in (x if isinstance(x, (list, tuple)) else (x,))]
+    first = segments[0]
+    batch = first.shape[0] if first.dim() == 3 else 1
+    for t in segments:
+        if t.dtype != first.dtype or (t.shape[0] if t.dim() == 3 else 1) != batch:
+            raise BdattnError("q, k, v and out must have the same dtype and batch")
+    if kv_len is not None:
+        if getattr(kv_len, "dtype", None) != _torch_int32():
+            raise BdattnError("kv_len must be INT32")
+        kv_len = _vector(kv_len, batch, "kv_len")
+    try:
+        w = _pack_window(window, sinks, kv_len or 0)
+    except struct.error as e:
+        raise TypeError(str(e)) from None
+    if key_mask is not None:
+        rows = sum(t.shape[-2] for t in k) if isinstance(k, (list, tuple)) else k.shape[-2]
+        if _dtype_code(key_mask) != F32:
+            raise BdattnError("key_mask must be FP32")
+        _vector(key_mask, rows, "key_mask")
+    sdpa_fwd(q, k, v, out, num_heads, mask_mode=MASK_CAUSAL, key_mask=key_mask, softmax_scale=softmax_scale,
+             num_kv_heads=num_kv_heads, stream=stream, _window=w)

@@ -52,4 +52,68 @@ int bdattn_add_rmsnorm_fwd(const bdattn_add_rmsnorm_params* p, bdattn_stream_t s
     return 0;
 }
 
+int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_params* w, bdattn_stream_t stream) {
+    const char* op = "flash_attention_windowed_forward";
+    if (p == nullptr || w == nullptr) return fail("%s: params is null", op);
+    if (require_sm100(op)) return -1;
+    if (!is_16bit(p->dtype)) return fail("%s: dtype must be BF16 or F16 (got %d)", op, p->dtype);
+    if (w->window < 0 || w->sinks < 0) return fail("%s: window and sinks must be >= 0 (got %d and %d)", op, w->window, w->sinks);
+    if (p->mask_mode != BDATTN_MASK_CAUSAL) return fail("%s: mask_mode must be CAUSAL (got %d)", op, p->mask_mode);
+    if (p->key_scale != nullptr || p->val_scale != nullptr) return fail("%s: per-key scales are not taken with a window", op);
+    if (p->q_gain[0] != nullptr || p->q_gain[1] != nullptr || p->q_cos != nullptr || p->q_sin != nullptr)
+        return fail("%s: query norm and RoPE are not taken with a window (bdattn_rmsnorm_rope ahead of it)", op);
+    if (p->batch < 1 || p->num_heads < 1 || p->batch > 65535 || p->num_heads > 65535)
+        return fail("%s: batch and num_heads must be in [1, 65535] (got %d and %d)", op, p->batch, p->num_heads);
+    const int hd = p->head_dim;
+    if (hd < 8 || hd > 256 || hd % 8 != 0) return fail("%s: head_dim must be a multiple of 8 in [8, 256] (got %d)", op, hd);
+    const int nkv = p->num_kv_heads > 0 ? p->num_kv_heads : p->num_heads;
+    if (p->num_kv_heads < 0 || p->num_heads % nkv != 0)
+        return fail("%s: num_kv_heads must divide num_heads (got %d and %d)", op, p->num_kv_heads, p->num_heads);
+    if (p->n_q_seg < 1 || p->n_q_seg > 2 || p->n_kv_seg < 1 || p->n_kv_seg > 2)
+        return fail("%s: n_q_seg and n_kv_seg must be 1 or 2", op);
+    if (!aligned_to(p->key_mask, 4) || !aligned_to(w->kv_len, 4)) return fail("%s: key_mask and kv_len must be 4-byte aligned", op);
+    bdattn::SdpaWindowArgs g;
+    std::memset(&g, 0, sizeof(g));
+    const long long D = static_cast<long long>(p->num_heads) * hd, Dkv = static_cast<long long>(nkv) * hd;
+    long long lq = 0, lk = 0;
+    // one operand of a segment: its checks, and the stride between batch items that 0 stands for
+    auto rows_of = [&](const char* what, int s, const void* ptr, int rows, long long ld, long long stride, long long cols,
+                       long long* out) {
+        if (ptr == nullptr) return fail("%s: %s segment %d is null", op, what, s);
+        if (rows < 1) return fail("%s: %s segment %d has no rows", op, what, s);
+        if (ld < cols) return fail("%s: the row stride of %s segment %d is smaller than its %lld columns", op, what, s, cols);
+        if (ld % 8 != 0 || stride % 8 != 0 || !aligned16(ptr))
+            return fail("%s: %s segment %d must be 16-byte aligned with strides that are multiples of 8 elements", op, what, s);
+        *out = stride > 0 ? stride : rows * ld;
+        return 0;
+    };
+    for (int s = 0; s < p->n_q_seg; ++s) {
+        if (rows_of("q", s, p->q[s], p->q_rows[s], p->q_ld[s], p->q_batch_stride[s], D, &g.q_bs[s]) ||
+            rows_of("o", s, p->o[s], p->q_rows[s], p->o_ld[s], p->o_batch_stride[s], D, &g.o_bs[s]))
+            return -1;
+        g.q[s] = p->q[s]; g.o[s] = p->o[s]; g.q_rows[s] = p->q_rows[s]; g.q_ld[s] = p->q_ld[s]; g.o_ld[s] = p->o_ld[s];
+        lq += p->q_rows[s];
+    }
+    for (int s = 0; s < p->n_kv_seg; ++s) {
+        if (rows_of("k", s, p->k[s], p->kv_rows[s], p->k_ld[s], p->k_batch_stride[s], Dkv, &g.k_bs[s]) ||
+            rows_of("v", s, p->v[s], p->kv_rows[s], p->v_ld[s], p->v_batch_stride[s], Dkv, &g.v_bs[s]))
+            return -1;
+        g.k[s] = p->k[s]; g.v[s] = p->v[s]; g.kv_rows[s] = p->kv_rows[s]; g.k_ld[s] = p->k_ld[s]; g.v_ld[s] = p->v_ld[s];
+        lk += p->kv_rows[s];
+    }
+    // positions and key numbers are 32-bit: n - Lq + i, P - window
+    if (lq > (1 << 30) || lk > (1 << 30)) return fail("%s: more than 2^30 query or key rows", op);
+    g.mask_mode = 1;
+    g.q_offset = static_cast<int>(lk - lq);
+    g.head_dim = hd;
+    g.kv_group = p->num_heads / nkv;
+    g.key_mask = p->key_mask;
+    g.scale = p->softmax_scale > 0.0f ? p->softmax_scale : 1.0f / std::sqrt(static_cast<float>(hd));
+    g.window = w->window; g.sinks = w->sinks; g.kv_len = w->kv_len;
+    cudaError_t e = bdattn::launch_sdpa_window(g, p->num_heads, p->batch, p->dtype == BDATTN_BF16,
+                                               reinterpret_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(op, e);
+    return 0;
+}
+
 }  // extern "C"

@@ -88,6 +88,14 @@ struct SdpaGeneralArgs {
 cudaError_t launch_sdpa_general(const SdpaGeneralArgs& a, int num_heads, int batch, bool bf16,
                                 cudaStream_t stream);
 
+// Causal attention with a sliding window and visible first keys (sdpa_window.cuh).
+struct SdpaWindowArgs : SdpaGeneralArgs {
+    int window;            // 0: unbounded
+    int sinks;
+    const int* kv_len;     // keys of each batch item, or null
+};
+cudaError_t launch_sdpa_window(const SdpaWindowArgs& a, int num_heads, int batch, bool bf16, cudaStream_t stream);
+
 // Head-averaged attention map of a query-row range x leading key range.
 struct AttnMapArgs {
     int q_rows[2], kv_rows[2];

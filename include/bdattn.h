@@ -563,6 +563,28 @@ typedef struct bdattn_add_rmsnorm_params {
 
 int bdattn_add_rmsnorm_fwd(const bdattn_add_rmsnorm_params* p, bdattn_stream_t stream);
 
+/* bdattn_sdpa_window_fwd: causal attention over a cache with a sliding window and a few
+ * first keys that stay visible, what flash_attention_windowed_forward
+ * (src/dit/qwenimage21_forward.cpp:659-662) does with window != 0 and, with window = 0,
+ * unbounded.  Batch item b has n = kv_len[b] keys (kv_len NULL: all Lk); query i of Lq sits
+ * at position P = n - Lq + i and sees key j iff
+ *   j <= P  and  (window == 0  or  j > P - window  or  j < sinks)  and  key_mask[j] != 0
+ * (window counts the query's own key).  A query that sees nothing, one before the first key included,
+ * gives zeros.  What masked places hold reaches no output, infinities and NaN included, and rows
+ * past kv_len[b] need not be initialised.
+ *   p       as for bdattn_sdpa_fwd: segments, strides, batch, grouped heads, key_mask, softmax_scale;
+ *           mask_mode must be CAUSAL; no per-key scales and no fused query norm / RoPE
+ *   kv_len  batch ints in device memory, read by the kernel (a captured graph follows their
+ *           growth); a value outside [0, Lk] counts as the nearer end
+ * Calls with few query rows share the keys of a head among CTAs; no workspace in either form. */
+typedef struct bdattn_window_params {
+    int window;            /* >= 0; 0: unbounded */
+    int sinks;             /* >= 0 */
+    const int* kv_len;     /* or NULL */
+} bdattn_window_params;
+
+int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_params* w, bdattn_stream_t stream);
+
 /* Y = a*Y + b*X over n dense elements, in place: the device side of the
  * prefix KV cache operations QwenImage21PrefixCache::scale_kv (brotensor
  * scale_inplace, x = NULL and b = 0) and ::blend_from (brotensor axpby_inplace
