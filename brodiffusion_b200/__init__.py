@@ -21,7 +21,8 @@ __all__ = [
     "BdattnError", "lib", "lib_path", "F32", "F16", "BF16", "MASK_NONE", "MASK_CAUSAL",
     "ROPE_INTERLEAVED", "ROPE_HALF_SPLIT", "SdpaParams", "NormRopeJob", "sdpa_fwd",
     "rmsnorm_rope", "linear_attn_relu_fwd", "rope_tables_flux", "rope_tables_qwen", "RopeSegment", "device_status", "last_error",
-    "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd", "WindowParams", "sdpa_window_fwd",
+    "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd", "WindowParams", "sdpa_window_fwd", "LinearActParams",
+    "linear_act_fwd",
 ]
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
@@ -128,6 +129,16 @@ class WindowParams(C.Structure):
     _fields_ = [("window", C.c_int), ("sinks", C.c_int), ("kv_len", C.c_void_p)]
 
 
+class LinearActParams(C.Structure):
+    """Mirror of ``bdattn_linear_act_params`` (include/bdattn.h)."""
+    _fields_ = [
+        ("dtype", C.c_int), ("in_dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int),
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("gate", C.c_void_p), ("residual", C.c_void_p),
+        ("y", C.c_void_p), ("x_scale", C.c_void_p), ("w_scale", C.c_void_p), ("act", C.c_int),
+        ("x_ld", C.c_longlong), ("w_ld", C.c_longlong), ("residual_ld", C.c_longlong), ("y_ld", C.c_longlong),
+    ]
+
+
 _FORMATS = {C.c_int: "i", C.c_longlong: "q", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
 
 
@@ -146,7 +157,7 @@ def _packer(cls):
 
 _pack_sdpa, _pack_qkv, _pack_qkvo = _packer(SdpaParams), _packer(QkvProjParams), _packer(QkvoParams)
 _pack_job = _packer(NormRopeJob)
-_pack_add_rmsnorm, _pack_window = _packer(AddRmsNormParams), _packer(WindowParams)
+_pack_add_rmsnorm, _pack_window, _pack_linear_act = _packer(AddRmsNormParams), _packer(WindowParams), _packer(LinearActParams)
 _FLT_MAX = struct.unpack("f", b"\xff\xff\x7f\x7f")[0]
 
 
@@ -155,7 +166,8 @@ def _f32(x):
     return x if -_FLT_MAX <= x <= _FLT_MAX else C.c_float(x).value
 
 
-_STRUCTURES = [C.POINTER(t) for t in (SdpaParams, QkvProjParams, QkvoParams, NormRopeJob, AddRmsNormParams, WindowParams)]
+_STRUCTURES = [C.POINTER(t) for t in (SdpaParams, QkvProjParams, QkvoParams, NormRopeJob, AddRmsNormParams,
+                                       WindowParams, LinearActParams)]
 
 _lib = None
 
@@ -225,11 +237,12 @@ def lib():
         L.bdattn_add_row_bias.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_longlong,
                                           C.c_int, C.c_void_p]
         L.bdattn_sdpa_window_fwd.argtypes = [C.POINTER(SdpaParams), C.POINTER(WindowParams), C.c_void_p]
+        L.bdattn_linear_act_fwd.argtypes = [C.POINTER(LinearActParams), C.c_void_p]
         L.bdattn_add_rmsnorm_fwd.argtypes = [C.POINTER(AddRmsNormParams), C.c_void_p]
         # The same entry points for this module's own calls, which pass packed structures (bytes) as pointers
         for name in ("sdpa_fwd", "sdpa_fwd_allgather", "sdpa_fwd_allgather_multicast", "mgpu_sdpa_fwd_headsharded",
                      "sdpa_traced_fwd", "rmsnorm_rope", "qkvo_fwd", "qkvo_fwd_static", "qkv_norm_rope_fwd",
-                     "add_rmsnorm_fwd", "sdpa_window_fwd"):
+                     "add_rmsnorm_fwd", "sdpa_window_fwd", "linear_act_fwd"):
             fn = L["bdattn_" + name]             # a function object of its own
             fn.argtypes = [C.c_void_p if t in _STRUCTURES else t for t in getattr(L, "bdattn_" + name).argtypes]
             setattr(L, "packed_" + name, fn)
@@ -712,3 +725,37 @@ def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, nu
         _vector(key_mask, rows, "key_mask")
     sdpa_fwd(q, k, v, out, num_heads, mask_mode=MASK_CAUSAL, key_mask=key_mask, softmax_scale=softmax_scale,
              num_kv_heads=num_kv_heads, stream=stream, _window=w)
+
+
+ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
+
+
+def linear_act_fwd(x, w, bias, y, *, act="none", gate=None, residual=None, x_scale=None, w_scale=None, stream=None):
+    """``bdattn_linear_act_fwd``: y = residual + gate * act((x @ w.T) * x_scale[:, None] * w_scale + bias); x and w of
+    the type of y, or both ``torch.float8_e4m3fn`` with FP32 scales per row.  act: a key of ``ACTIVATIONS``."""
+    xp, x_ld = _matrix(x, "x")
+    wp, w_ld = _matrix(w, "w")
+    (M, K), N = x.shape, w.shape[0]
+    if w.shape[1] != K:
+        raise BdattnError(f"w has {w.shape[1]} columns, x {K}")
+    shape = (M, N)
+    yp, y_ld = _matrix(y, "y", shape)
+    dtype = y.dtype
+    if w.dtype != x.dtype:
+        raise BdattnError("x and w must have the same dtype")
+    rp = r_ld = 0
+    if residual is not None:
+        rp, r_ld = _matrix(residual, "residual", shape)
+    for t in (bias, gate, residual):
+        if t is not None and t.dtype != dtype:
+            raise BdattnError("bias, gate and residual must have the dtype of y")
+    for t in (x_scale, w_scale):
+        if t is not None and _dtype_code(t) != F32:
+            raise BdattnError("x_scale and w_scale must be FP32")
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        raise BdattnError(f"unknown activation {act!r} (one of {', '.join(ACTIVATIONS)})")
+    _check(lib().packed_linear_act_fwd(
+        _pack_linear_act(_dtype_code(y), _dtype_code(x), M, N, K, xp, wp, _vector(bias, N, "bias"), _vector(gate, N, "gate"), rp, yp,
+                         _vector(x_scale, M, "x_scale"), _vector(w_scale, N, "w_scale"), code, x_ld, w_ld, r_ld, y_ld),
+        _stream(stream)))

@@ -52,6 +52,42 @@ int bdattn_add_rmsnorm_fwd(const bdattn_add_rmsnorm_params* p, bdattn_stream_t s
     return 0;
 }
 
+int bdattn_linear_act_fwd(const bdattn_linear_act_params* p, bdattn_stream_t stream) {
+    const char* op = "bdattn_linear_act_fwd";
+    if (p == nullptr) return fail("%s: params is null", op);
+    if (require_sm100(op)) return -1;
+    if (!is_16bit(p->dtype)) return fail("%s: dtype must be BF16 or F16 (got %d)", op, p->dtype);
+    const bool fp8 = p->in_dtype == BDATTN_E4M3;
+    if (!fp8 && p->in_dtype != p->dtype) return fail("%s: in_dtype must be dtype or E4M3 (got %d)", op, p->in_dtype);
+    if (!fp8 && (p->x_scale != nullptr || p->w_scale != nullptr)) return fail("%s: scales go with E4M3 operands only", op);
+    if (p->act < BDATTN_ACT_NONE || p->act > BDATTN_ACT_SILU) return fail("%s: unknown activation %d", op, p->act);
+    if (p->M < 0 || p->N < 1 || p->K < 1) return fail("%s: M must be >= 0, N and K >= 1 (got %d, %d, %d)", op, p->M, p->N, p->K);
+    if (p->M == 0) return 0;
+    const long long ldx = p->x_ld != 0 ? p->x_ld : p->K, ldw = p->w_ld != 0 ? p->w_ld : p->K;
+    const long long ldr = p->residual_ld != 0 ? p->residual_ld : p->N, ldy = p->y_ld != 0 ? p->y_ld : p->N;
+    if (fp8 && (p->K % 16 != 0 || ldx % 16 != 0 || ldw % 16 != 0))
+        return fail("%s: inner size and row strides of E4M3 operands must be multiples of 16 (K=%d ldx=%lld ldw=%lld)", op, p->K, ldx, ldw);
+    if (p->residual != nullptr && (ldr < p->N || ldr % 8 != 0 || !aligned16(p->residual)))
+        return fail("%s: residual must be 16-byte aligned with a row stride of at least N and a multiple of 8 (got %lld)", op, ldr);
+    if (!aligned_to(p->bias, 2) || !aligned_to(p->gate, 2) || !aligned_to(p->x_scale, 4) || !aligned_to(p->w_scale, 4))
+        return fail("%s: bias, gate or scales are not aligned to their element type", op);
+    bdattn::GemmLaunch L;
+    std::memset(&L, 0, sizeof(L));
+    L.bf16 = p->dtype == BDATTN_BF16;
+    L.layer = true;
+    L.fp8 = fp8;
+    const int half = fp8 ? 2 : 1;        // e4m3 operands go through the 16-bit tensor maps in pairs
+    if (add_gemm_problem(op, L, 0, p->x, ldx / half, p->w, ldw / half, p->bias, p->y, ldy, p->M, p->N, p->K / half, 0, 0)) return -1;
+    bdattn::GemmProblem& g = L.args.p[0];
+    g.act = p->act;
+    g.gate = p->gate;
+    g.residual = p->residual;
+    g.ldr = ldr;
+    g.x_scale = p->x_scale;
+    g.w_scale = p->w_scale;
+    return launch_gemm(op, L, 1, reinterpret_cast<cudaStream_t>(stream));
+}
+
 int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_params* w, bdattn_stream_t stream) {
     const char* op = "flash_attention_windowed_forward";
     if (p == nullptr || w == nullptr) return fail("%s: params is null", op);

@@ -33,6 +33,7 @@
 // the pair, tcgen05.mma issuer for both, warps 2-9 = epilogue of the CTA's 128 rows (warp w
 // owns TMEM lanes 32 * (w % 4)..; warps 2-5 take the first half of a tile's output columns,
 // warps 6-9 the second half).
+#include "gemm_layer.cuh"
 #include "gemm_plan.h"
 #include "sdpa_internal.h"
 #include "tc05.cuh"
@@ -44,6 +45,7 @@ constexpr int kPThreads = 320;
 constexpr int kPRows = 256;                   // rows of a pair's tile
 constexpr int kPChunk = 128 * 64 * 2;         // 128 rows x 64 columns: one TMA box of A
 constexpr int kPStgBytes = 2048 + 512;        // one epilogue warp: staging, and 128 bias values as FP32
+constexpr int kPStgLayer = 2048 + 3 * 512;    // with a layer's epilogue: bias, weight scales, gate
 constexpr int kPPrefetch = 384;               // columns of K whose weights are asked for ahead
 constexpr int kPGroup = 16;                   // row blocks of a group
 
@@ -55,6 +57,8 @@ struct PairCfg {
     static constexpr int kBChunk = kN / 2 * 64 * 2;
     static constexpr int kStageBytes = 2 * kPChunk + 2 * kBChunk;
     static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kPStgBytes + 256 + 3 * 128 * 4 + 1024;
+    static constexpr int kSmemLayer = kSmemBytes + 8 * (kPStgLayer - kPStgBytes);
+    static_assert(kSmemLayer <= 227 * 1024, "shared memory of one CTA");
     static constexpr int kHalf = kN / 2;      // output columns of an epilogue warp
     static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 };
@@ -227,22 +231,24 @@ __device__ __forceinline__ void epilogue_heads(const GemmProblem& p, uint32_t ta
 
 // What the epilogue does with a tile: one instantiation each, so that each has the registers to itself and no
 // code to fetch around (GEGLU 4096 x 320 -> 1280 16.2 -> 14.9 us, 1024 x 640 -> 2560 12.8 -> 12.0, QKV of 256 rows 18.6 -> 18.4).
-enum PairEpilogue { kEpiPlain, kEpiGeglu, kEpiHeads };
+enum PairEpilogue { kEpiPlain, kEpiGeglu, kEpiHeads, kEpiLayer };
 
-template <bool kBf16, int kN, PairEpilogue kEpi>
+// kFp8: e4m3 operands (kEpiLayer only).
+template <bool kBf16, int kN, PairEpilogue kEpi, bool kFp8 = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                  const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB0,
                  const __grid_constant__ CUtensorMap tmB1, const __grid_constant__ CUtensorMap tmB2,
                  const GemmArgs g, const int total_tiles) {
     using C = PairCfg<kN>;
+    constexpr int kStg = kEpi == kEpiLayer ? kPStgLayer : kPStgBytes;
     constexpr int kPStages = C::kStages;
     constexpr int kPStageBytes = C::kStageBytes;
     extern __shared__ uint8_t gemm_pair_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(gemm_pair_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
-    uint8_t* stg_all = smem + kPStages * kPStageBytes;      // [8][kPStgBytes]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(stg_all + 8 * kPStgBytes);
+    uint8_t* stg_all = smem + kPStages * kPStageBytes;      // [8][kStg]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stg_all + 8 * kStg);
     uint64_t* full = bars;                   // [kPStages]
     uint64_t* empty = bars + kPStages;       // [kPStages]
     uint64_t* acc_full = empty + kPStages;   // [2]
@@ -342,7 +348,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         __syncwarp();
     } else if (warp == 1) {
         // ---------------------------------------- MMA issuer (first CTA of the pair)
-        constexpr uint32_t idesc = make_idesc_f16(kBf16 ? 1 : 0, kPRows, kN, 0, 0);
+        constexpr uint32_t idesc = make_idesc_f16(kBf16 && !kFp8 ? 1 : 0, kPRows, kN, 0, 0);
+        auto mma = [](uint32_t d, uint64_t a, uint64_t b, uint32_t acc) {
+            if constexpr (kFp8) umma_ss_pair_f8(d, a, b, idesc, acc);
+            else umma_ss_pair(d, a, b, idesc, acc);
+        };
         const uint64_t a0 = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
         const uint64_t b0 = make_smem_desc_sw128(smem_u32(smem) + 2 * kPChunk, 16, 1024);
         int slot = 0;
@@ -370,11 +380,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                     const uint64_t ad = a0 + slot * (kPStageBytes >> 4), bd = b0 + slot * (kPStageBytes >> 4);
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma_ss_pair(d_tmem, ad + 2 * kk, bd + 2 * kk, idesc, (c > 0 || kk > 0) ? 1u : 0u);
+                        mma(d_tmem, ad + 2 * kk, bd + 2 * kk, (c > 0 || kk > 0) ? 1u : 0u);
                     if (c + 1 < chunks) {
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            umma_ss_pair(d_tmem, ad + (kPChunk >> 4) + 2 * kk, bd + (C::kBChunk >> 4) + 2 * kk, idesc, 1u);
+                            mma(d_tmem, ad + (kPChunk >> 4) + 2 * kk, bd + (C::kBChunk >> 4) + 2 * kk, 1u);
                     }
                     umma_commit_pair(&empty[slot]);
                     if (c + 2 >= chunks) umma_commit_pair(&acc_full[as]);
@@ -387,7 +397,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         // -------------------------------------------------------- epilogue
         const int q = warp & 3;             // TMEM lane quarter of this warp
         const int half = (warp - 2) >> 2;   // which half of the tile's output columns
-        uint8_t* const stg = stg_all + (warp - 2) * kPStgBytes;
+        uint8_t* const stg = stg_all + (warp - 2) * kStg;
         float* const bias_w = reinterpret_cast<float*>(stg + 2048);    // behind the output staging
         // RMSNorm gains of the three problems as FP32 for the 256 threads of these warps
         for (int idx = threadIdx.x - 64; idx < 3 * 128; idx += kPThreads - 64) {
@@ -413,7 +423,22 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
             // where the 128 columns whose bias this warp keeps begin in the tile, and its own among them
             constexpr bool kWide = kN == 256;
             const int c_base = kWide ? half * 128 : 0, c_own = kWide ? 0 : half * C::kHalf;
-            {
+            ResidualPiece res;
+            const uint16_t* res0 = nullptr;
+            float x_scale = 1.0f;
+            if constexpr (kEpi == kEpiLayer) {
+                // what the columns, the rows and the first piece of the residual have, while the tile is computed
+#pragma unroll
+                for (int e = 0; e < 128; e += 32) layer_columns<kBf16>(p, bias_w, 128, e + lane, t.n0 + c_base + e + lane, true);
+                if (rows > 0) {
+                    if (p.residual != nullptr) {
+                        res0 = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<long long>(row0) * p.ldr + t.n0;
+                        res.load(res0 + c_base + c_own, p.ldr, rows, 32, lane);
+                    }
+                    if (kFp8 && p.x_scale != nullptr && lane < rows) x_scale = __ldg(p.x_scale + row0 + lane);
+                }
+                __syncwarp();
+            } else {
                 // 128 bias values (GEGLU: 64 and those of their gates), fetched while the tile is computed
                 const int lc = lane * 4;
                 const long long at = geglu
@@ -465,6 +490,20 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                         store_words32(packed, stg, lane, cbase + c, p.ldc, rows, 32);
                     }
                 }
+            } else if (kEpi == kEpiLayer) {
+#pragma unroll 1
+                for (int c = c_base + c_own; c < c_base + c_own + C::kHalf; c += 32) {
+                    uint32_t w[16] = {};
+                    if (res0 != nullptr) {
+                        res.row_of_lane(stg, lane, w);
+                        if (c + 32 < c_base + c_own + C::kHalf) res.load(res0 + c + 32, p.ldr, rows, 32, lane);
+                    }
+                    float f[32];
+                    tmem_ld32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(&f[0]));
+                    tmem_wait_ld();
+                    layer_values<kBf16, kFp8>(p, f, bias_w + (c - c_base), 128, x_scale, w);
+                    store_tile32<kBf16>(f, stg, lane, cbase + c, p.ldc, rows, 32);
+                }
             } else {
 #pragma unroll 1
                 for (int c = c_base + c_own; c < c_base + c_own + C::kHalf; c += 32) {
@@ -504,10 +543,11 @@ static cudaError_t launch_gemm_pair_n(const GemmLaunch& L, cudaStream_t stream) 
         total += pair_tiles_m(L.args.p[i]) * (L.args.p[i].N / pair_out_cols<kN>(L.args.p[i]));
     const int pairs = sm_count() / 2;
     const dim3 grid(static_cast<unsigned>(2 * (total < pairs ? total : pairs)));
+    const int smem = L.layer ? PairCfg<kN>::kSmemLayer : PairCfg<kN>::kSmemBytes;
     auto go = [&](auto kern) {
-        cudaError_t e = set_max_smem_once(kern, PairCfg<kN>::kSmemBytes);
+        cudaError_t e = set_max_smem_once(kern, smem);
         if (e != cudaSuccess) return e;
-        return launch_dependent(kern, grid, dim3(kPThreads), PairCfg<kN>::kSmemBytes, stream, L.tmA[0], L.tmA[1], L.tmA[2],
+        return launch_dependent(kern, grid, dim3(kPThreads), smem, stream, L.tmA[0], L.tmA[1], L.tmA[2],
                                 L.tmB[0], L.tmB[1], L.tmB[2], L.args, total);
     };
     bool geglu = false, heads = false;
@@ -515,7 +555,9 @@ static cudaError_t launch_gemm_pair_n(const GemmLaunch& L, cudaStream_t stream) 
         geglu = geglu || L.args.p[i].geglu_offset > 0;
         heads = heads || L.args.p[i].norm_rope;
     }
-    if (geglu && heads) return cudaErrorInvalidValue;        // no entry point asks for both
+    if ((geglu && heads) || (L.layer && (geglu || heads))) return cudaErrorInvalidValue;        // no entry point asks for both
+    if (L.layer && L.fp8) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiLayer, true>) : go(gemm_pair_kernel<false, kN, kEpiLayer, true>);
+    if (L.layer) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiLayer>) : go(gemm_pair_kernel<false, kN, kEpiLayer>);
     if (geglu) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiGeglu>) : go(gemm_pair_kernel<false, kN, kEpiGeglu>);
     if (heads) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiHeads>) : go(gemm_pair_kernel<false, kN, kEpiHeads>);
     return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiPlain>) : go(gemm_pair_kernel<false, kN, kEpiPlain>);

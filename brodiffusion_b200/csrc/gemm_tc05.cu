@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 #include <type_traits>
 
+#include "gemm_layer.cuh"
 #include "gemm_plan.h"
 #include "sdpa_internal.h"
 #include "tc05.cuh"
@@ -60,7 +61,7 @@ __device__ __forceinline__ float gemm_ld16(const void* base, long long i) {
 // over two 13.4 -> 11.5).  Up to 64 rows are dealt out one by one, so that every CTA has some; more are
 // taken as blocks (128 x 640 x 5120 over eight 7.8 us dealt out, 7.4; 64 x 1280 x 1280 4.7, 5.2 in blocks).  Of a narrow
 // tile no thread gets columns that do not exist: 5251 x 8 x 1064 8.0 -> 6.9 us, 113 x 8 x 680 5.4 -> 4.2.
-template <bool kBf16>
+template <bool kBf16, bool kLayer, bool kFp8>
 __device__ __forceinline__ void epilogue_split(const GemmProblem& p, cooperative_groups::cluster_group& cluster,
                                                float* red, const float* bias_s, int split, int part, int tid, int m0, int n0) {
     const int ld = gemm_red_ld(p.n_tile);
@@ -76,6 +77,16 @@ __device__ __forceinline__ void epilogue_split(const GemmProblem& p, cooperative
         const int j = i >> sh, c = (i & ((1 << sh) - 1)) * 8;
         const int r = dealt ? part + split * j : part * (128 / split) + j;
         if (r >= rows || c >= n_valid) continue;
+        uint32_t res[4] = {};
+        float x_scale = 1.0f;
+        if constexpr (kLayer) {
+            if (p.residual != nullptr) {
+                const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.residual) +
+                                                                static_cast<long long>(m0 + r) * p.ldr + n0 + c);
+                res[0] = w.x; res[1] = w.y; res[2] = w.z; res[3] = w.w;
+            }
+            if (kFp8 && p.x_scale != nullptr) x_scale = __ldg(p.x_scale + m0 + r);
+        }
         float4 u[8], v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -93,8 +104,12 @@ __device__ __forceinline__ void epilogue_split(const GemmProblem& p, cooperative
                 f[4] += v[k].x; f[5] += v[k].y; f[6] += v[k].z; f[7] += v[k].w;
             }
         }
+        if constexpr (kLayer) {
+            layer_values<kBf16, kFp8>(p, f, bias_s + c, 128, x_scale, res);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] += bias_s[c + e];
+            for (int e = 0; e < 8; ++e) f[e] += bias_s[c + e];
+        }
         uint4 w;
         w.x = pack2<kBf16>(f[0], f[1]); w.y = pack2<kBf16>(f[2], f[3]);
         w.z = pack2<kBf16>(f[4], f[5]); w.w = pack2<kBf16>(f[6], f[7]);
@@ -106,7 +121,8 @@ __device__ __forceinline__ void epilogue_split(const GemmProblem& p, cooperative
 // GEGLU and the norm + RoPE code are long, and an epilogue that only branches around them
 // spent more time fetching instructions than storing (5.6 us for one 128 x 128 tile
 // against 2.3 us).
-template <bool kBf16, bool kGeglu, bool kNormRope, bool kSplit>
+// kLayer: scales, activation, gate and residual (gemm_layer.cuh); kFp8: e4m3 operands.
+template <bool kBf16, bool kGeglu, bool kNormRope, bool kSplit, bool kLayer = false, bool kFp8 = false>
 __global__ void __launch_bounds__(kGemmThreads)
 gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                  const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB0,
@@ -133,7 +149,8 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
     uint64_t* empty = bars + kGemmMaxStages;
     uint64_t* acc_done = empty + kGemmMaxStages;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_done + 1);
-    float* bias_s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);    // [128] and [128] of the gate
+    // [128] and [128] of the gate, or with kLayer bias, weight scale and gate
+    float* bias_s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);
 
     const int warp = warp_index();
     const int lane = threadIdx.x & 31;
@@ -203,7 +220,7 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         // One elected thread runs the whole loop (with the warp in step and the lane elected for each
         // block 576 x 1280 x 1280 takes 7.3 us, this way 6.5).  The slot and its parity are counted on, a
         // division by the runtime ring size cost more than the four MMAs.
-        const uint32_t idesc = make_idesc_f16(kBf16 ? 1 : 0, 128, p.n_tile, 0, 0);
+        const uint32_t idesc = make_idesc_f16(kBf16 && !kFp8 ? 1 : 0, 128, p.n_tile, 0, 0);
         const uint64_t a0 = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
         const uint64_t b0 = make_smem_desc_sw128(smem_u32(smem) + kGemmABytes, 16, 1024);
         const uint32_t stage_units = static_cast<uint32_t>(kGemmStageBytes) >> 4;   // descriptors count 16 bytes
@@ -217,7 +234,8 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                 const uint64_t ad = a0 + slot * stage_units, bd = b0 + slot * stage_units;
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
-                    umma_ss(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                    if constexpr (kFp8) umma_ss_f8(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                    else umma_ss(tmem_base, ad + 2 * kk, bd + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
                     if (geglu) umma_ss(tmem_base + 128, ad + 2 * kk, bd + gate_units + 2 * kk, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
                 }
                 umma_commit(&empty[slot]);
@@ -234,10 +252,23 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
             // the tile's bias, zero where there is none, while the tile is computed
             const int t = static_cast<int>(threadIdx.x) - 64;
             const bool on = p.bias != nullptr && t < p.n_tile && n0 + t < p.N;
-            bias_s[t] = on ? gemm_ld16<kBf16>(p.bias, n0 + t) : 0.0f;
+            if constexpr (kLayer) layer_columns<kBf16>(p, bias_s, 128, t, n0 + t, t < p.n_tile && n0 + t < p.N);
+            else bias_s[t] = on ? gemm_ld16<kBf16>(p.bias, n0 + t) : 0.0f;
             if constexpr (kGeglu)
                 bias_s[128 + t] = on && geglu ? gemm_ld16<kBf16>(p.bias, static_cast<long long>(n0) + p.geglu_offset + t) : 0.0f;
             asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+        const int n_valid = min(p.n_tile, p.N - n0);      // a ragged last tile stops at the matrix edge
+        // the residual's first piece and the rows' scales, while the tile is computed
+        ResidualPiece res;
+        float x_scale = 1.0f;
+        const uint16_t* res0 = nullptr;
+        if constexpr (kLayer && !kSplit) {
+            if (p.residual != nullptr) {
+                res0 = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<long long>(m0 + q * 32) * p.ldr + n0;
+                res.load(res0, p.ldr, p.M - m0 - q * 32, n_valid, lane);
+            }
+            if (kFp8 && p.x_scale != nullptr && row < p.M) x_scale = __ldg(p.x_scale + row);
         }
         bool ok = mbar_wait(acc_done, 0);
         ok = __all_sync(0xffffffffu, ok);
@@ -245,7 +276,6 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
         uint16_t* crow0 = reinterpret_cast<uint16_t*>(p.C) + static_cast<long long>(m0 + q * 32) * p.ldc + n0;
         uint16_t* crow = crow0 + static_cast<long long>(lane) * p.ldc;
-        const int n_valid = min(p.n_tile, p.N - n0);      // a ragged last tile stops at the matrix edge
         if constexpr (kSplit) {
             // partial sums to shared memory: the ring is at rest, its last MMA has completed
             float* rrow = reinterpret_cast<float*>(smem) + (q * 32 + lane) * gemm_red_ld(p.n_tile);
@@ -329,6 +359,20 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                     }
                 }
             }
+        } else if (kLayer) {
+#pragma unroll 1
+            for (int c = 0; ok && c < n_valid; c += 32) {
+                uint32_t w[16] = {};
+                if (res0 != nullptr) {
+                    res.row_of_lane(smem + q * 2048, lane, w);
+                    if (c + 32 < n_valid) res.load(res0 + c + 32, p.ldr, p.M - m0 - q * 32, n_valid - c - 32, lane);
+                }
+                float f[32];
+                tmem_ld32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(&f[0]));
+                tmem_wait_ld();
+                layer_values<kBf16, kFp8>(p, f, bias_s + c, 128, x_scale, w);
+                store_tile32<kBf16>(f, smem + q * 2048, lane, crow0 + c, p.ldc, p.M - m0 - q * 32, n_valid - c);
+            }
         } else if (ok) {
             for (int c = 0; c < n_valid; c += 32) {
                 uint32_t v[32], gt[32];
@@ -356,7 +400,7 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         cg::cluster_group cluster = cg::this_cluster();
         cluster_sync();
         if (warp >= 2)
-            epilogue_split<kBf16>(p, cluster, reinterpret_cast<float*>(smem), bias_s, split, part,
+            epilogue_split<kBf16, kLayer, kFp8>(p, cluster, reinterpret_cast<float*>(smem), bias_s, split, part,
                                   static_cast<int>(threadIdx.x) - 64, m0, n0);
         cluster_sync_relaxed();      // the peers' shared memory stays until everyone has read it
     }
@@ -408,7 +452,7 @@ cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream) {
         // so that one CTA's epilogue runs under the others' loads (4096 x 320 -> 960: 18.1 -> 12.2 us).
         args.stages = 2;
     }
-    const int smem = args.stages * stage + 256 + 1024 + 1024;    // barriers, bias, alignment
+    const int smem = args.stages * stage + 256 + (L.layer ? 1536 : 1024) + 1024;    // barriers, bias, alignment
     const dim3 grid(static_cast<unsigned>(tn), static_cast<unsigned>(tm),
                     static_cast<unsigned>(L.n_problems * args.split));
     cudaError_t e = cudaSuccess;
@@ -420,6 +464,10 @@ cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream) {
     };
     auto pick = [&](auto bf16) {
         constexpr bool kB = decltype(bf16)::value;
+        if (L.layer && args.split > 1) return L.fp8 ? go(gemm_tc05_kernel<kB, false, false, true, true, true>)
+                                                    : go(gemm_tc05_kernel<kB, false, false, true, true, false>);
+        if (L.layer) return L.fp8 ? go(gemm_tc05_kernel<kB, false, false, false, true, true>)
+                                  : go(gemm_tc05_kernel<kB, false, false, false, true, false>);
         if (any_norm_rope) go(gemm_tc05_kernel<kB, false, true, false>);        // never split
         else if (any_geglu) go(gemm_tc05_kernel<kB, true, false, false>);
         else if (args.split > 1) go(gemm_tc05_kernel<kB, false, false, true>);

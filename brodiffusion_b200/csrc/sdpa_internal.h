@@ -186,7 +186,16 @@ struct GemmProblem {
     const float* sin;
     int rope_row0;
     int norm_rope;      // 1: run the per-head epilogue
+    // Scales of 8-bit operands, activation, gate and residual (GemmLaunch::layer):
+    //   C = residual + gate * act(acc * x_scale * w_scale + bias)
+    int act;                // GemmAct
+    const void* gate;       // N values of the output dtype, or null
+    const void* residual;   // (M, N) of the output dtype, or null; may be C
+    long long ldr;
+    const float* x_scale;   // M values, or null
+    const float* w_scale;   // N values, or null
 };
+enum GemmAct { kActNone = 0, kActGelu = 1, kActGeluTanh = 2, kActSilu = 3 };
 struct GemmArgs {
     GemmProblem p[3];
     int n_tile_max;   // largest n_tile of the launch: sizes the shared-memory stages
@@ -203,6 +212,8 @@ struct GemmLaunch {
     GemmArgs args;
     int n_problems;
     bool bf16;
+    bool layer;            // the epilogue with scales, activation, gate and residual
+    bool fp8;              // e4m3 operands: K and their strides then count pairs of elements
 };
 cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream);
 // Persistent kernel of CTA pairs with tiles of 256 rows x tile_cols (256 or 128) accumulator columns; every

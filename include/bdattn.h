@@ -563,6 +563,38 @@ typedef struct bdattn_add_rmsnorm_params {
 
 int bdattn_add_rmsnorm_fwd(const bdattn_add_rmsnorm_params* p, bdattn_stream_t stream);
 
+/* bdattn_linear_act_fwd: a projection with what stands behind it,
+ *   z = (sum_k X[m, k] W[n, k]) * x_scale[m] * w_scale[n] + bias[n],
+ *   Y[m, n] = residual[m, n] + gate[n] * act(z)
+ * in FP32, rounded once.  X (M, K) and W (N, K, row-major as everywhere here) are of in_dtype: dtype, or
+ * E4M3 with FP32 scales per row of X (what bdattn_add_rmsnorm_fwd writes) and per row of W.  bias, gate
+ * (N values), residual and Y (M, N) are of dtype BF16 / F16; bias, gate, residual and the scales may be
+ * NULL (scales go with E4M3 only); residual may be Y (same ld).  16-byte aligned matrices, N and the
+ * strides of Y and residual multiples of 8, K and the strides of X and W of 8 (E4M3: 16). */
+enum { BDATTN_ACT_NONE = 0, BDATTN_ACT_GELU = 1 /* erf */, BDATTN_ACT_GELU_TANH = 2, BDATTN_ACT_SILU = 3 };
+typedef struct bdattn_linear_act_params {
+    int dtype;
+    int in_dtype;
+    int M;                 /* 0: nothing is done */
+    int N;
+    int K;
+    const void* x;
+    const void* w;
+    const void* bias;
+    const void* gate;
+    const void* residual;
+    void* y;
+    const float* x_scale;
+    const float* w_scale;
+    int act;               /* BDATTN_ACT_* */
+    long long x_ld;        /* 0 => K */
+    long long w_ld;        /* 0 => K */
+    long long residual_ld; /* 0 => N */
+    long long y_ld;        /* 0 => N */
+} bdattn_linear_act_params;
+
+int bdattn_linear_act_fwd(const bdattn_linear_act_params* p, bdattn_stream_t stream);
+
 /* bdattn_sdpa_window_fwd: causal attention over a cache with a sliding window and a few
  * first keys that stay visible, what flash_attention_windowed_forward
  * (src/dit/qwenimage21_forward.cpp:659-662) does with window != 0 and, with window = 0,
