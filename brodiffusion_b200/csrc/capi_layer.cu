@@ -10,6 +10,43 @@ namespace {
 bool is_16bit(int dtype) { return dtype == BDATTN_BF16 || dtype == BDATTN_F16; }
 bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// The tensor-core attention kernel's arguments for a call with a window: head_dim <= 128.
+int window_launch(const char* op, bdattn::SdpaLaunch& L, const bdattn::SdpaWindowArgs& g, int num_heads, int num_kv_heads, int batch,
+                  bool bf16) {
+    std::memset(&L, 0, sizeof(L));
+    bdattn::SdpaDevArgs& a = L.args;
+    for (int s = 0; s < 2; ++s) {
+        // (a second segment that does not exist has the first one's maps and no rows)
+        const int q = g.q_rows[s] > 0 ? s : 0, k = g.kv_rows[s] > 0 ? s : 0;
+        if (make_map_heads(op, &L.tmQ[s], g.q[q], bf16, g.head_dim, num_heads, g.q_rows[q], batch, g.q_ld[q], g.q_bs[q], 128) ||
+            make_map_heads(op, &L.tmK[s], g.k[k], bf16, g.head_dim, num_kv_heads, g.kv_rows[k], batch, g.k_ld[k], g.k_bs[k], 128) ||
+            make_map_heads(op, &L.tmV[s], g.v[k], bf16, g.head_dim, num_kv_heads, g.kv_rows[k], batch, g.v_ld[k], g.v_bs[k], 128))
+            return -1;
+        a.q_rows[s] = g.q_rows[s];
+        a.kv_rows[s] = g.kv_rows[s];
+        a.o[s] = g.o[s];
+        a.o_ld[s] = g.o_ld[s];
+        a.o_bs[s] = g.o_bs[s];
+    }
+    a.q_ctas0 = (a.q_rows[0] + 255) / 256;
+    a.kv_tiles0 = (a.kv_rows[0] + 127) / 128;
+    a.kv_tiles = a.kv_tiles0 + (a.kv_rows[1] + 127) / 128;
+    a.mask_mode = 1;
+    a.q_offset = g.q_offset;
+    a.lq_total = g.q_rows[0] + g.q_rows[1];
+    a.hd_out = g.head_dim;
+    a.kv_group = g.kv_group;
+    a.key_mask = g.key_mask;
+    a.scale_log2 = g.scale * 1.4426950408889634f;
+    L.window = &g;
+    L.q_ctas = a.q_ctas0 + (a.q_rows[1] + 255) / 256;
+    L.num_heads = num_heads;
+    L.batch = batch;
+    L.head_dim = g.head_dim <= 64 ? 64 : 128;
+    L.bf16 = bf16;
+    return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -145,9 +182,20 @@ int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_para
     g.kv_group = p->num_heads / nkv;
     g.key_mask = p->key_mask;
     g.scale = p->softmax_scale > 0.0f ? p->softmax_scale : 1.0f / std::sqrt(static_cast<float>(hd));
-    g.window = w->window; g.sinks = w->sinks; g.kv_len = w->kv_len;
-    cudaError_t e = bdattn::launch_sdpa_window(g, p->num_heads, p->batch, p->dtype == BDATTN_BF16,
-                                               reinterpret_cast<cudaStream_t>(stream));
+    // a window, or sinks, of all keys is no window: from here on both are below 2^30
+    g.window = w->window >= lk || w->sinks >= lk ? 0 : w->window;
+    g.sinks = w->sinks < lk ? w->sinks : static_cast<int>(lk);
+    g.kv_len = w->kv_len;
+    const bool bf16 = p->dtype == BDATTN_BF16;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (hd <= 128) {
+        bdattn::SdpaLaunch L;
+        if (window_launch(op, L, g, p->num_heads, nkv, p->batch, bf16)) return -1;
+        e = bdattn::launch_sdpa_tc05(L, st);
+    } else {
+        e = bdattn::launch_sdpa_window(g, p->num_heads, p->batch, bf16, st);
+    }
     if (e != cudaSuccess) return cuda_fail(op, e);
     return 0;
 }

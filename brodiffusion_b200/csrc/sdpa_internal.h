@@ -54,9 +54,11 @@ struct SdpaDevArgs {
     void* o_mc[2];
 };
 
+struct SdpaWindowArgs;
 struct SdpaLaunch {
     CUtensorMap tmQ[2], tmK[2], tmV[2];
     SdpaDevArgs args;
+    const SdpaWindowArgs* window;    // sliding window and sinks, or null
     int q_ctas;
     int num_heads;
     int batch;
@@ -93,6 +95,10 @@ struct SdpaWindowArgs : SdpaGeneralArgs {
     int window;            // 0: unbounded
     int sinks;
     const int* kv_len;     // keys of each batch item, or null
+};
+// The arguments of the tensor-core kernel with them.
+struct SdpaDevArgsWindow : SdpaDevArgs {
+    SdpaWindowArgs w;
 };
 cudaError_t launch_sdpa_window(const SdpaWindowArgs& a, int num_heads, int batch, bool bf16, cudaStream_t stream);
 

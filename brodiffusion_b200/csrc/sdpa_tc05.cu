@@ -46,7 +46,10 @@
 // Arithmetic follows the attention core of dit::joint_attention_traced
 // (src/dit/common.cpp:246-305): scale 1/sqrt(hd), stable softmax,
 // inv = denom > 0 ? 1/denom : 0, with FP32 scores and accumulation.
+#include <type_traits>
+
 #include "sdpa_internal.h"
+#include "sdpa_window.cuh"
 #include "tc05.cuh"
 
 namespace bdattn {
@@ -168,12 +171,16 @@ __device__ __forceinline__ void setmaxnreg_dec() {
 // k_full_ / v_full_ copies does, src/dit/qwenimage21_forward.cpp:606-645); the
 // softmax code does not change.
 // kMixed: some CTAs of the launch have one query tile (launch_t); without it every CTA has two.
-template <int HD, bool kBf16, int kHooks, bool kScale, bool kMixed>
+// kWindow: causal with a sliding window and visible first keys (sdpa_window.cuh).  A CTA visits the key tiles that
+// some row of it sees, those of the sinks and those of the window, and nothing between; a column that a row does not see is
+// hidden by its number in the tiles at the ends.  A weight of zero times a value that is not finite is NaN: rows that
+// come out so, though their weights are finite, are worked out again from the visible keys alone.
+template <int HD, bool kBf16, int kHooks, bool kScale, bool kMixed, bool kWindow = false>
 __global__ void __launch_bounds__(Roles<kScale>::kThreads, 1)
 sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant__ CUtensorMap tmQ1,
                  const __grid_constant__ CUtensorMap tmK0, const __grid_constant__ CUtensorMap tmK1,
                  const __grid_constant__ CUtensorMap tmV0, const __grid_constant__ CUtensorMap tmV1,
-                 const SdpaDevArgs a) {
+                 const __grid_constant__ std::conditional_t<kWindow, SdpaDevArgsWindow, SdpaDevArgs> a) {
     using C = Cfg<HD, kHooks == 3>;
     constexpr int KS = C::kKStages;
     constexpr int VS = C::kVStages;
@@ -227,7 +234,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
 
     // Key tiles this CTA has to visit.
     int n_kv = a.kv_tiles;
-    if (a.mask_mode == 1) {
+    if (!kWindow && a.mask_mode == 1) {
         const int last = q_global0 + min(n_t * kBM, seg_rows - qrow0) - 1;
         const int max_key = last + a.q_offset;
         int n = 0;
@@ -276,6 +283,23 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
     // barriers, tensor memory and descriptors are set up; from here on global memory is touched
     wait_for_prior_grid();
 
+    // The tiles of the sinks and of the window: the j-th of them is tile j, or j + skip from n_sink on.
+    int q_offset = a.q_offset, n_sink = 0, skip = 0;
+    if constexpr (kWindow) {
+        q_offset = window_keys(a.w.kv_len, batch, a.kv_rows[0] + a.kv_rows[1]) - a.lq_total;
+        const int first = q_global0 + q_offset;
+        const WindowSpan span = window_span(first, first + min(n_t * kBM, seg_rows - qrow0) - 1, a.w.window, a.w.sinks);
+        auto tile_of = [&](int key) { return key < a.kv_rows[0] ? key / kBN : a.kv_tiles0 + (key - a.kv_rows[0]) / kBN; };
+        n_sink = span.sink_end > 0 ? tile_of(span.sink_end - 1) + 1 : 0;
+        n_kv = n_sink;
+        if (span.win_end > 0) {
+            const int begin = max(n_sink, tile_of(span.win_begin)), end = tile_of(span.win_end - 1) + 1;
+            skip = begin - n_sink;
+            n_kv += max(0, end - begin);
+        }
+    }
+    auto raw_tile = [&](int j) { return kWindow && j >= n_sink ? j + skip : j; };
+
     // With a key mask, tiles without a visible key (the padding of a caption) are left out: they
     // would add nothing to any row.  The warps look at the tiles in turn, one load per lane
     // and 32 keys, and the flags become the list that all roles walk.  (512 text keys of
@@ -291,7 +315,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
     };
     bool listed = false;
     if constexpr (kHooks >= 1 && !kScale) {
-        if (a.key_mask != nullptr && n_kv <= kMaxListed) {
+        if (a.key_mask != nullptr && n_kv <= kMaxListed && (!kWindow || a.kv_tiles <= kPartTile)) {
             listed = true;
             if (warp == 9 && lane == 0) {      // the query tiles travel meanwhile
                 load_q(0);
@@ -300,7 +324,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             __syncwarp();
 #pragma unroll 2
             for (int t = warp; t < n_kv; t += Roles<kScale>::kThreads / 32) {
-                const TileInfo ti = kv_tile(a, t);
+                const TileInfo ti = kv_tile(a, raw_tile(t));
                 float mv[4];
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
@@ -323,7 +347,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
                 const bool on = f != 0;
                 const uint32_t m = __ballot_sync(0xffffffffu, on);
                 __syncthreads();
-                if (warp == 0 && on) tile_list[n + __popc(m & ((1u << lane) - 1u))] = static_cast<uint16_t>(t | (f & kPartTile));
+                if (warp == 0 && on) tile_list[n + __popc(m & ((1u << lane) - 1u))] = static_cast<uint16_t>(raw_tile(t) | (f & kPartTile));
                 n += __popc(m);
             }
             __syncthreads();
@@ -331,7 +355,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
         }
     }
     // the j-th key tile of this CTA
-    auto tile_at = [&](int j) { return kv_tile(a, listed ? tile_list[j] & (kPartTile - 1) : j); };
+    auto tile_at = [&](int j) { return kv_tile(a, listed ? tile_list[j] & (kPartTile - 1) : raw_tile(j)); };
 
     if (warp < 4 * n_t) {
         // ------------------------------------------------ softmax + epilogue
@@ -518,7 +542,14 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
                 }
             }
             int lim = ti.valid - 1;
-            if (a.mask_mode == 1) lim = min(lim, q_glob + a.q_offset - ti.kbase);
+            if (kWindow || a.mask_mode == 1) lim = min(lim, q_glob + q_offset - ti.kbase);
+            // columns [hide, hide + hidden) lie between the sinks and the window
+            uint32_t hide = 0, hidden = 0;
+            if constexpr (kWindow) {
+                hide = static_cast<uint32_t>(max(0, a.w.sinks - ti.kbase));
+                if (a.w.window > 0)
+                    hidden = static_cast<uint32_t>(max(0, q_glob + q_offset - a.w.window + 1 - ti.kbase - static_cast<int>(hide)));
+            }
             // A wait that runs out leaves `ok` false in its lane and the step goes on with
             // whatever is there; the vote on the row maximum below ends the loop for the
             // whole warp (one vote per step instead of one per wait).
@@ -579,7 +610,12 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
                 }
             }
             // (uniform over the CTA without the causal rule: no vote on whole tiles)
-            if (a.mask_mode == 1 ? __any_sync(0xffffffffu, lim < kBN - 1) : ti.valid < kBN) {
+            if constexpr (kWindow) {
+                if (__any_sync(0xffffffffu, lim < kBN - 1 || (hidden > 0 && hide < kBN))) {
+#pragma unroll
+                    for (int c = 0; c < kBN; ++c) s[c] = (c <= lim && c - hide >= hidden) ? s[c] : -INFINITY;
+                }
+            } else if (a.mask_mode == 1 ? __any_sync(0xffffffffu, lim < kBN - 1) : ti.valid < kBN) {
 #pragma unroll
                 for (int c = 0; c < kBN; ++c) s[c] = (c <= lim) ? s[c] : -INFINITY;
             }
@@ -702,6 +738,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
         // a CTA's 11700 outside the key steps.
         constexpr int kRowChunks = HD / 8;
         uint8_t* stg = smem_q + t * C::kQBytes;
+        bool spoiled = false;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
             uint32_t o[32];
@@ -711,6 +748,10 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = 0u;
+            }
+            if constexpr (kWindow) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) spoiled = spoiled || !(fabsf(__uint_as_float(o[i])) <= FLT_MAX);
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -769,6 +810,12 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
                                  : "memory");
                 }
             }
+        }
+        if constexpr (kWindow) {
+            uint32_t again = __ballot_sync(0xffffffffu, ok && spoiled && fabsf(l_sum) <= FLT_MAX && row_in_seg < seg_rows);
+            for (; again != 0; again &= again - 1)
+                window_row<kBf16>(a.w, batch, head, q_global0 + t * kBM + (warp & 3) * 32 + __ffs(again) - 1,
+                                  reinterpret_cast<float*>(stg + (warp & 3) * 32 * HD * 2), lane);
         }
     } else if (warp >= 8) {
         setmaxnreg_dec<Roles<kScale>::kRegsOther>();
@@ -966,7 +1013,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
     }
 }
 
-template <int HD, bool kBf16, int kHooks, bool kScale>
+template <int HD, bool kBf16, int kHooks, bool kScale, bool kWindow = false>
 cudaError_t launch_t(const SdpaLaunch& L, cudaStream_t stream) {
     using C = Cfg<HD, kHooks == 3>;
     // The CTAs of a last wave that fills no more than half of the SMs have one query tile each: a key step of
@@ -977,7 +1024,9 @@ cudaError_t launch_t(const SdpaLaunch& L, cudaStream_t stream) {
     // 40, 50.1 us against 53.1).
     const int sms = sm_count();
     const long long items = static_cast<long long>(L.q_ctas) * L.num_heads * L.batch, rest = items % sms;
-    SdpaDevArgs args = L.args;
+    std::conditional_t<kWindow, SdpaDevArgsWindow, SdpaDevArgs> args;
+    static_cast<SdpaDevArgs&>(args) = L.args;
+    if constexpr (kWindow) args.w = *L.window;
     args.q_ctas = L.q_ctas;
     args.num_heads = L.num_heads;
     args.whole_items = static_cast<int>(items - rest);
@@ -990,7 +1039,8 @@ cudaError_t launch_t(const SdpaLaunch& L, cudaStream_t stream) {
         return launch_dependent(kern, grid, dim3(Roles<kScale>::kThreads), C::kSmemBytes, stream, L.tmQ[0], L.tmQ[1], L.tmK[0],
                                 L.tmK[1], L.tmV[0], L.tmV[1], args);
     };
-    return mixed ? go(sdpa_tc05_kernel<HD, kBf16, kHooks, kScale, true>) : go(sdpa_tc05_kernel<HD, kBf16, kHooks, kScale, false>);
+    return mixed ? go(sdpa_tc05_kernel<HD, kBf16, kHooks, kScale, true, kWindow>)
+                 : go(sdpa_tc05_kernel<HD, kBf16, kHooks, kScale, false, kWindow>);
 }
 
 template <int HD, bool kBf16>
@@ -1000,6 +1050,8 @@ cudaError_t launch_hd(const SdpaLaunch& L, cudaStream_t stream) {
     // statistics 8.8 -> 8.1 at 344 tokens); 1: key mask only (the common case: padded captions; with the statistics'
     // store at its end 441 x 2365, 3 heads, takes 35.1 us instead of 32.9); 0: none.  The per-key scale vectors are
     // handled outside the softmax (kScale) and combine with 0, 2 and 3.
+    if (L.window != nullptr)
+        return L.args.key_mask != nullptr ? launch_t<HD, kBf16, 1, false, true>(L, stream) : launch_t<HD, kBf16, 0, false, true>(L, stream);
     const bool scale = L.args.key_scale != nullptr || L.args.val_scale != nullptr;
     if (L.args.bias != nullptr) {
         // A bias of few rows concerns a warp or two, and a piece of it behind the other through shared memory held up

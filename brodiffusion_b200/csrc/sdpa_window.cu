@@ -8,7 +8,7 @@ namespace {
 constexpr int kWinWarps = 8;
 
 template <bool kBf16>
-__global__ void __launch_bounds__(kWinWarps * 32) sdpa_window_kernel(const SdpaWindowArgs a) {
+__global__ void __launch_bounds__(kWinWarps * 32) sdpa_window_kernel(const __grid_constant__ SdpaWindowArgs a) {
     __shared__ float q_s[kWinWarps][256];
     wait_for_prior_grid();
     const int warp = warp_index(), lane = threadIdx.x & 31;

@@ -5,6 +5,7 @@
 // A row without a visible key gives zeros.
 #pragma once
 
+#include <cfloat>
 #include <cuda_fp16.h>
 
 #include "sdpa_internal.h"
