@@ -10,6 +10,9 @@ namespace {
 bool is_16bit(int dtype) { return dtype == BDATTN_BF16 || dtype == BDATTN_F16; }
 bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// Query rows that share a K/V head, up to which they go to the kernel for few rows.
+constexpr int kFewMost = 64;
+
 // The tensor-core attention kernel's arguments for a call with a window: head_dim <= 128.
 int window_launch(const char* op, bdattn::SdpaLaunch& L, const bdattn::SdpaWindowArgs& g, int num_heads, int num_kv_heads, int batch,
                   bool bf16) {
@@ -189,7 +192,19 @@ int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_para
     const bool bf16 = p->dtype == BDATTN_BF16;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (hd <= 128) {
+    if (hd <= 128 && p->n_q_seg == 1 && lq * g.kv_group <= kFewMost && nkv * ((lq * g.kv_group + 15) / 16) <= 65535) {
+        bdattn::SdpaFewLaunch L;
+        for (int s = 0; s < 2; ++s) {
+            const int k = s < p->n_kv_seg ? s : 0;
+            if (make_map_heads(op, &L.tmK[s], g.k[k], bf16, hd, nkv, g.kv_rows[k], p->batch, g.k_ld[k], g.k_bs[k], 64) ||
+                make_map_heads(op, &L.tmV[s], g.v[k], bf16, hd, nkv, g.kv_rows[k], p->batch, g.v_ld[k], g.v_bs[k], 64))
+                return -1;
+        }
+        L.args = g;
+        L.num_kv_heads = nkv;
+        L.batch = p->batch;
+        e = bdattn::launch_sdpa_few(L, bf16, st);
+    } else if (hd <= 128) {
         bdattn::SdpaLaunch L;
         if (window_launch(op, L, g, p->num_heads, nkv, p->batch, bf16)) return -1;
         e = bdattn::launch_sdpa_tc05(L, st);

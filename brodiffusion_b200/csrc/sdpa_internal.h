@@ -100,6 +100,13 @@ struct SdpaWindowArgs : SdpaGeneralArgs {
 struct SdpaDevArgsWindow : SdpaDevArgs {
     SdpaWindowArgs w;
 };
+// Few query rows: one query segment, head_dim <= 128, at most 65535 times num_kv_heads * row tiles of 16.
+struct SdpaFewLaunch {
+    CUtensorMap tmK[2], tmV[2];      // boxes of 64 key rows
+    SdpaWindowArgs args;
+    int num_kv_heads, batch;
+};
+cudaError_t launch_sdpa_few(const SdpaFewLaunch& L, bool bf16, cudaStream_t stream);
 cudaError_t launch_sdpa_window(const SdpaWindowArgs& a, int num_heads, int batch, bool bf16, cudaStream_t stream);
 
 // Head-averaged attention map of a query-row range x leading key range.
