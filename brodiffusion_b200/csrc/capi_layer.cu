@@ -10,6 +10,9 @@ namespace {
 bool is_16bit(int dtype) { return dtype == BDATTN_BF16 || dtype == BDATTN_F16; }
 bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// Rows up to which a product goes to the kernel for few rows.
+constexpr int kFewRowsMost = 16;
+
 // Query rows that share a K/V head, up to which they go to the kernel for few rows.
 constexpr int kFewMost = 64;
 
@@ -125,6 +128,10 @@ int bdattn_linear_act_fwd(const bdattn_linear_act_params* p, bdattn_stream_t str
     g.ldr = ldr;
     g.x_scale = p->x_scale;
     g.w_scale = p->w_scale;
+    if (p->M <= kFewRowsMost && !getenv("GF_OFF")) {
+        const cudaError_t e = bdattn::launch_gemm_few(L, p->x, ldx / half, reinterpret_cast<cudaStream_t>(stream));
+        return e != cudaSuccess ? cuda_fail(op, e) : 0;
+    }
     return launch_gemm(op, L, 1, reinterpret_cast<cudaStream_t>(stream));
 }
 

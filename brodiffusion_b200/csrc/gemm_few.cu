@@ -1,0 +1,165 @@
+// A layer's product (gemm_layer.cuh) for few rows: single tokens and small batches of them.
+//   C[m, n] = residual + gate * act(sum_k X[m, k] W[n, k] * scales + bias),  M <= 16
+// What such a call costs is reading W once, so the weights go from memory straight to registers, many 16-byte
+// loads in flight to a thread, and the products are mma.sync with sixteen rows of W as A and the (up to
+// eight, or two eights of) rows of X as B: an instruction for 512 bytes of weights, no shared memory on the way.
+// The order of K inside a product is free as long as both operands have the same: a lane's 16 bytes of
+// a row are its words of two products (of 16 values of 16 bits, or 32 of 8 bits), so nothing is rearranged.
+// The warps of a CTA share the K of sixteen rows in turns of 128 bytes, and where there are few rows of W a cluster of
+// CTAs does; the sums meet in shared memory.
+#include "gemm_layer.cuh"
+#include "sdpa_internal.h"
+#include "tc05.cuh"
+
+namespace bdattn {
+namespace {
+
+constexpr int kFewN = 16;              // rows of W to a CTA
+constexpr int kFewDepth = 3;           // turns of a warp in flight
+constexpr int kFewMaxParts = 8;
+
+template <bool kBf16, bool kFp8>
+__device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (kFp8) {
+        asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    } else {
+        const uint32_t a[4] = {a0, a1, a2, a3};
+        gen_mma<kBf16>(d, a, b0, b1);
+    }
+}
+// Weights are read once: they leave what is kept in L1 where it is.
+__device__ __forceinline__ uint4 load_stream(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+struct GemmFewArgs {
+    GemmProblem p;          // K and the strides of X and W in 16-bit units
+    const uint16_t* x;
+    const uint16_t* w;
+    long long ldx, ldw;
+    int parts;              // CTAs of a cluster
+};
+
+// NR: rows of X in eights.
+template <bool kBf16, bool kFp8, int W, int NR>
+__global__ void __launch_bounds__(W * 32)
+gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
+    __shared__ float sums[W][kFewN * 8 * NR];
+    __shared__ float parts_s[kFewMaxParts][kFewN * 8 * NR];
+    const GemmProblem& p = a.p;
+    const int warp = warp_index(), lane = threadIdx.x & 31;
+    const int part = a.parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int n0 = static_cast<int>(blockIdx.y) * kFewN;
+    const int g = lane >> 2, q = lane & 3;
+    const int turns = (p.K + 63) / 64, step = W * a.parts, first = part * W + warp;
+    const bool on[2] = {n0 + g < p.N, n0 + g + 8 < p.N};
+    const uint16_t* wrow[2] = {a.w + static_cast<long long>(n0 + (on[0] ? g : 0)) * a.ldw,
+                               a.w + static_cast<long long>(n0 + (on[1] ? g + 8 : 0)) * a.ldw};
+    if (a.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    dependents_may_launch();
+    // While the kernel before this one ends, the first weights come into the L2.
+#pragma unroll
+    for (int i = 0; i < kFewDepth; ++i) {
+        const int k = (first + i * step) * 64 + q * 16;
+        if (k < p.K && q < 4) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(wrow[0] + k));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(wrow[1] + k));
+        }
+    }
+    wait_for_prior_grid();
+
+    uint4 wv[kFewDepth][2][2], xv[kFewDepth][2][NR];
+    auto fetch = [&](int turn, uint4 (&w)[2][2], uint4 (&x)[2][NR]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int k = turn * 64 + s * 32 + q * 8;
+            const bool in = k < p.K;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[s][h] = in && on[h] ? load_stream(wrow[h] + k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+                x[s][r] = in && r * 8 + g < p.M ? __ldg(reinterpret_cast<const uint4*>(a.x + (r * 8 + g) * a.ldx + k)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    };
+    float acc[NR][4] = {};
+#pragma unroll
+    for (int i = 0; i < kFewDepth; ++i) fetch(first + i * step, wv[i], xv[i]);
+    for (int t = first; t < turns; t += kFewDepth * step) {
+#pragma unroll
+        for (int i = 0; i < kFewDepth; ++i) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    few_mma<kBf16, kFp8>(acc[r], wv[i][s][0].x, wv[i][s][1].x, wv[i][s][0].y, wv[i][s][1].y, xv[i][s][r].x, xv[i][s][r].y);
+                    few_mma<kBf16, kFp8>(acc[r], wv[i][s][0].z, wv[i][s][1].z, wv[i][s][0].w, wv[i][s][1].w, xv[i][s][r].z, xv[i][s][r].w);
+                }
+            }
+            fetch(t + (kFewDepth + i) * step, wv[i], xv[i]);      // (past the end: zeros, nothing is read)
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[warp][(r * 8 + q * 2 + (e & 1)) * kFewN + g + 8 * (e >> 1)] = acc[r][e];
+    }
+    __syncthreads();
+    if (a.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int i = threadIdx.x; i < kFewN * 8 * NR; i += W * 32) {
+        float f = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) f += sums[w][i];
+        if (a.parts > 1)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa(smem_u32(&parts_s[part][i]), 0)), "f"(f) : "memory");
+        else parts_s[0][i] = f;
+    }
+    // (the first CTA of a cluster finishes; without one a thread reads what it wrote itself)
+    if (a.parts > 1) cluster_sync();
+    if (part != 0) return;
+    for (int i = threadIdx.x; i < kFewN * 8 * NR; i += W * 32) {
+        const int m = i / kFewN, n = n0 + i % kFewN;
+        if (m >= p.M || n >= p.N) continue;
+        float f[1] = {0.0f};
+        for (int k = 0; k < a.parts; ++k) f[0] += parts_s[k][i];
+        if (kFp8) f[0] *= (p.x_scale != nullptr ? __ldg(p.x_scale + m) : 1.0f) * (p.w_scale != nullptr ? __ldg(p.w_scale + n) : 1.0f);
+        if (p.bias != nullptr) f[0] += layer_ld16<kBf16>(p.bias, n);
+        activate(f, p.act);
+        if (p.gate != nullptr) f[0] *= layer_ld16<kBf16>(p.gate, n);
+        if (p.residual != nullptr) f[0] += layer_ld16<kBf16>(p.residual, m * p.ldr + n);
+        store1<kBf16>(p.C, m * p.ldc + n, f[0]);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_gemm_few(const GemmLaunch& L, const void* x, long long ldx, cudaStream_t stream) {
+    GemmFewArgs a;
+    a.p = L.args.p[0];
+    a.x = reinterpret_cast<const uint16_t*>(x);
+    a.w = reinterpret_cast<const uint16_t*>(L.W[0]);
+    a.ldx = ldx;
+    a.ldw = L.ldw[0];
+    const int tiles = (a.p.N + kFewN - 1) / kFewN, turns = (a.p.K + 63) / 64;
+    int W = 4, parts = 1;
+    if (getenv("GF_W")) W = atoi(getenv("GF_W"));
+    if (getenv("GF_P")) parts = atoi(getenv("GF_P"));
+    (void)turns;
+    a.parts = parts;
+    auto go = [&](auto kern, int w) {
+        return launch_dependent_cluster(kern, dim3(parts, tiles), dim3(w * 32), 0, stream, dim3(parts), a);
+    };
+    auto pick = [&](auto b, auto f) {
+        constexpr bool kB = decltype(b)::value, kF = decltype(f)::value;
+        if (W == 8) return a.p.M <= 8 ? go(gemm_few_kernel<kB, kF, 8, 1>, 8) : go(gemm_few_kernel<kB, kF, 8, 2>, 8);
+        return a.p.M <= 8 ? go(gemm_few_kernel<kB, kF, 4, 1>, 4) : go(gemm_few_kernel<kB, kF, 4, 2>, 4);
+    };
+    if (L.fp8) return L.bf16 ? pick(std::true_type{}, std::true_type{}) : pick(std::false_type{}, std::true_type{});
+    return L.bf16 ? pick(std::true_type{}, std::false_type{}) : pick(std::false_type{}, std::false_type{});
+}
+
+}  // namespace bdattn

@@ -233,6 +233,9 @@ cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream);
 // problem of the launch must have whole tiles of that width.
 cudaError_t launch_gemm_pair(const GemmLaunch& L, int tile_cols, cudaStream_t stream);
 
+// A layer's product of at most 16 rows (one problem, L.layer).
+cudaError_t launch_gemm_few(const GemmLaunch& L, const void* x, long long ldx, cudaStream_t stream);
+
 // Residual addition + RMSNorm of rows (16-bit in; 16-bit or e4m3 out).
 struct AddRmsNormArgs {
     const void* x;
@@ -245,6 +248,7 @@ struct AddRmsNormArgs {
     int rows, cols;
     long long ldx, ldr, ldro, ldo;
     float eps;
+    int shift;                 // set by the launch: elements that x lies off 16 bytes
 };
 cudaError_t launch_add_rmsnorm(const AddRmsNormArgs& a, bool bf16, bool fp8, cudaStream_t stream);
 
