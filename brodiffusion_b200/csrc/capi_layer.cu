@@ -12,6 +12,7 @@ bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_
 
 // Rows up to which a product goes to the kernel for few rows.
 constexpr int kFewRowsMost = 16;
+constexpr int kFewColsMost = 16 * 65535;      // its grid
 
 // Query rows that share a K/V head, up to which they go to the kernel for few rows.
 constexpr int kFewMost = 64;
@@ -128,7 +129,7 @@ int bdattn_linear_act_fwd(const bdattn_linear_act_params* p, bdattn_stream_t str
     g.ldr = ldr;
     g.x_scale = p->x_scale;
     g.w_scale = p->w_scale;
-    if (p->M <= kFewRowsMost && !getenv("GF_OFF")) {
+    if (p->M <= kFewRowsMost && p->N <= kFewColsMost) {
         const cudaError_t e = bdattn::launch_gemm_few(L, p->x, ldx / half, reinterpret_cast<cudaStream_t>(stream));
         return e != cudaSuccess ? cuda_fail(op, e) : 0;
     }

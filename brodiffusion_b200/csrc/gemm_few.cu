@@ -15,7 +15,6 @@ namespace bdattn {
 namespace {
 
 constexpr int kFewN = 16;              // rows of W to a CTA
-constexpr int kFewDepth = 3;           // turns of a warp in flight
 constexpr int kFewMaxParts = 8;
 
 template <bool kBf16, bool kFp8>
@@ -45,9 +44,11 @@ struct GemmFewArgs {
     int parts;              // CTAs of a cluster
 };
 
-// NR: rows of X in eights.
-template <bool kBf16, bool kFp8, int W, int NR>
-__global__ void __launch_bounds__(W * 32)
+// W: warps.  NR: rows of X in eights.  kDepth: turns of a warp in flight.  kCtas: CTAs of an SM; what hides the latency
+// of memory are many warps with little in flight each (26 MB of weights, one row: 8 warps, two turns, three CTAs to an
+// SM 6.3 us; 4 warps, three turns 8.6; a plain read of as many bytes takes 5.5).
+template <bool kBf16, bool kFp8, int W, int NR, int kDepth, int kCtas>
+__global__ void __launch_bounds__(W * 32, kCtas)
 gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
     __shared__ float sums[W][kFewN * 8 * NR];
     __shared__ float parts_s[kFewMaxParts][kFewN * 8 * NR];
@@ -56,52 +57,77 @@ gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
     const int part = a.parts > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int n0 = static_cast<int>(blockIdx.y) * kFewN;
     const int g = lane >> 2, q = lane & 3;
-    const int turns = (p.K + 63) / 64, step = W * a.parts, first = part * W + warp;
-    const bool on[2] = {n0 + g < p.N, n0 + g + 8 < p.N};
-    const uint16_t* wrow[2] = {a.w + static_cast<long long>(n0 + (on[0] ? g : 0)) * a.ldw,
-                               a.w + static_cast<long long>(n0 + (on[1] ? g + 8 : 0)) * a.ldw};
+    const int step = W * a.parts, first = part * W + warp;
+    // Rows that do not exist are read as the last one that does: their sums go nowhere.
+    const uint16_t* wp[2] = {a.w + static_cast<long long>(min(n0 + g, p.N - 1)) * a.ldw + first * 64 + q * 8,
+                             a.w + static_cast<long long>(min(n0 + g + 8, p.N - 1)) * a.ldw + first * 64 + q * 8};
+    const uint16_t* xp[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) xp[r] = a.x + min(r * 8 + g, p.M - 1) * a.ldx + first * 64 + q * 8;
+    const int full = p.K / 64, n = first < full ? (full - first + step - 1) / step : 0;      // whole turns of this warp
+    const long long advance = static_cast<long long>(step) * 64;
     if (a.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     dependents_may_launch();
     // While the kernel before this one ends, the first weights come into the L2.
+    // While the kernel before this one ends, the first weights come into the L2.
+    if (lane < 16 && n > 0) {
+        const uint16_t* const at = a.w + static_cast<long long>(min(n0 + lane, p.N - 1)) * a.ldw + first * 64;
 #pragma unroll
-    for (int i = 0; i < kFewDepth; ++i) {
-        const int k = (first + i * step) * 64 + q * 16;
-        if (k < p.K && q < 4) {
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(wrow[0] + k));
-            asm volatile("prefetch.global.L2 [%0];" ::"l"(wrow[1] + k));
-        }
+        for (int i = 0; i < kDepth; ++i)
+            if (i < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + i * advance));
     }
     wait_for_prior_grid();
 
-    uint4 wv[kFewDepth][2][2], xv[kFewDepth][2][NR];
-    auto fetch = [&](int turn, uint4 (&w)[2][2], uint4 (&x)[2][NR]) {
+    uint4 wv[kDepth][2][2], xv[kDepth][2][NR];
+    auto fetch = [&](uint4 (&w)[2][2], uint4 (&x)[2][NR]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int k = turn * 64 + s * 32 + q * 8;
-            const bool in = k < p.K;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) w[s][h] = in && on[h] ? load_stream(wrow[h] + k) : make_uint4(0u, 0u, 0u, 0u);
+            for (int h = 0; h < 2; ++h) w[s][h] = load_stream(wp[h] + s * 32);
 #pragma unroll
-            for (int r = 0; r < NR; ++r)
-                x[s][r] = in && r * 8 + g < p.M ? __ldg(reinterpret_cast<const uint4*>(a.x + (r * 8 + g) * a.ldx + k)) : make_uint4(0u, 0u, 0u, 0u);
+            for (int r = 0; r < NR; ++r) x[s][r] = __ldg(reinterpret_cast<const uint4*>(xp[r] + s * 32));
         }
+        wp[0] += advance;
+        wp[1] += advance;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) xp[r] += advance;
     };
     float acc[NR][4] = {};
+    auto products = [&](const uint4 (&w)[2][2], const uint4 (&x)[2][NR]) {
 #pragma unroll
-    for (int i = 0; i < kFewDepth; ++i) fetch(first + i * step, wv[i], xv[i]);
-    for (int t = first; t < turns; t += kFewDepth * step) {
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int i = 0; i < kFewDepth; ++i) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-#pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    few_mma<kBf16, kFp8>(acc[r], wv[i][s][0].x, wv[i][s][1].x, wv[i][s][0].y, wv[i][s][1].y, xv[i][s][r].x, xv[i][s][r].y);
-                    few_mma<kBf16, kFp8>(acc[r], wv[i][s][0].z, wv[i][s][1].z, wv[i][s][0].w, wv[i][s][1].w, xv[i][s][r].z, xv[i][s][r].w);
-                }
+            for (int r = 0; r < NR; ++r) {
+                few_mma<kBf16, kFp8>(acc[r], w[s][0].x, w[s][1].x, w[s][0].y, w[s][1].y, x[s][r].x, x[s][r].y);
+                few_mma<kBf16, kFp8>(acc[r], w[s][0].z, w[s][1].z, w[s][0].w, w[s][1].w, x[s][r].z, x[s][r].w);
             }
-            fetch(t + (kFewDepth + i) * step, wv[i], xv[i]);      // (past the end: zeros, nothing is read)
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kDepth; ++i)
+        if (i < n) fetch(wv[i], xv[i]);
+    for (int t = 0; t < n; t += kDepth) {
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) {
+            if (t + i < n) {
+                products(wv[i], xv[i]);
+                if (t + i + kDepth < n) fetch(wv[i], xv[i]);
+            }
+        }
+    }
+    if (p.K % 64 != 0 && full % step == first) {
+        // the last columns, fewer than a turn's
+        uint4 w[2][2] = {}, x[2][NR] = {};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (full * 64 + s * 32 + q * 8 < p.K) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) w[s][h] = load_stream(wp[h] + s * 32);
+#pragma unroll
+                for (int r = 0; r < NR; ++r) x[s][r] = __ldg(reinterpret_cast<const uint4*>(xp[r] + s * 32));
+            }
+        }
+        products(w, x);
     }
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -145,18 +171,25 @@ cudaError_t launch_gemm_few(const GemmLaunch& L, const void* x, long long ldx, c
     a.ldx = ldx;
     a.ldw = L.ldw[0];
     const int tiles = (a.p.N + kFewN - 1) / kFewN, turns = (a.p.K + 63) / 64;
-    int W = 4, parts = 1;
-    if (getenv("GF_W")) W = atoi(getenv("GF_W"));
-    if (getenv("GF_P")) parts = atoi(getenv("GF_P"));
-    (void)turns;
+    // K over a cluster while all CTAs run at once, three to an SM, and a warp has two turns (2560 x 2560 4.6 us over two,
+    // 5.6 whole, 6.4 over four; 64 x 10240 3.4 over four, 6.8 whole; 1280 x 1280, 20 turns, 3.1 over two, 2.8 whole).
+    int parts = 1;
+    while (parts < kFewMaxParts && tiles * parts * 2 <= 3 * sm_count() && turns >= 32 * parts) parts *= 2;
     a.parts = parts;
-    auto go = [&](auto kern, int w) {
-        return launch_dependent_cluster(kern, dim3(parts, tiles), dim3(w * 32), 0, stream, dim3(parts), a);
+    auto go = [&](auto kern, int warps) {
+        return launch_dependent_cluster(kern, dim3(parts, tiles), dim3(warps * 32), 0, stream, dim3(parts), a);
     };
+    // More CTAs than that: with a short K five of four warps to an SM (10240 x 1280 words 6.3 us, eight warps 7.9), else
+    // four of eight warps with one turn in flight (8 rows x 10240 x 2560 9.4 us, 12.5 with two turns, 10.8 with four
+    // warps; 20480 x 5120 31.9, 34.0 and 38.4).  Two eights of rows have no registers for more than one turn (16 x 5120 x 5120 in 8
+    // bits 8.6 us, 16.3 with two; 16 x 20480 x 5120 38.5 with three CTAs, 44.1 with four).
+    const bool many = tiles > 3 * sm_count(), brief = many && turns < 32;
     auto pick = [&](auto b, auto f) {
         constexpr bool kB = decltype(b)::value, kF = decltype(f)::value;
-        if (W == 8) return a.p.M <= 8 ? go(gemm_few_kernel<kB, kF, 8, 1>, 8) : go(gemm_few_kernel<kB, kF, 8, 2>, 8);
-        return a.p.M <= 8 ? go(gemm_few_kernel<kB, kF, 4, 1>, 4) : go(gemm_few_kernel<kB, kF, 4, 2>, 4);
+        if (a.p.M <= 8)
+            return brief ? go(gemm_few_kernel<kB, kF, 4, 1, 2, 5>, 4) : many ? go(gemm_few_kernel<kB, kF, 8, 1, 1, 4>, 8)
+                                                                             : go(gemm_few_kernel<kB, kF, 8, 1, 2, 3>, 8);
+        return brief ? go(gemm_few_kernel<kB, kF, 4, 2, 1, 5>, 4) : go(gemm_few_kernel<kB, kF, 8, 2, 1, 3>, 8);
     };
     if (L.fp8) return L.bf16 ? pick(std::true_type{}, std::true_type{}) : pick(std::false_type{}, std::true_type{});
     return L.bf16 ? pick(std::true_type{}, std::false_type{}) : pick(std::false_type{}, std::false_type{});
