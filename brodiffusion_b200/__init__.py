@@ -25,7 +25,7 @@ __all__ = [
     "linear_act_fwd",
 ]
 
-F32, F16, BF16, E4M3 = 0, 1, 2, 3
+F32, F16, BF16, E4M3 = 0, 1, 2, 16
 MASK_NONE, MASK_CAUSAL = 0, 1
 STATUS_WAIT_TIMEOUT, STATUS_BAD_ARGS = 1, 2
 ROPE_INTERLEAVED, ROPE_HALF_SPLIT = 0, 1

@@ -33,7 +33,7 @@ typedef struct CUstream_st* bdattn_stream_t; /* == cudaStream_t */
 
 /* Element types; values follow brotensor::Dtype order as used by the callers
  * (FP32, FP16, BF16). */
-enum { BDATTN_F32 = 0, BDATTN_F16 = 1, BDATTN_BF16 = 2, BDATTN_E4M3 = 3 /* 8 bits, no infinity, largest 448 */ };
+enum { BDATTN_F32 = 0, BDATTN_F16 = 1, BDATTN_BF16 = 2, BDATTN_E4M3 = 16 /* 8 bits, no infinity, largest 448; no brotensor type */ };
 
 /* Attention visibility rules. */
 enum {

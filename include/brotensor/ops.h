@@ -42,11 +42,27 @@ inline void flash_attention_forward(const Tensor& Q, const Tensor& K, const Tens
     detail::bd_check(bdattn_sdpa_fwd(&p, detail::bd_stream()));
 }
 
-// src/dit/qwenimage21_forward.cpp:662 — window 0: unbounded causal with q_offset = Lk - Lq
+// src/dit/qwenimage21_forward.cpp:662 — window 0: unbounded causal with q_offset = Lk - Lq; otherwise the last
+// `window` keys up to the query's own position
 inline void flash_attention_windowed_forward(const Tensor& Q, const Tensor& K, const Tensor& V,
                                              const float* d_mask, int num_heads, int window, Tensor& O) {
-    if (window != 0) throw std::runtime_error("flash_attention_windowed_forward: only window = 0 is supported");
-    flash_attention_forward(Q, K, V, d_mask, num_heads, /*causal=*/true, O);
+    if (window == 0) {
+        flash_attention_forward(Q, K, V, d_mask, num_heads, /*causal=*/true, O);
+        return;
+    }
+    detail::require_gpu(Q, "flash_attention_windowed_forward");
+    if (num_heads <= 0 || Q.cols % num_heads != 0 || K.cols != Q.cols || V.cols != Q.cols || K.rows != V.rows)
+        throw std::runtime_error("flash_attention_windowed_forward: Q/K/V shapes do not agree with num_heads");
+    O.resize(Q.rows, Q.cols, Q.dtype);
+    bdattn_sdpa_params p{};
+    p.dtype = detail::bd_dtype(Q.dtype);
+    p.batch = 1; p.num_heads = num_heads; p.head_dim = Q.cols / num_heads;
+    p.n_q_seg = 1; p.q[0] = Q.data; p.o[0] = O.data; p.q_rows[0] = Q.rows; p.q_ld[0] = Q.cols; p.o_ld[0] = O.cols;
+    p.n_kv_seg = 1; p.k[0] = K.data; p.v[0] = V.data; p.kv_rows[0] = K.rows; p.k_ld[0] = K.cols; p.v_ld[0] = V.cols;
+    p.mask_mode = BDATTN_MASK_CAUSAL;
+    p.key_mask = d_mask;
+    const bdattn_window_params w{window, 0, nullptr};
+    detail::bd_check(bdattn_sdpa_window_fwd(&p, &w, detail::bd_stream()));
 }
 
 // src/dit/common.cpp:192-193, src/dit/qwenimage21_forward.cpp:584-585
