@@ -53,7 +53,8 @@ constexpr int kPGroup = 16;                   // row blocks of a group
 // 128 rows of A and two of its kN / 2 weight rows.
 template <int kN>
 struct PairCfg {
-    static constexpr int kStages = kN == 256 ? 3 : 4;
+    static constexpr int kStages = kN == 128 ? 4 : 3;
+    static constexpr int kTmemCols = kN == 128 ? 256 : 512;       // two accumulators, a power of two
     static constexpr int kBChunk = kN / 2 * 64 * 2;
     static constexpr int kStageBytes = 2 * kPChunk + 2 * kBChunk;
     static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kPStgBytes + 256 + 3 * 128 * 4 + 1024;
@@ -271,7 +272,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc_pair(tmem_slot, 2 * kN);
+        tmem_alloc_pair(tmem_slot, C::kTmemCols);
         tmem_relinquish_pair();
     }
     // The first tile of this pair: found before the wait for the kernel before this one, so that the first
@@ -369,7 +370,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                 if (!ok) break;
                 tc_fence_after();
             }
-            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(as * kN);
+            const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(as * (C::kTmemCols / 2));
             for (int c = 0; c < chunks; c += 2) {
                 ok = mbar_wait_warp(&full[slot], phase);
                 if (!ok) break;
@@ -426,14 +427,18 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
             ResidualPiece res;
             const uint16_t* res0 = nullptr;
             float x_scale = 1.0f;
+            // a layer's columns of this warp: whole 32s, the first half of the warps takes one more where they are odd
+            constexpr int kSplit = (kN + 63) / 64 * 32;
+            const int l_begin = half * kSplit, l_end = half ? kN : kSplit;
             if constexpr (kEpi == kEpiLayer) {
                 // what the columns, the rows and the first piece of the residual have, while the tile is computed
 #pragma unroll
-                for (int e = 0; e < 128; e += 32) layer_columns<kBf16>(p, bias_w, 128, e + lane, t.n0 + c_base + e + lane, true);
+                for (int e = 0; e < 128; e += 32)
+                    layer_columns<kBf16>(p, bias_w, 128, e + lane, t.n0 + l_begin + e + lane, l_begin + e < l_end);
                 if (rows > 0) {
                     if (p.residual != nullptr) {
                         res0 = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<long long>(row0) * p.ldr + t.n0;
-                        res.load(res0 + c_base + c_own, p.ldr, rows, 32, lane);
+                        res.load(res0 + l_begin, p.ldr, rows, 32, lane);
                     }
                     if (kFp8 && p.x_scale != nullptr && lane < rows) x_scale = __ldg(p.x_scale + row0 + lane);
                 }
@@ -457,7 +462,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&acc_full[as], static_cast<uint32_t>((ti >> 1) & 1)));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(as * kN);
+            const uint32_t tacc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(as * (C::kTmemCols / 2));
             uint16_t* cbase = reinterpret_cast<uint16_t*>(p.C) + static_cast<long long>(row0) * p.ldc + t.n0;
             if (rows <= 0) {
                 // rows past the matrix: nothing to store
@@ -492,16 +497,16 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                 }
             } else if (kEpi == kEpiLayer) {
 #pragma unroll 1
-                for (int c = c_base + c_own; c < c_base + c_own + C::kHalf; c += 32) {
+                for (int c = l_begin; c < l_end; c += 32) {
                     uint32_t w[16] = {};
                     if (res0 != nullptr) {
                         res.row_of_lane(stg, lane, w);
-                        if (c + 32 < c_base + c_own + C::kHalf) res.load(res0 + c + 32, p.ldr, rows, 32, lane);
+                        if (c + 32 < l_end) res.load(res0 + c + 32, p.ldr, rows, 32, lane);
                     }
                     float f[32];
                     tmem_ld32(tacc + c, *reinterpret_cast<uint32_t(*)[32]>(&f[0]));
                     tmem_wait_ld();
-                    layer_values<kBf16, kFp8>(p, f, bias_w + (c - c_base), 128, x_scale, w);
+                    layer_values<kBf16, kFp8>(p, f, bias_w + (c - l_begin), 128, x_scale, w);
                     store_tile32<kBf16>(f, stg, lane, cbase + c, p.ldc, rows, 32);
                 }
             } else {
@@ -530,7 +535,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
     cluster_sync_relaxed();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem_base, 2 * kN);
+        tmem_dealloc_pair(tmem_base, C::kTmemCols);
     }
 }
 
@@ -556,15 +561,28 @@ static cudaError_t launch_gemm_pair_n(const GemmLaunch& L, cudaStream_t stream) 
         heads = heads || L.args.p[i].norm_rope;
     }
     if ((geglu && heads) || (L.layer && (geglu || heads))) return cudaErrorInvalidValue;        // no entry point asks for both
+    // a layer has the widths between 128 and 256 too
+    if constexpr (kN != 128 && kN != 256) {
+        if (!L.layer) return cudaErrorInvalidValue;
+        if (L.fp8) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiLayer, true>) : go(gemm_pair_kernel<false, kN, kEpiLayer, true>);
+        return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiLayer>) : go(gemm_pair_kernel<false, kN, kEpiLayer>);
+    } else {
     if (L.layer && L.fp8) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiLayer, true>) : go(gemm_pair_kernel<false, kN, kEpiLayer, true>);
     if (L.layer) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiLayer>) : go(gemm_pair_kernel<false, kN, kEpiLayer>);
     if (geglu) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiGeglu>) : go(gemm_pair_kernel<false, kN, kEpiGeglu>);
     if (heads) return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiHeads>) : go(gemm_pair_kernel<false, kN, kEpiHeads>);
     return L.bf16 ? go(gemm_pair_kernel<true, kN, kEpiPlain>) : go(gemm_pair_kernel<false, kN, kEpiPlain>);
+    }
 }
 
 cudaError_t launch_gemm_pair(const GemmLaunch& L, int tile_cols, cudaStream_t stream) {
-    return tile_cols == 128 ? launch_gemm_pair_n<128>(L, stream) : launch_gemm_pair_n<256>(L, stream);
+    switch (tile_cols) {
+        case 128: return launch_gemm_pair_n<128>(L, stream);
+        case 160: return launch_gemm_pair_n<160>(L, stream);
+        case 192: return launch_gemm_pair_n<192>(L, stream);
+        case 224: return launch_gemm_pair_n<224>(L, stream);
+        default: return launch_gemm_pair_n<256>(L, stream);
+    }
 }
 
 }  // namespace bdattn

@@ -78,7 +78,7 @@ BDATTN_HD constexpr bool pair_acc_reused(int tile, int pairs, int total_tiles) {
 // The problems of a launch may differ in K (the queries and the keys of a cross-attention): the
 // longest sets the time, the shortest how far its tiles can be split, a CTA without a K
 // block would have nothing to add and nothing to wait for.
-inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms) {
+inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, bool layer = false) {
     bool geglu = false, heads = false, odd = false;
     int kb = 0, kb_min = 0, m_max = 0;
     for (int i = 0; i < n; ++i) {
@@ -181,6 +181,13 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms) {
             offer({true, 64, 1, 128}, heads ? 3.7 + 0.06 * f + x * (4.0 + 0.165 * f) : geglu ? 1.9 + 0.02 * f + x * (2.1 + 0.147 * f)
                                                                                      : 1.45 + 0.06 * f + x * (2.04 + 0.143 * f));
         }
+    }
+    // A layer's tiles (gemm_layer.cuh) come in widths between these too, where they fill the pairs better; the times lie between.
+    for (int cols = 160; layer && cols < 256; cols += 32) {
+        if (p[0].N % cols != 0) continue;
+        const double x = rounds(static_cast<long long>(gemm_pair_row_tiles(gemm_row_tiles(p[0].M))) * (p[0].N / cols), sms / 2);
+        const double u = (cols - 128) / 128.0, f = odd ? (1.35 - 0.2 * u) * kb : kb;
+        offer({true, 64, 1, cols}, 1.45 + 2.3 * u + 0.06 * f + x * (2.04 + 0.46 * u + (0.143 + 0.085 * u) * f));
     }
     return best;
 }
