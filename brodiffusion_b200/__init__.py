@@ -647,19 +647,6 @@ def qkv_norm_rope_fwd(x, wq, wk, wv, q_out, k_out, v_out, num_heads, head_dim, *
     _check(lib().packed_qkv_norm_rope_fwd(p, _stream(stream)))
 
 
-def _matrix(t, what, shape=None):
-    """(pointer, ld) of a 2-D tensor with contiguous columns (a single row or column may have any stride)."""
-    sh, st = t.shape, t.stride()
-    if len(st) != 2:
-        raise BdattnError(f"{what} must be a 2-D tensor")
-    if shape is not None and sh != shape:
-        raise BdattnError(f"{what} has shape {tuple(sh)}, expected {tuple(shape)}")
-    rows, cols = sh
-    if st[1] != 1 and cols > 1:
-        raise BdattnError(f"{what} must have contiguous columns")
-    return t.data_ptr(), st[0] if rows > 1 else cols
-
-
 def _int32(t, what):
     """Pointer of an INT32 tensor."""
     if _torch is None:
@@ -681,28 +668,40 @@ def _vector(t, n, what):
 def add_rmsnorm_fwd(x, out, gain=None, *, residual=None, residual_out=None, out_scale=None, eps=1e-6, stream=None):
     """``bdattn_add_rmsnorm_fwd``: h = x (+ residual), residual_out = h, out = rmsnorm(h) * gain; with a
     ``torch.float8_e4m3fn`` out, out_scale (rows, FP32) receives the rows' scales."""
-    xp, x_ld = _matrix(x, "x")
-    shape = x.shape
-    op, o_ld = _matrix(out, "out", shape)
-    dtype, out_dtype = _dtype_code(x), _dtype_code(out)
-    rp = r_ld = rop = ro_ld = 0
+    # (written out: helpers for each tensor took 4 of the call's 7 us)
+    shape, st, ot = x.shape, x.stride(), out.stride()
+    if len(shape) != 2 or out.shape != shape:
+        raise BdattnError("x and out must be 2-D tensors of the same shape")
+    rows, cols = shape
+    if cols > 1 and (st[1] != 1 or ot[1] != 1):
+        raise BdattnError("tensor columns must be contiguous")
+    x_dtype = x.dtype
+    rp = r_ld = rop = ro_ld = gp = sp = 0
+    g_code = F32
     if residual is not None:
-        rp, r_ld = _matrix(residual, "residual", shape)
-        if residual.dtype != x.dtype:
-            raise BdattnError("residual must have the dtype of x")
+        rp, rt = residual.data_ptr(), residual.stride()
+        r_ld = rt[0] if rows > 1 else cols
+        if residual.shape != shape or residual.dtype is not x_dtype or (cols > 1 and rt[1] != 1):
+            raise BdattnError("residual must have the shape and dtype of x, with contiguous columns")
     if residual_out is not None:
-        rop, ro_ld = _matrix(residual_out, "residual_out", shape)
-        if residual_out.dtype != x.dtype:
-            raise BdattnError("residual_out must have the dtype of x")
-    if out_scale is not None and _dtype_code(out_scale) != F32:
-        raise BdattnError("out_scale must be FP32")
+        rop, rt = residual_out.data_ptr(), residual_out.stride()
+        ro_ld = rt[0] if rows > 1 else cols
+        if residual_out.shape != shape or residual_out.dtype is not x_dtype or (cols > 1 and rt[1] != 1):
+            raise BdattnError("residual_out must have the shape and dtype of x, with contiguous columns")
+    if gain is not None:
+        gp, g_code = _vector(gain, cols, "gain"), _dtype_code(gain)
+    if out_scale is not None:
+        if _dtype_code(out_scale) != F32:
+            raise BdattnError("out_scale must be FP32")
+        sp = _vector(out_scale, rows, "out_scale")
     try:
-        p = _pack_add_rmsnorm(dtype, shape[0], shape[1], xp, rp, rop, _vector(gain, shape[1], "gain"),
-                              _dtype_code(gain) if gain is not None else F32, op, out_dtype,
-                              _vector(out_scale, shape[0], "out_scale"), x_ld, r_ld, ro_ld, o_ld, _f32(eps))
+        p = _pack_add_rmsnorm(_dtype_code(x), rows, cols, x.data_ptr(), rp, rop, gp, g_code, out.data_ptr(), _dtype_code(out), sp,
+                              st[0] if rows > 1 else cols, r_ld, ro_ld, ot[0] if rows > 1 else cols,
+                              eps if eps == 1e-6 else _f32(eps))
     except struct.error as e:
         raise TypeError(str(e)) from None
-    _check(lib().packed_add_rmsnorm_fwd(p, _stream(stream)))
+    if lib().packed_add_rmsnorm_fwd(p, _stream(stream)):
+        raise BdattnError(last_error())
 
 
 def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, num_kv_heads=0, key_mask=None,
@@ -723,6 +722,8 @@ def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, nu
             for t in x:
                 if t.dtype is not first.dtype or _rows2d(t)[4] != batch:
                     raise BdattnError("q, k, v and out must have the same dtype and batch")
+                if batch > 1 and t.stride()[0] == 0:
+                    raise BdattnError("a tensor's batch items must not be the same memory")
                 if t.shape[-1] * num_heads != first.shape[-1] * heads:
                     raise BdattnError("q and out must have num_heads, k and v num_kv_heads heads of the same width")
         if kv_len is not None:
@@ -732,31 +733,45 @@ def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, nu
         sdpa_fwd(q, k, v, out, num_heads, mask_mode=MASK_CAUSAL, key_mask=key_mask, softmax_scale=softmax_scale,
                  num_kv_heads=num_kv_heads, stream=stream, _window=w)
         return
-    # one segment each, the usual call of a decoding step, without the lists: 7.2 -> 5.5 us of Python
-    qp, lq, q_ld, q_bs, batch = _rows2d(q)
-    kp, lk, k_ld, k_bs, kb = _rows2d(k)
-    vp, lv, v_ld, v_bs, vb = _rows2d(v)
-    op, lo, o_ld, o_bs, ob = _rows2d(out)
+    # one segment each, the usual call of a decoding step, without the lists
+    qs, qt, ks, kt, vt, ot = q.shape, q.stride(), k.shape, k.stride(), v.stride(), out.stride()
+    if out.shape != qs or v.shape != ks:
+        raise BdattnError("out must have the shape of q and v that of k")
+    if len(qs) == 3 and len(ks) == 3:
+        batch, lq, cols = qs
+        kb, lk, kv_cols = ks
+        q_bs, q_ld, q1 = qt
+        k_bs, k_ld, k1 = kt
+        v_bs, v_ld, v1 = vt
+        o_bs, o_ld, o1 = ot
+        if batch > 1 and not (q_bs and k_bs and v_bs and o_bs):         # (the library takes 0 for dense items)
+            raise BdattnError("a tensor's batch items must not be the same memory")
+    elif len(qs) == 2 and len(ks) == 2:
+        batch = kb = 1
+        q_bs = k_bs = v_bs = o_bs = 0
+        (lq, cols), (lk, kv_cols) = qs, ks
+        (q_ld, q1), (k_ld, k1), (v_ld, v1), (o_ld, o1) = qt, kt, vt, ot
+    else:
+        raise BdattnError("expected 2-D or 3-D tensors")
+    if not q1 == k1 == v1 == o1 == 1:
+        raise BdattnError("tensor columns must be contiguous")
     dtype = q.dtype
-    if k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or not kb == vb == ob == batch:
+    if k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or kb != batch:
         raise BdattnError("q, k, v and out must have the same dtype and batch")
-    if lo != lq or lv != lk:
-        raise BdattnError("out must have the rows of q and v those of k")
-    cols, kv_cols = q.shape[-1], k.shape[-1]
-    if (out.shape[-1] != cols or v.shape[-1] != kv_cols or cols % num_heads or
-            kv_cols * num_heads != cols * (num_kv_heads or num_heads)):
+    if cols % num_heads or kv_cols * num_heads != cols * (num_kv_heads or num_heads):
         raise BdattnError("q and out must have num_heads, k and v num_kv_heads heads of the same width")
     if kv_len is not None:
         _vector(kv_len, batch, "kv_len")
     try:
         p = _pack_sdpa(_dtype_code(q), batch, num_heads, cols // num_heads,
-                       1, qp, 0, op, 0, lq, 0, q_ld, 0, o_ld, 0, q_bs, 0, o_bs, 0,
-                       1, kp, 0, vp, 0, lk, 0, k_ld, 0, v_ld, 0, k_bs, 0, v_bs, 0,
+                       1, q.data_ptr(), 0, out.data_ptr(), 0, lq, 0, q_ld, 0, o_ld, 0, q_bs, 0, o_bs, 0,
+                       1, k.data_ptr(), 0, v.data_ptr(), 0, lk, 0, k_ld, 0, v_ld, 0, k_bs, 0, v_bs, 0,
                        MASK_CAUSAL, _vector(key_mask, lk, "key_mask"), 0, 0, softmax_scale and _f32(softmax_scale), num_kv_heads,
                        0, 0, 0, 0.0, 0, 0, 0)
     except struct.error as e:
         raise TypeError(str(e)) from None
-    _check(lib().packed_sdpa_window_fwd(p, w, _stream(stream)))
+    if lib().packed_sdpa_window_fwd(p, w, _stream(stream)):
+        raise BdattnError(last_error())
 
 
 ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
@@ -765,36 +780,43 @@ ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
 def linear_act_fwd(x, w, bias, y, *, act="none", gate=None, residual=None, x_scale=None, w_scale=None, stream=None):
     """``bdattn_linear_act_fwd``: y = residual + gate * act((x @ w.T) * x_scale[:, None] * w_scale + bias); x and w of
     the type of y, or both ``torch.float8_e4m3fn`` with FP32 scales per row.  act: a key of ``ACTIVATIONS``."""
-    xp, x_ld = _matrix(x, "x")
-    wp, w_ld = _matrix(w, "w")
-    (M, K), (N, Kw) = x.shape, w.shape
-    if Kw != K:
-        raise BdattnError(f"w has {Kw} columns, x {K}")
-    shape = (M, N)
-    yp, y_ld = _matrix(y, "y", shape)
+    xs, ws, ys = x.shape, w.shape, y.shape
+    xt, wt, yt = x.stride(), w.stride(), y.stride()
+    if len(xs) != 2 or len(ws) != 2 or ws[1] != xs[1] or ys != (xs[0], ws[0]):
+        raise BdattnError(f"x (M, K), w (N, K) and y (M, N) do not fit: {tuple(xs)}, {tuple(ws)} and {tuple(ys)}")
+    M, K = xs
+    N = ws[0]
+    if (xt[1] != 1 or wt[1] != 1) and K > 1 or yt[1] != 1 and N > 1:
+        raise BdattnError("tensor columns must be contiguous")
     dtype = y.dtype
     if w.dtype is not x.dtype:
         raise BdattnError("x and w must have the same dtype")
-    rp = r_ld = bp = gp = xs = ws = 0
+    rp = r_ld = bp = gp = xp = wp = 0
     if residual is not None:
-        rp, r_ld = _matrix(residual, "residual", shape)
-    for t in (bias, gate, residual):
-        if t is not None and t.dtype is not dtype:
-            raise BdattnError("bias, gate and residual must have the dtype of y")
-    for t in (x_scale, w_scale):
-        if t is not None and _dtype_code(t) != F32:
-            raise BdattnError("x_scale and w_scale must be FP32")
+        rp, rt = residual.data_ptr(), residual.stride()
+        r_ld = rt[0] if M > 1 else N
+        if residual.shape != ys or residual.dtype is not dtype or (N > 1 and rt[1] != 1):
+            raise BdattnError("residual must have the shape and dtype of y, with contiguous columns")
     if bias is not None:
         bp = _vector(bias, N, "bias")
+        if bias.dtype is not dtype:
+            raise BdattnError("bias must have the dtype of y")
     if gate is not None:
         gp = _vector(gate, N, "gate")
+        if gate.dtype is not dtype:
+            raise BdattnError("gate must have the dtype of y")
     if x_scale is not None:
-        xs = _vector(x_scale, M, "x_scale")
+        xp = _vector(x_scale, M, "x_scale")
+        if _dtype_code(x_scale) != F32:
+            raise BdattnError("x_scale must be FP32")
     if w_scale is not None:
-        ws = _vector(w_scale, N, "w_scale")
+        wp = _vector(w_scale, N, "w_scale")
+        if _dtype_code(w_scale) != F32:
+            raise BdattnError("w_scale must be FP32")
     code = ACTIVATIONS.get(act)
     if code is None:
         raise BdattnError(f"unknown activation {act!r} (one of {', '.join(ACTIVATIONS)})")
-    _check(lib().packed_linear_act_fwd(
-        _pack_linear_act(_dtype_code(y), _dtype_code(x), M, N, K, xp, wp, bp, gp, rp, yp, xs, ws, code, x_ld, w_ld, r_ld, y_ld),
-        _stream(stream)))
+    p = _pack_linear_act(_dtype_code(y), _dtype_code(x), M, N, K, x.data_ptr(), w.data_ptr(), bp, gp, rp, y.data_ptr(), xp, wp, code,
+                         xt[0] if M > 1 else K, wt[0] if N > 1 else K, r_ld, yt[0] if M > 1 else N)
+    if lib().packed_linear_act_fwd(p, _stream(stream)):
+        raise BdattnError(last_error())

@@ -158,8 +158,11 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, bool layer = false
         for (int s = 2; s <= 8 && kb >= 3 * s && kb_min >= s && tiles(64) * s * 2 <= 3LL * sms; s *= 2) {
             // (with more CTAs than SMs a longer part of K costs more than the split saves, and of tiles with more than 64 rows
             // any: 135 x 640 x 5120 over eight 11.5 us, over four 8.0, and the same for 100 shapes drawn at random)
-            if (waves(64, s) <= 1.0) offer({false, 64, s}, 3.15 + 0.15 * kb / s);
-            else if (kb <= 12 * s && m_max <= 64) offer({false, 64, s}, 3.22 + 0.27 * kb / s * tiles(64) * s / sms);
+            // (a layer's are entered at what they take: 333 x 1288 x 648 6.4 us whole, 7.2 over two; 128 x 2560 x 2560 9.8 and 10.7;
+            // 17 x 2560 x 10240 27.1 and 17.4)
+            const double more = layer ? 0.8 : 0.0;
+            if (waves(64, s) <= 1.0) offer({false, 64, s}, 3.15 + more + 0.15 * kb / s);
+            else if (kb <= 12 * s && m_max <= 64) offer({false, 64, s}, 3.22 + more + 0.27 * kb / s * tiles(64) * s / sms);
         }
     }
     for (int cols = 256; cols >= 128; cols /= 2) {
@@ -182,7 +185,9 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, bool layer = false
                                                                                      : 1.45 + 0.06 * f + x * (2.04 + 0.143 * f));
         }
     }
-    // A layer's tiles (gemm_layer.cuh) come in widths between these too, where they fill the pairs better; the times lie between.
+    // A layer's tiles (gemm_layer.cuh) come in widths between these too, where they fill the pairs better; the times lie between
+    // (128, 160, 192, 224 and 256 columns: 2166 x 2560 x 10240 96, 90, -, -, 109 us, 1024 x 2560 x 2560 19.9, 15.8, -, -, 20.8, 1500 x
+    // 2304 x 2240 18.9, -, 16.6, -, 19.2, 2048 x 2240 x 2240 -, 24.2, -, 27.0, -, 3000 x 1920 x 2560 28.1, 26.0, 27.4, -, -).
     for (int cols = 160; layer && cols < 256; cols += 32) {
         if (p[0].N % cols != 0) continue;
         const double x = rounds(static_cast<long long>(gemm_pair_row_tiles(gemm_row_tiles(p[0].M))) * (p[0].N / cols), sms / 2);

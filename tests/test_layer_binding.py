@@ -77,7 +77,9 @@ def test_shapes_that_do_not_fit_are_refused_before_any_launch():
                  lambda: bd.sdpa_window_fwd(q, [k, k[:, :, :32]], [k, k], q, 2, **good),
                  lambda: bd.sdpa_window_fwd(q, k, k, q, 2, kv_len=torch.zeros(2), **good),
                  lambda: bd.sdpa_window_fwd(q, k, k, q, 2, kv_len=torch.zeros(3, dtype=torch.int32), **good),
-                 lambda: bd.sdpa_window_fwd(q, k, k, q, 2, key_mask=torch.zeros(8), **good)):
+                 lambda: bd.sdpa_window_fwd(q, k, k, q, 2, key_mask=torch.zeros(8), **good),
+                 lambda: bd.sdpa_window_fwd(q, k[:1].expand(2, 9, 64), k, q, 2, **good),         # one sequence's rows for two
+                 lambda: bd.sdpa_window_fwd([q], [k[:1].expand(2, 9, 64)], [k], [q], 2, **good)):
         with pytest.raises(bd.BdattnError):
             call()
     for w in (2.0, "4", None):
