@@ -182,7 +182,7 @@ int launch_gemm(const char* op, bdattn::GemmLaunch& L, int n, cudaStream_t strea
         const bdattn::GemmProblem& p = L.args.p[i];
         shapes[i] = {p.M, p.N, p.K, p.geglu_offset > 0, p.norm_rope != 0, L.whole[i]};
     }
-    const bdattn::GemmPlan plan = bdattn::plan_gemm(shapes, n, bdattn::sm_count(), L.layer);
+    const bdattn::GemmPlan plan = bdattn::plan_gemm(shapes, n, bdattn::sm_count(), !L.layer ? 0 : L.args.p[0].act == bdattn::kActNone ? 1 : 2);
     L.args.split = plan.split;
     for (int i = 0; i < n; ++i) {
         bdattn::GemmProblem& p = L.args.p[i];

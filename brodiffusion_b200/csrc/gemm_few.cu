@@ -29,10 +29,16 @@ __device__ __forceinline__ void few_mma(float (&d)[4], uint32_t a0, uint32_t a1,
         gen_mma<kBf16>(d, a, b0, b1);
     }
 }
-// Weights are read once: they leave what is kept in L1 where it is.
+// Weights are read once: they leave what is kept in L1 where it is.  (Neither these loads nor those of X are of the
+// read-only kind: this kernel may be resident while the one that writes its operands still runs.)
 __device__ __forceinline__ uint4 load_stream(const void* p) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 load_kept(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 
@@ -85,7 +91,7 @@ gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) w[s][h] = load_stream(wp[h] + s * 32);
 #pragma unroll
-            for (int r = 0; r < NR; ++r) x[s][r] = __ldg(reinterpret_cast<const uint4*>(xp[r] + s * 32));
+            for (int r = 0; r < NR; ++r) x[s][r] = load_kept(xp[r] + s * 32);
         }
         wp[0] += advance;
         wp[1] += advance;
@@ -124,7 +130,7 @@ gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) w[s][h] = load_stream(wp[h] + s * 32);
 #pragma unroll
-                for (int r = 0; r < NR; ++r) x[s][r] = __ldg(reinterpret_cast<const uint4*>(xp[r] + s * 32));
+                for (int r = 0; r < NR; ++r) x[s][r] = load_kept(xp[r] + s * 32);
             }
         }
         products(w, x);
@@ -152,7 +158,7 @@ gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
         if (m >= p.M || n >= p.N) continue;
         float f[1] = {0.0f};
         for (int k = 0; k < a.parts; ++k) f[0] += parts_s[k][i];
-        if (kFp8) f[0] *= (p.x_scale != nullptr ? __ldg(p.x_scale + m) : 1.0f) * (p.w_scale != nullptr ? __ldg(p.w_scale + n) : 1.0f);
+        if (kFp8) f[0] *= (p.x_scale != nullptr ? load_scale(p.x_scale + m) : 1.0f) * (p.w_scale != nullptr ? __ldg(p.w_scale + n) : 1.0f);
         if (p.bias != nullptr) f[0] += layer_ld16<kBf16>(p.bias, n);
         activate(f, p.act);
         if (p.gate != nullptr) f[0] *= layer_ld16<kBf16>(p.gate, n);

@@ -40,6 +40,14 @@ __device__ __forceinline__ float2 layer_pair(uint32_t w) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
+// A row's scale.  Not through the read-only path: the kernel before this one writes it, and may still run when
+// this one is resident.
+__device__ __forceinline__ float load_scale(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+
 // Column values of a tile in shared memory, n to each of three arrays: bias, weight scale, gate.
 template <bool kBf16>
 __device__ __forceinline__ void layer_columns(const GemmProblem& p, float* cols, int n, int i, long long column, bool on) {

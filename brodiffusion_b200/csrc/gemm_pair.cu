@@ -440,7 +440,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                         res0 = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<long long>(row0) * p.ldr + t.n0;
                         res.load(res0 + l_begin, p.ldr, rows, 32, lane);
                     }
-                    if (kFp8 && p.x_scale != nullptr && lane < rows) x_scale = __ldg(p.x_scale + row0 + lane);
+                    if (kFp8 && p.x_scale != nullptr && lane < rows) x_scale = load_scale(p.x_scale + row0 + lane);
                 }
                 __syncwarp();
             } else {

@@ -74,11 +74,12 @@ BDATTN_HD constexpr bool pair_acc_reused(int tile, int pairs, int total_tiles) {
 // four, 8.8 over eight; 256 x 1280 x 5120 14.2, 11.4, 13.7.  The splits are entered at about 0.8 us less than they
 // take when all CTAs run at once, and three when not: with the times themselves launches of a few tiles would be
 // split less than tests/test_gemm_plan.py has it (256 x 1280 x 1280 6.1 us over two, 5.7 whole).
+// layer: 0 none, 1 one without an activation (gemm_layer.cuh), 2 one with.
 // GEGLU is not split: the two accumulators of a tile double the exchange.
 // The problems of a launch may differ in K (the queries and the keys of a cross-attention): the
 // longest sets the time, the shortest how far its tiles can be split, a CTA without a K
 // block would have nothing to add and nothing to wait for.
-inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, bool layer = false) {
+inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, int layer = 0) {
     bool geglu = false, heads = false, odd = false;
     int kb = 0, kb_min = 0, m_max = 0;
     for (int i = 0; i < n; ++i) {
@@ -159,8 +160,8 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, bool layer = false
             // (with more CTAs than SMs a longer part of K costs more than the split saves, and of tiles with more than 64 rows
             // any: 135 x 640 x 5120 over eight 11.5 us, over four 8.0, and the same for 100 shapes drawn at random)
             // (a layer's are entered at what they take: 333 x 1288 x 648 6.4 us whole, 7.2 over two; 128 x 2560 x 2560 9.8 and 10.7;
-            // 17 x 2560 x 10240 27.1 and 17.4)
-            const double more = layer ? 0.8 : 0.0;
+            // 17 x 2560 x 10240 27.1 and 17.4; but with an activation, whose time is shared as well, 333 x 1288 x 648 8.3 and 7.6)
+            const double more = layer == 1 ? 0.8 : 0.0;
             if (waves(64, s) <= 1.0) offer({false, 64, s}, 3.15 + more + 0.15 * kb / s);
             else if (kb <= 12 * s && m_max <= 64) offer({false, 64, s}, 3.22 + more + 0.27 * kb / s * tiles(64) * s / sms);
         }

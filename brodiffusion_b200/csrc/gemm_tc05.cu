@@ -85,7 +85,7 @@ __device__ __forceinline__ void epilogue_split(const GemmProblem& p, cooperative
                                                                 static_cast<long long>(m0 + r) * p.ldr + n0 + c);
                 res[0] = w.x; res[1] = w.y; res[2] = w.z; res[3] = w.w;
             }
-            if (kFp8 && p.x_scale != nullptr) x_scale = __ldg(p.x_scale + m0 + r);
+            if (kFp8 && p.x_scale != nullptr) x_scale = load_scale(p.x_scale + m0 + r);
         }
         float4 u[8], v[8];
 #pragma unroll
@@ -268,7 +268,7 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                 res0 = reinterpret_cast<const uint16_t*>(p.residual) + static_cast<long long>(m0 + q * 32) * p.ldr + n0;
                 res.load(res0, p.ldr, p.M - m0 - q * 32, n_valid, lane);
             }
-            if (kFp8 && p.x_scale != nullptr && row < p.M) x_scale = __ldg(p.x_scale + row);
+            if (kFp8 && p.x_scale != nullptr && row < p.M) x_scale = load_scale(p.x_scale + row);
         }
         bool ok = mbar_wait(acc_done, 0);
         ok = __all_sync(0xffffffffu, ok);

@@ -14,9 +14,12 @@
 namespace bdattn {
 
 // Keys of batch item b.  The lengths lie in device memory, where the host cannot check them: one outside
-// [0, Lk] counts as the nearer end.
+// [0, Lk] counts as the nearer end.  (Not read through the read-only path: the kernel before this one may write them.)
 __device__ __forceinline__ int window_keys(const int* kv_len, int batch, int lk) {
-    return kv_len == nullptr ? lk : max(0, min(lk, __ldg(kv_len + batch)));
+    if (kv_len == nullptr) return lk;
+    int n;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(n) : "l"(kv_len + batch));
+    return max(0, min(lk, n));
 }
 
 // What queries at positions [first, last] see of n keys, but for the key mask: keys [0, sink_end) and

@@ -608,7 +608,8 @@ int bdattn_linear_act_fwd(const bdattn_linear_act_params* p, bdattn_stream_t str
  *           mask_mode must be CAUSAL; no per-key scales and no fused query norm / RoPE
  *   kv_len  batch ints in device memory, read by the kernel (a captured graph follows their
  *           growth); a value outside [0, Lk] counts as the nearer end
- * Calls with few query rows share the keys of a head among CTAs; no workspace in either form. */
+ * The output may not overlap q, k or v.  Batch strides of 0 stand for dense items.  Calls with few query rows share the
+ * keys of a head among CTAs; no workspace in either form. */
 typedef struct bdattn_window_params {
     int window;            /* >= 0; 0: unbounded */
     int sinks;             /* >= 0 */

@@ -182,6 +182,27 @@ def test_segments(bd, lq, lk0, lk1):
         assert torch.isfinite(one).all()
 
 
+@pytest.mark.parametrize("lq", [1, 4, 140])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_segments_with_lengths_and_a_mask(bd, lq, hd):
+    """Lengths that end in either segment, masked keys in both; NaN in every place that nobody sees."""
+    nh, nkv, lk0, lk1 = 4, 2, 150, 200
+    lens = [0, 1, 140, 150, 151, 288, 350]
+    q, k, v = inputs(hd + lq, len(lens), lq, lk0 + lk1, nh, nkv, hd)
+    mask = torch.ones(lk0 + lk1, device="cuda")
+    mask[20:60] = mask[145:155] = mask[300] = 0
+    for t in (k, v):
+        t[:, mask == 0] = float("nan")
+        for b, n in enumerate(lens):
+            t[b, n:] = float("nan")
+    kv_len = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    for window, sinks in ((0, 0), (120, 30), (50, 160)):
+        out = torch.empty_like(q)
+        bd.sdpa_window_fwd([q], [k[:, :lk0], k[:, lk0:]], [v[:, :lk0], v[:, lk0:]], [out], nh, window=window, sinks=sinks, num_kv_heads=nkv,
+                           kv_len=kv_len, key_mask=mask)
+        check(bd, q, k, v, nh, nkv, window, sinks, lens, mask, out=out)
+
+
 @pytest.mark.parametrize("lq", [1, 2, 150])
 def test_strides(bd, lq):
     """Heads inside a wider row (a fused projection's output), a cache with room behind every sequence."""
