@@ -157,7 +157,7 @@ def _packer(cls):
 
 _pack_sdpa, _pack_qkv, _pack_qkvo = _packer(SdpaParams), _packer(QkvProjParams), _packer(QkvoParams)
 _pack_job = _packer(NormRopeJob)
-_pack_add_rmsnorm, _pack_window, _pack_linear_act = _packer(AddRmsNormParams), _packer(WindowParams), _packer(LinearActParams)
+_pack_window = _packer(WindowParams)
 _FLT_MAX = struct.unpack("f", b"\xff\xff\x7f\x7f")[0]
 
 
@@ -242,7 +242,7 @@ def lib():
         # The same entry points for this module's own calls, which pass packed structures (bytes) as pointers
         for name in ("sdpa_fwd", "sdpa_fwd_allgather", "sdpa_fwd_allgather_multicast", "mgpu_sdpa_fwd_headsharded",
                      "sdpa_traced_fwd", "rmsnorm_rope", "qkvo_fwd", "qkvo_fwd_static", "qkv_norm_rope_fwd",
-                     "add_rmsnorm_fwd", "sdpa_window_fwd", "linear_act_fwd"):
+                     "sdpa_window_fwd"):
             fn = L["bdattn_" + name]             # a function object of its own
             fn.argtypes = [C.c_void_p if t in _STRUCTURES else t for t in getattr(L, "bdattn_" + name).argtypes]
             setattr(L, "packed_" + name, fn)
@@ -647,19 +647,30 @@ def qkv_norm_rope_fwd(x, wq, wk, wv, q_out, k_out, v_out, num_heads, head_dim, *
     _check(lib().packed_qkv_norm_rope_fwd(p, _stream(stream)))
 
 
-def _int32(t, what):
-    """Pointer of an INT32 tensor."""
-    if _torch is None:
-        _bind_torch()
-    if getattr(t, "dtype", None) is not _torch.int32:
-        raise BdattnError(f"{what} must be INT32")
-    return t.data_ptr()
+_binding = None          # the module of csrc/binding.cpp
+
+
+def _load_binding():
+    """Load ``_binding.so``: the layer operators' calls, which check and pass torch tensors without Python."""
+    global _binding
+    path = _build.BINDING_PATH
+    if not os.path.exists(path):
+        raise BdattnError(f"{path} is missing: build it with `python -m brodiffusion_b200._build` "
+                          "(there is no fallback implementation)")
+    lib()
+    import torch  # noqa: F401  (its libraries, which the module needs)
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_file_location
+    loader = ExtensionFileLoader("_binding", path)
+    m = module_from_spec(spec_from_file_location("_binding", path, loader=loader))
+    loader.exec_module(m)
+    m.set_error(BdattnError)
+    _binding = m
+    return m
 
 
 def _vector(t, n, what):
-    """Pointer of a dense 1-D tensor of n values, 0 for None."""
-    if t is None:
-        return 0
+    """Pointer of a dense 1-D tensor of n values."""
     if t.shape != (n,) or (n > 1 and t.stride() != (1,)):
         raise BdattnError(f"{what} must be a dense tensor of {n} values")
     return t.data_ptr()
@@ -668,40 +679,8 @@ def _vector(t, n, what):
 def add_rmsnorm_fwd(x, out, gain=None, *, residual=None, residual_out=None, out_scale=None, eps=1e-6, stream=None):
     """``bdattn_add_rmsnorm_fwd``: h = x (+ residual), residual_out = h, out = rmsnorm(h) * gain; with a
     ``torch.float8_e4m3fn`` out, out_scale (rows, FP32) receives the rows' scales."""
-    # (written out: helpers for each tensor took 4 of the call's 7 us)
-    shape, st, ot = x.shape, x.stride(), out.stride()
-    if len(shape) != 2 or out.shape != shape:
-        raise BdattnError("x and out must be 2-D tensors of the same shape")
-    rows, cols = shape
-    if cols > 1 and (st[1] != 1 or ot[1] != 1):
-        raise BdattnError("tensor columns must be contiguous")
-    x_dtype = x.dtype
-    rp = r_ld = rop = ro_ld = gp = sp = 0
-    g_code = F32
-    if residual is not None:
-        rp, rt = residual.data_ptr(), residual.stride()
-        r_ld = rt[0] if rows > 1 else cols
-        if residual.shape != shape or residual.dtype is not x_dtype or (cols > 1 and rt[1] != 1):
-            raise BdattnError("residual must have the shape and dtype of x, with contiguous columns")
-    if residual_out is not None:
-        rop, rt = residual_out.data_ptr(), residual_out.stride()
-        ro_ld = rt[0] if rows > 1 else cols
-        if residual_out.shape != shape or residual_out.dtype is not x_dtype or (cols > 1 and rt[1] != 1):
-            raise BdattnError("residual_out must have the shape and dtype of x, with contiguous columns")
-    if gain is not None:
-        gp, g_code = _vector(gain, cols, "gain"), _dtype_code(gain)
-    if out_scale is not None:
-        if _dtype_code(out_scale) != F32:
-            raise BdattnError("out_scale must be FP32")
-        sp = _vector(out_scale, rows, "out_scale")
-    try:
-        p = _pack_add_rmsnorm(_dtype_code(x), rows, cols, x.data_ptr(), rp, rop, gp, g_code, out.data_ptr(), _dtype_code(out), sp,
-                              st[0] if rows > 1 else cols, r_ld, ro_ld, ot[0] if rows > 1 else cols,
-                              eps if eps == 1e-6 else _f32(eps))
-    except struct.error as e:
-        raise TypeError(str(e)) from None
-    if lib().packed_add_rmsnorm_fwd(p, _stream(stream)):
-        raise BdattnError(last_error())
+    (_binding or _load_binding()).add_rmsnorm(x, out, gain, residual, residual_out, out_scale, eps,
+                                              None if stream is None else stream.cuda_stream)
 
 
 def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, num_kv_heads=0, key_mask=None,
@@ -709,69 +688,34 @@ def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, nu
     """``bdattn_sdpa_window_fwd``: causal attention over a cache; query i of Lq sits at position P = n - Lq + i, where
     n = kv_len[b] (INT32, one value per batch item) or all rows of k, and sees the last ``window`` keys up to P (0: all) and
     the first ``sinks``.  Tensors and segments as for ``sdpa_fwd``."""
-    try:
-        w = _pack_window(window, sinks, _int32(kv_len, "kv_len") if kv_len is not None else 0)
-    except struct.error as e:
-        raise TypeError(str(e)) from None
-    if key_mask is not None and _dtype_code(key_mask) != F32:
-        raise BdattnError("key_mask must be FP32")
-    if isinstance(q, (list, tuple)) or isinstance(k, (list, tuple)):
-        lists = [x if isinstance(x, (list, tuple)) else (x,) for x in (q, k, v, out)]
-        first, batch = lists[0][0], _rows2d(lists[0][0])[4]
-        for x, heads in zip(lists, (num_heads, num_kv_heads or num_heads, num_kv_heads or num_heads, num_heads)):
-            for t in x:
-                if t.dtype is not first.dtype or _rows2d(t)[4] != batch:
-                    raise BdattnError("q, k, v and out must have the same dtype and batch")
-                if batch > 1 and t.stride()[0] == 0:
-                    raise BdattnError("a tensor's batch items must not be the same memory")
-                if t.shape[-1] * num_heads != first.shape[-1] * heads:
-                    raise BdattnError("q and out must have num_heads, k and v num_kv_heads heads of the same width")
-        if kv_len is not None:
-            _vector(kv_len, batch, "kv_len")
-        if key_mask is not None:
-            _vector(key_mask, sum(t.shape[-2] for t in (k if isinstance(k, (list, tuple)) else (k,))), "key_mask")
-        sdpa_fwd(q, k, v, out, num_heads, mask_mode=MASK_CAUSAL, key_mask=key_mask, softmax_scale=softmax_scale,
-                 num_kv_heads=num_kv_heads, stream=stream, _window=w)
+    if not (isinstance(q, (list, tuple)) or isinstance(k, (list, tuple))):
+        (_binding or _load_binding()).sdpa_window(q, k, v, out, num_heads, window, sinks, num_kv_heads, kv_len, key_mask, softmax_scale,
+                                                  None if stream is None else stream.cuda_stream)
         return
-    # one segment each, the usual call of a decoding step, without the lists
-    qs, qt, ks, kt, vt, ot = q.shape, q.stride(), k.shape, k.stride(), v.stride(), out.stride()
-    if out.shape != qs or v.shape != ks:
-        raise BdattnError("out must have the shape of q and v that of k")
-    if len(qs) == 3 and len(ks) == 3:
-        batch, lq, cols = qs
-        kb, lk, kv_cols = ks
-        q_bs, q_ld, q1 = qt
-        k_bs, k_ld, k1 = kt
-        v_bs, v_ld, v1 = vt
-        o_bs, o_ld, o1 = ot
-        if batch > 1 and not (q_bs and k_bs and v_bs and o_bs):         # (the library takes 0 for dense items)
-            raise BdattnError("a tensor's batch items must not be the same memory")
-    elif len(qs) == 2 and len(ks) == 2:
-        batch = kb = 1
-        q_bs = k_bs = v_bs = o_bs = 0
-        (lq, cols), (lk, kv_cols) = qs, ks
-        (q_ld, q1), (k_ld, k1), (v_ld, v1), (o_ld, o1) = qt, kt, vt, ot
-    else:
-        raise BdattnError("expected 2-D or 3-D tensors")
-    if not q1 == k1 == v1 == o1 == 1:
-        raise BdattnError("tensor columns must be contiguous")
-    dtype = q.dtype
-    if k.dtype is not dtype or v.dtype is not dtype or out.dtype is not dtype or kb != batch:
-        raise BdattnError("q, k, v and out must have the same dtype and batch")
-    if cols % num_heads or kv_cols * num_heads != cols * (num_kv_heads or num_heads):
-        raise BdattnError("q and out must have num_heads, k and v num_kv_heads heads of the same width")
+    lists = [x if isinstance(x, (list, tuple)) else (x,) for x in (q, k, v, out)]
+    first, batch = lists[0][0], _rows2d(lists[0][0])[4]
+    for x, heads in zip(lists, (num_heads, num_kv_heads or num_heads, num_kv_heads or num_heads, num_heads)):
+        for t in x:
+            if t.dtype is not first.dtype or _rows2d(t)[4] != batch:
+                raise BdattnError("q, k, v and out must have the same dtype and batch")
+            if batch > 1 and t.stride()[0] == 0:
+                raise BdattnError("a tensor's batch items must not be the same memory")
+            if t.shape[-1] * num_heads != first.shape[-1] * heads:
+                raise BdattnError("q and out must have num_heads, k and v num_kv_heads heads of the same width")
     if kv_len is not None:
+        if str(kv_len.dtype) != "torch.int32":
+            raise BdattnError("kv_len must be INT32")
         _vector(kv_len, batch, "kv_len")
+    if key_mask is not None:
+        if _dtype_code(key_mask) != F32:
+            raise BdattnError("key_mask must be FP32")
+        _vector(key_mask, sum(t.shape[-2] for t in lists[1]), "key_mask")
     try:
-        p = _pack_sdpa(_dtype_code(q), batch, num_heads, cols // num_heads,
-                       1, q.data_ptr(), 0, out.data_ptr(), 0, lq, 0, q_ld, 0, o_ld, 0, q_bs, 0, o_bs, 0,
-                       1, k.data_ptr(), 0, v.data_ptr(), 0, lk, 0, k_ld, 0, v_ld, 0, k_bs, 0, v_bs, 0,
-                       MASK_CAUSAL, _vector(key_mask, lk, "key_mask"), 0, 0, softmax_scale and _f32(softmax_scale), num_kv_heads,
-                       0, 0, 0, 0.0, 0, 0, 0)
+        w = _pack_window(window, sinks, _addr(kv_len))
     except struct.error as e:
         raise TypeError(str(e)) from None
-    if lib().packed_sdpa_window_fwd(p, w, _stream(stream)):
-        raise BdattnError(last_error())
+    sdpa_fwd(q, k, v, out, num_heads, mask_mode=MASK_CAUSAL, key_mask=key_mask, softmax_scale=softmax_scale,
+             num_kv_heads=num_kv_heads, stream=stream, _window=w)
 
 
 ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
@@ -780,43 +724,8 @@ ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_tanh": 2, "silu": 3}
 def linear_act_fwd(x, w, bias, y, *, act="none", gate=None, residual=None, x_scale=None, w_scale=None, stream=None):
     """``bdattn_linear_act_fwd``: y = residual + gate * act((x @ w.T) * x_scale[:, None] * w_scale + bias); x and w of
     the type of y, or both ``torch.float8_e4m3fn`` with FP32 scales per row.  act: a key of ``ACTIVATIONS``."""
-    xs, ws, ys = x.shape, w.shape, y.shape
-    xt, wt, yt = x.stride(), w.stride(), y.stride()
-    if len(xs) != 2 or len(ws) != 2 or ws[1] != xs[1] or ys != (xs[0], ws[0]):
-        raise BdattnError(f"x (M, K), w (N, K) and y (M, N) do not fit: {tuple(xs)}, {tuple(ws)} and {tuple(ys)}")
-    M, K = xs
-    N = ws[0]
-    if (xt[1] != 1 or wt[1] != 1) and K > 1 or yt[1] != 1 and N > 1:
-        raise BdattnError("tensor columns must be contiguous")
-    dtype = y.dtype
-    if w.dtype is not x.dtype:
-        raise BdattnError("x and w must have the same dtype")
-    rp = r_ld = bp = gp = xp = wp = 0
-    if residual is not None:
-        rp, rt = residual.data_ptr(), residual.stride()
-        r_ld = rt[0] if M > 1 else N
-        if residual.shape != ys or residual.dtype is not dtype or (N > 1 and rt[1] != 1):
-            raise BdattnError("residual must have the shape and dtype of y, with contiguous columns")
-    if bias is not None:
-        bp = _vector(bias, N, "bias")
-        if bias.dtype is not dtype:
-            raise BdattnError("bias must have the dtype of y")
-    if gate is not None:
-        gp = _vector(gate, N, "gate")
-        if gate.dtype is not dtype:
-            raise BdattnError("gate must have the dtype of y")
-    if x_scale is not None:
-        xp = _vector(x_scale, M, "x_scale")
-        if _dtype_code(x_scale) != F32:
-            raise BdattnError("x_scale must be FP32")
-    if w_scale is not None:
-        wp = _vector(w_scale, N, "w_scale")
-        if _dtype_code(w_scale) != F32:
-            raise BdattnError("w_scale must be FP32")
     code = ACTIVATIONS.get(act)
     if code is None:
         raise BdattnError(f"unknown activation {act!r} (one of {', '.join(ACTIVATIONS)})")
-    p = _pack_linear_act(_dtype_code(y), _dtype_code(x), M, N, K, x.data_ptr(), w.data_ptr(), bp, gp, rp, y.data_ptr(), xp, wp, code,
-                         xt[0] if M > 1 else K, wt[0] if N > 1 else K, r_ld, yt[0] if M > 1 else N)
-    if lib().packed_linear_act_fwd(p, _stream(stream)):
-        raise BdattnError(last_error())
+    (_binding or _load_binding()).linear_act(x, w, bias, y, code, gate, residual, x_scale, w_scale,
+                                             None if stream is None else stream.cuda_stream)

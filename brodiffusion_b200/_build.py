@@ -18,6 +18,32 @@ NVCC_FLAGS = [
 ]
 
 
+# The Python module of the calls of a decoding step (csrc/binding.cpp): torch tensors in, the library's entry points out.
+BINDING_PATH = os.path.join(PKG_DIR, "_binding.so")
+
+
+def build_binding(force: bool = False) -> str:
+    src = os.path.join(CSRC, "binding.cpp")
+    header = os.path.join(PKG_DIR, "..", "include", "bdattn.h")
+    if not force and os.path.exists(BINDING_PATH) and os.path.getmtime(BINDING_PATH) >= max(map(os.path.getmtime, (src, header))):
+        return BINDING_PATH
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *[f"-I{p}" for p in cpp_extension.include_paths()], f"-I{cuda}/include", f"-I{sysconfig.get_paths()['include']}",
+           src, "-o", BINDING_PATH, f"-L{PKG_DIR}", "-lbdattn", f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("building _binding.so failed")
+    return BINDING_PATH
+
+
 def sources():
     out = []
     for root, _, files in os.walk(CSRC):
@@ -36,6 +62,7 @@ def is_stale() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile every CUDA source of the package into ``libbdattn.so``."""
     if not force and not is_stale():
+        build_binding()
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     cmd = [nvcc, *NVCC_FLAGS, "-o", LIB_PATH, os.path.join(CSRC, "bdattn_lib.cu")]
@@ -48,6 +75,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         raise RuntimeError("nvcc failed building libbdattn.so")
     if verbose:
         print(log)
+    build_binding(force)
     return LIB_PATH
 
 
