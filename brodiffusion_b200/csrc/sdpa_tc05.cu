@@ -543,12 +543,19 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             }
             int lim = ti.valid - 1;
             if (kWindow || a.mask_mode == 1) lim = min(lim, q_glob + q_offset - ti.kbase);
-            // columns [hide, hide + hidden) lie between the sinks and the window
-            uint32_t hide = 0, hidden = 0;
+            // With a window columns [hide, past) lie between the sinks and the window.  What the row sees as 128 bits, worked out
+            // ahead of the scores: a test and a select for each of them, where comparisons with all three bounds take four.
+            uint32_t seen[4] = {};
+            bool cut = false;
             if constexpr (kWindow) {
-                hide = static_cast<uint32_t>(max(0, a.w.sinks - ti.kbase));
-                if (a.w.window > 0)
-                    hidden = static_cast<uint32_t>(max(0, q_glob + q_offset - a.w.window + 1 - ti.kbase - static_cast<int>(hide)));
+                const int hide = max(0, a.w.sinks - ti.kbase), past = a.w.window > 0 ? q_glob + q_offset - a.w.window + 1 - ti.kbase : 0;
+                auto below = [](int n, int w) {          // columns below n of the w-th 32
+                    n -= 32 * w;
+                    return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+                };
+                cut = lim < kBN - 1 || (past > hide && hide < kBN);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) seen[w] = below(lim + 1, w) & (below(hide, w) | ~below(past, w));
             }
             // A wait that runs out leaves `ok` false in its lane and the step goes on with
             // whatever is there; the vote on the row maximum below ends the loop for the
@@ -611,9 +618,9 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             }
             // (uniform over the CTA without the causal rule: no vote on whole tiles)
             if constexpr (kWindow) {
-                if (__any_sync(0xffffffffu, lim < kBN - 1 || (hidden > 0 && hide < kBN))) {
+                if (__any_sync(0xffffffffu, cut)) {
 #pragma unroll
-                    for (int c = 0; c < kBN; ++c) s[c] = (c <= lim && c - hide >= hidden) ? s[c] : -INFINITY;
+                    for (int c = 0; c < kBN; ++c) s[c] = (seen[c >> 5] & (1u << (c & 31))) != 0 ? s[c] : -INFINITY;
                 }
             } else if (a.mask_mode == 1 ? __any_sync(0xffffffffu, lim < kBN - 1) : ti.valid < kBN) {
 #pragma unroll
