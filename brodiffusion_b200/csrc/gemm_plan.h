@@ -159,9 +159,10 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, int layer = 0) {
         for (int s = 2; s <= 8 && kb >= 3 * s && kb_min >= s && tiles(64) * s * 2 <= 3LL * sms; s *= 2) {
             // (with more CTAs than SMs a longer part of K costs more than the split saves, and of tiles with more than 64 rows
             // any: 135 x 640 x 5120 over eight 11.5 us, over four 8.0, and the same for 100 shapes drawn at random)
-            // (a layer's are entered at what they take: 333 x 1288 x 648 6.4 us whole, 7.2 over two; 128 x 2560 x 2560 9.8 and 10.7;
-            // 17 x 2560 x 10240 27.1 and 17.4; but with an activation, whose time is shared as well, 333 x 1288 x 648 8.3 and 7.6)
-            const double more = layer == 1 ? 0.8 : 0.0;
+            // (a layer's are entered at what they take: tiles of more than 64 rows 2.5 us more, 128 x 2560 x 2560 10.6 over two and 9.7
+            // whole, 600 x 640 x 2560 10.1 and 9.3, 256 x 1280 x 5120 11.4 and 14.2; of up to 64 rows 0.8, or nothing with an
+            // activation, whose time is shared as well: 17 x 2560 x 10240 17.1 and 24.9)
+            const double more = layer == 0 ? 0.0 : m_max > 64 ? 2.5 : layer == 1 ? 0.8 : 0.0;
             if (waves(64, s) <= 1.0) offer({false, 64, s}, 3.15 + more + 0.15 * kb / s);
             else if (kb <= 12 * s && m_max <= 64) offer({false, 64, s}, 3.22 + more + 0.27 * kb / s * tiles(64) * s / sms);
         }
@@ -186,7 +187,10 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, int layer = 0) {
                                                                                      : 1.45 + 0.06 * f + x * (2.04 + 0.143 * f));
         }
     }
-    // A layer's tiles (gemm_layer.cuh) come in widths between these too, where they fill the pairs better; the times lie between
+    // A layer's tile of 32 columns, where all of them run at once: half of the epilogue, which nothing hides there (128 x 2560 x
+    // 2560 8.9 us, with 64 columns 9.7, 100 x 1280 x 1280 in 8 bits 3.8 and 4.8, 24 x 640 x 640 3.6 and 4.2).
+    if (layer != 0 && waves(32, 1) <= 1.0) offer({false, 32, 1}, 1.9 + 0.16 * kb);
+    // Its tiles (gemm_layer.cuh) come in widths between these too, where they fill the pairs better; the times lie between
     // (128, 160, 192, 224 and 256 columns: 2166 x 2560 x 10240 96, 90, -, -, 109 us, 1024 x 2560 x 2560 19.9, 15.8, -, -, 20.8, 1500 x
     // 2304 x 2240 18.9, -, 16.6, -, 19.2, 2048 x 2240 x 2240 -, 24.2, -, 27.0, -, 3000 x 1920 x 2560 28.1, 26.0, 27.4, -, -).
     for (int cols = 160; layer && cols < 256; cols += 32) {
