@@ -14,8 +14,27 @@ bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_
 constexpr int kFewRowsMost = 16;
 constexpr int kFewColsMost = 16 * 65535;      // its grid
 
-// Query rows that share a K/V head, up to which they go to the kernel for few rows.
-constexpr int kFewMost = 64;
+// Whether a call with a window goes to the kernel for few query rows.  Up to 64 rows that share a K/V head it always
+// does: the tensor-core kernel computes 128 rows of a single head whatever they are, and its CTAs walk the keys alone (8
+// K/V heads of 128 with 24 query heads, 63 rows and 66, that is 21 tokens and 22: 300 keys 7.3 us and 8.4, 4000 keys 12.2 and 44.6; 8
+// sequences of 4000 keys 49.9 and 89.7).  More rows go there as long as each sixteen of them have an SM, so that
+// clusters can share their keys, and the modelled time is the lower one (few rows and tensor-core kernel: 8 query heads over 2 K/V
+// heads of 128, 128 tokens over 16000 keys 47 and 159 us; 64 heads' tokens over 1000 keys 7.5 and 14.3; 64 tokens by themselves 5.7 and
+// 5.6; with more CTAs than SMs 1000 tokens of 24 heads 68 and 18, 858 tokens of 2 x 3 heads 22 and 13).
+bool few_rows(const bdattn::SdpaWindowArgs& g, int num_heads, int num_kv_heads, int batch) {
+    const int sms = bdattn::sm_count(), lq = g.q_rows[0], lk = g.kv_rows[0] + g.kv_rows[1];
+    const long long rows = static_cast<long long>(lq) * g.kv_group, tiles = num_kv_heads * ((rows + 15) / 16), units = batch * tiles;
+    if (g.q_rows[1] > 0 || tiles > 65535) return false;
+    if (rows <= 64) return true;
+    if (units > sms) return false;
+    // keys that sixteen rows see on average, and those that the 128 or 256 of the other kernel's CTA with the most see
+    auto seen = [&](double keys, int more) { return g.window > 0 && 1.0 * g.window + g.sinks + more < keys ? 1.0 * g.window + g.sinks + more : keys; };
+    const double few = 4.0 + 0.45 * (g.head_dim > 64 ? 1.0 : 0.7) * units * (seen(lk - 0.5 * lq, 16) / 64 + 0.5) / sms;
+    const double pairs = 1.0 * batch * num_heads * ((lq + 255) / 256), singles = 1.0 * batch * num_heads * ((lq + 127) / 128);
+    const bool lone = 2 * pairs <= sms;           // (its CTAs have one query tile each then: launch_t in sdpa_tc05.cu)
+    const double steps = seen(lk, lone ? 128 : 256) / 128 + 1;
+    return few < 4.0 + std::ceil((lone ? singles : pairs) / sms) * (2.0 + steps * (lone ? 1.2 : 1.45));
+}
 
 // The tensor-core attention kernel's arguments for a call with a window: head_dim <= 128.
 int window_launch(const char* op, bdattn::SdpaLaunch& L, const bdattn::SdpaWindowArgs& g, int num_heads, int num_kv_heads, int batch,
@@ -200,7 +219,7 @@ int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_para
     const bool bf16 = p->dtype == BDATTN_BF16;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (hd <= 128 && p->n_q_seg == 1 && lq * g.kv_group <= kFewMost && nkv * ((lq * g.kv_group + 15) / 16) <= 65535) {
+    if (hd <= 128 && few_rows(g, p->num_heads, nkv, p->batch)) {
         bdattn::SdpaFewLaunch L;
         for (int s = 0; s < 2; ++s) {
             const int k = s < p->n_kv_seg ? s : 0;
