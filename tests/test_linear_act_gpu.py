@@ -7,6 +7,8 @@ error below 4e-6 |z|."""
 import pytest
 import torch
 
+from layer_shapes import SHAPES
+
 pytestmark = pytest.mark.gpu
 
 UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
@@ -86,6 +88,24 @@ def test_sizes(bd, M, N, K, kind):
     check(call(bd, p, "none"), p, "none")
     p = problem(M + N + K + 9, M, N, K, dtype, kind == "fp8", gate=True, residual=True)
     check(call(bd, p, "gelu_tanh"), p, "gelu_tanh")
+
+
+@pytest.mark.parametrize("M,N,K,act,kernel,cols,split", SHAPES)
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+def test_every_tile_width_and_split(bd, M, N, K, act, kernel, cols, split, kind):
+    p = problem(M + N + K, M, N, 2 * K if kind == "fp8" else K, torch.float16 if kind == "fp16" else torch.bfloat16, kind == "fp8", True, True, True)
+    name = "gelu" if act else "none"
+    check(call(bd, p, name), p, name)
+
+
+# up to 16 rows: one and two eights of them; many rows of W with a short K and a long one, few with K over two, four and eight
+# CTAs; K with a remainder of a turn of 64
+@pytest.mark.parametrize("N,K", [(7200, 64), (7200, 640), (8192, 2560), (64, 10240), (1280, 5120), (640, 2560), (72, 4112), (2560, 2576), (24, 16), (8, 8208)])
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 16])
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+def test_few_rows(bd, M, N, K, kind):
+    p = problem(M + N + K, M, N, K, torch.float16 if kind == "fp16" else torch.bfloat16, kind == "fp8", True, M % 2 == 0, True)
+    check(call(bd, p, "silu"), p, "silu")
 
 
 @pytest.mark.parametrize("act", list(ACT))
