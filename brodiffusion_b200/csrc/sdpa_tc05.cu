@@ -549,13 +549,15 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             bool cut = false;
             if constexpr (kWindow) {
                 const int hide = max(0, a.w.sinks - ti.kbase), past = a.w.window > 0 ? q_glob + q_offset - a.w.window + 1 - ti.kbase : 0;
-                auto below = [](int n, int w) {          // columns below n of the w-th 32
-                    n -= 32 * w;
-                    return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
-                };
-                cut = lim < kBN - 1 || (past > hide && hide < kBN);
+                cut = __any_sync(0xffffffffu, lim < kBN - 1 || (past > hide && hide < kBN));
+                if (cut) {
+                    auto below = [](int n, int w) {          // columns below n of the w-th 32
+                        n -= 32 * w;
+                        return n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1u : 0u;
+                    };
 #pragma unroll
-                for (int w = 0; w < 4; ++w) seen[w] = below(lim + 1, w) & (below(hide, w) | ~below(past, w));
+                    for (int w = 0; w < 4; ++w) seen[w] = below(lim + 1, w) & (below(hide, w) | ~below(past, w));
+                }
             }
             // A wait that runs out leaves `ok` false in its lane and the step goes on with
             // whatever is there; the vote on the row maximum below ends the loop for the
@@ -618,7 +620,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             }
             // (uniform over the CTA without the causal rule: no vote on whole tiles)
             if constexpr (kWindow) {
-                if (__any_sync(0xffffffffu, cut)) {
+                if (cut) {
 #pragma unroll
                     for (int c = 0; c < kBN; ++c) s[c] = (seen[c >> 5] & (1u << (c & 31))) != 0 ? s[c] : -INFINITY;
                 }
