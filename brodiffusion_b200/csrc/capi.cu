@@ -165,7 +165,8 @@ int add_gemm_problem(const char* op, bdattn::GemmLaunch& L, int idx, const void*
     p.tiles_m = bdattn::gemm_row_tiles(M);
     p.geglu_offset = geglu_offset;
     p.n_tile = head_dim;       // 0: chosen at the launch
-    if (make_map_2d(op, &L.tmA[idx], A, L.bf16, K, M, lda, 128)) return -1;
+    L.A[idx] = A;
+    L.lda[idx] = lda;
     // the weight matrix has N (+ D_out for GEGLU) rows
     L.W[idx] = W;
     L.ldw[idx] = ldw;
@@ -174,7 +175,7 @@ int add_gemm_problem(const char* op, bdattn::GemmLaunch& L, int idx, const void*
     return 0;
 }
 
-// Makes the weight maps for the plan and launches.
+// Makes the maps for the plan and launches.
 int launch_gemm(const char* op, bdattn::GemmLaunch& L, int n, cudaStream_t stream) {
     L.n_problems = n;
     bdattn::GemmShape shapes[3];
@@ -184,8 +185,10 @@ int launch_gemm(const char* op, bdattn::GemmLaunch& L, int n, cudaStream_t strea
     }
     const bdattn::GemmPlan plan = bdattn::plan_gemm(shapes, n, bdattn::sm_count(), !L.layer ? 0 : L.args.p[0].act == bdattn::kActNone ? 1 : 2);
     L.args.split = plan.split;
+    L.args.a_rows = L.layer && !plan.pair && shapes[0].M < 128 ? (shapes[0].M + 7) / 8 * 8 : 128;
     for (int i = 0; i < n; ++i) {
         bdattn::GemmProblem& p = L.args.p[i];
+        if (make_map_2d(op, &L.tmA[i], L.A[i], L.bf16, p.K, p.M, L.lda[i], L.args.a_rows)) return -1;
         if (p.n_tile == 0) p.n_tile = plan.width;
         p.tiles_n = (p.N + p.n_tile - 1) / p.n_tile;
         // a CTA of a pair stages half of the tile's weight rows

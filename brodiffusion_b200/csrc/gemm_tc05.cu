@@ -31,14 +31,14 @@ namespace {
 
 constexpr int kGemmThreads = 192;
 constexpr int kGemmPrefetch = 20;            // K blocks whose weights are asked for ahead
-constexpr int kGemmMaxStages = 8;
-constexpr int kGemmABytes = 128 * 64 * 2;   // A stage
+constexpr int kGemmMaxStages = 14;          // their barriers take 256 bytes with the two others
+constexpr int kGemmABytes = 128 * 64 * 2;   // what an MMA block reads of A
 // A B (or gate) tile is n_tile rows x 128 B; a stage holds A, B and, for GEGLU,
 // the gate tile, rounded up to the 1024-byte swizzle period.  Sizing the stage by
 // the tile shape keeps a 64-column GEMM at 96 KB so that two CTAs share an SM.
 __host__ __device__ inline int gemm_b_bytes(int n_tile) { return (n_tile * 128 + 1023) / 1024 * 1024; }
-__host__ __device__ inline int gemm_stage_bytes(int n_tile, bool geglu) {
-    return kGemmABytes + (geglu ? 2 : 1) * gemm_b_bytes(n_tile);
+__host__ __device__ inline int gemm_stage_bytes(int a_rows, int n_tile, bool geglu) {
+    return a_rows * 128 + (geglu ? 2 : 1) * gemm_b_bytes(n_tile);
 }
 
 // Partial sums of a split tile in shared memory: row-major, four floats of padding per
@@ -143,7 +143,13 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                                                ~static_cast<uintptr_t>(1023));
     const int kGemmStages = g.stages;
     const int kGemmBBytes = gemm_b_bytes(g.n_tile_max);
-    const int kGemmStageBytes = gemm_stage_bytes(g.n_tile_max, g.any_geglu != 0);
+    // Of a layer's only row tile the stage holds the rows that there are.  The MMA reads 128 all the same, what lies behind
+    // them in shared memory for the rest: those rows of the accumulator are nobody's.  Several small rings then share an SM,
+    // and a larger part of what an SM takes in is weights (33 x 8528 x 2992 in 8 bits 16.0 -> 11.3 us, 38 x 4704 x 456 7.5 -> 4.8,
+    // 32 x 10240 x 2560 13.9 -> 13.0).
+    const int a_rows = kLayer ? g.a_rows : 128;
+    const int a_bytes = a_rows * 128;
+    const int kGemmStageBytes = gemm_stage_bytes(a_rows, g.n_tile_max, g.any_geglu != 0);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kGemmStages * kGemmStageBytes);
     uint64_t* full = bars;
     uint64_t* empty = bars + kGemmMaxStages;
@@ -193,7 +199,7 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
 
     if (warp == 0) {
         if (elect_one()) {
-            const uint32_t bytes = kGemmABytes + (geglu ? 2u : 1u) * static_cast<uint32_t>(p.n_tile) * 128u;
+            const uint32_t bytes = a_bytes + (geglu ? 2u : 1u) * static_cast<uint32_t>(p.n_tile) * 128u;
             bool ok = true;
             int issued = 0;
             int slot = 0;
@@ -205,8 +211,8 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
                 mbar_arrive_expect_tx(&full[slot], bytes);
                 const int x = (k_begin + kb) * 64;
                 tma_load_2d(st, tmA, &full[slot], x, m0);
-                tma_load_2d(st + kGemmABytes, tmB, &full[slot], x, n0);
-                if (geglu) tma_load_2d(st + kGemmABytes + kGemmBBytes, tmB, &full[slot], x, n0 + p.geglu_offset);
+                tma_load_2d(st + a_bytes, tmB, &full[slot], x, n0);
+                if (geglu) tma_load_2d(st + a_bytes + kGemmBBytes, tmB, &full[slot], x, n0 + p.geglu_offset);
                 issued = kb + 1;
                 if (++slot == kGemmStages) { slot = 0; phase ^= 1; }
             }
@@ -222,7 +228,7 @@ gemm_tc05_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant
         // division by the runtime ring size cost more than the four MMAs.
         const uint32_t idesc = make_idesc_f16(kBf16 && !kFp8 ? 1 : 0, 128, p.n_tile, 0, 0);
         const uint64_t a0 = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
-        const uint64_t b0 = make_smem_desc_sw128(smem_u32(smem) + kGemmABytes, 16, 1024);
+        const uint64_t b0 = make_smem_desc_sw128(smem_u32(smem) + a_bytes, 16, 1024);
         const uint32_t stage_units = static_cast<uint32_t>(kGemmStageBytes) >> 4;   // descriptors count 16 bytes
         const uint32_t gate_units = static_cast<uint32_t>(kGemmBBytes) >> 4;
         if (elect_one()) {
@@ -441,18 +447,21 @@ cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream) {
     // kernel's CTAs in the slots of the first finishers would undo that order for a kernel of this
     // kind (4096 rows, 2 heads of 64, K = 1024: 28.8 us a launch, 20.7 kept back).
     args.one_wave = ctas <= sm_count();
-    const int stage = gemm_stage_bytes(nt_max, any_geglu != 0);
+    const int stage = gemm_stage_bytes(args.a_rows, nt_max, any_geglu != 0);
     // three stages with the gate tile: the stage ring stays below 114 KB and two CTAs fit per SM
     args.stages = any_geglu ? 3 : 4;
     if (ctas <= sm_count()) {
         // a CTA has its SM to itself: the ring may take all of the shared memory
-        args.stages = 192 * 1024 / stage < kGemmMaxStages ? 192 * 1024 / stage : kGemmMaxStages;
+        // (32 x 5120 x 5120, 12 KB a stage: 8 of them 20.7 us, 14 16.0; other than a layer's stay at 8, which they were timed with)
+        const int most = L.layer ? kGemmMaxStages : 8;
+        args.stages = 192 * 1024 / stage < most ? 192 * 1024 / stage : most;
     } else if (!any_geglu && k_max <= 512 && args.split == 1) {
         // Short K and more tiles than SMs: a ring of two (64 KB) lets up to three CTAs share an SM,
         // so that one CTA's epilogue runs under the others' loads (4096 x 320 -> 960: 18.1 -> 12.2 us).
         args.stages = 2;
     }
-    const int smem = args.stages * stage + 256 + (L.layer ? 1536 : 1024) + 1024;    // barriers, bias, alignment
+    // barriers, bias, alignment; the MMAs of the last stage read a whole block of A from its start on
+    const int smem = args.stages * stage + max(256 + (L.layer ? 1536 : 1024), kGemmABytes - stage) + 1024;
     const dim3 grid(static_cast<unsigned>(tn), static_cast<unsigned>(tm),
                     static_cast<unsigned>(L.n_problems * args.split));
     cudaError_t e = cudaSuccess;

@@ -214,14 +214,16 @@ struct GemmArgs {
     int n_tile_max;   // largest n_tile of the launch: sizes the shared-memory stages
     int any_geglu;
     int stages;
+    int a_rows;       // rows of A in a stage (rows of the A box): 128, or of a layer's only row tile as many eights as it has
     int split;        // CTAs (a cluster) that share the K blocks of a tile
     bool one_wave;    // no more CTAs than SMs
 };
 struct GemmLaunch {
     CUtensorMap tmA[3], tmB[3];
     bool whole[3];         // problem i has whole 256-column tiles (128 for GEGLU)
-    const void* W[3];      // weights: their maps are made once the tile width is chosen
-    long long ldw[3], w_rows[3];
+    const void* A[3];      // the maps are made once kernel and tile width are chosen
+    const void* W[3];
+    long long lda[3], ldw[3], w_rows[3];
     GemmArgs args;
     int n_problems;
     bool bf16;

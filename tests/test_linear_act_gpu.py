@@ -108,6 +108,16 @@ def test_few_rows(bd, M, N, K, kind):
     check(call(bd, p, "silu"), p, "silu")
 
 
+# one row tile with fewer rows than the MMA reads: several tiles to an SM (a short ring, a ring of two), one (the longest
+# ring, more turns than it has slots), K over two and eight CTAs
+@pytest.mark.parametrize("N,K", [(9600, 208), (9600, 640), (2080, 2064), (2528, 1280), (72, 2560)])
+@pytest.mark.parametrize("M", [17, 25, 56, 65, 120, 127])
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+def test_one_row_tile(bd, M, N, K, kind):
+    p = problem(M + N + K, M, N, K, torch.float16 if kind == "fp16" else torch.bfloat16, kind == "fp8", True, True, True)
+    check(call(bd, p, "gelu"), p, "gelu")
+
+
 @pytest.mark.parametrize("act", list(ACT))
 @pytest.mark.parametrize("bias,gate,residual", [(b, g, r) for b in (0, 1) for g in (0, 1) for r in (0, 1)])
 @pytest.mark.parametrize("M,N,K", [(2, 512, 320), (40, 264, 1280), (700, 768, 256), (1300, 2560, 512)])
