@@ -187,6 +187,11 @@ inline GemmPlan plan_gemm(const GemmShape* p, int n, int sms, int layer = 0) {
                                                                                      : 1.45 + 0.06 * f + x * (2.04 + 0.143 * f));
         }
     }
+    // A layer's tiles of 96 columns over CTAs that all run at once: up to 96 rows of X are read by fewer CTAs than with 64
+    // (32 x 5120 x 5120 16.0 us whole with 64, 13.9 over two; 32 x 2560 x 10240 16.5 with 64 over two, 13.3 over four;
+    // 90 x 2560 x 10240 20.0 and 16.8; 40 x 1280 x 5120 8.0 with 64 over eight, 7.6; 128 x 2560 x 2560 8.8 with 32, 10.2 over four).
+    for (int s = 2; layer && m_max <= 96 && s <= 8 && kb >= 3 * s; s *= 2)
+        if (waves(96, s) <= 1.0) offer({false, 96, s}, 4.4 + (0.165 + 0.0017 * m_max) * kb / s);
     // A layer's tile of 32 columns, where all of them run at once: half of the epilogue, which nothing hides there (128 x 2560 x
     // 2560 8.9 us, with 64 columns 9.7, 100 x 1280 x 1280 in 8 bits 3.8 and 4.8, 24 x 640 x 640 3.6 and 4.2).
     if (layer != 0 && waves(32, 1) <= 1.0) offer({false, 32, 1}, 1.9 + 0.16 * kb);
