@@ -440,6 +440,10 @@ cudaError_t launch_gemm_tc05(const GemmLaunch& L, cudaStream_t stream) {
         any_norm_rope |= p.norm_rope ? 1 : 0;
     }
     GemmArgs args = L.args;
+    // the kernel's own rule: the shared memory is sized here for what it stages there
+    if (!L.layer) args.a_rows = 128;
+    if (args.a_rows < 8 || args.a_rows > 128 || args.a_rows % 8 != 0 || (args.a_rows < 128 && args.p[0].M > args.a_rows))
+        return cudaErrorInvalidValue;
     args.n_tile_max = nt_max;
     args.any_geglu = any_geglu;
     const long long ctas = static_cast<long long>(tn) * tm * L.n_problems * args.split;
