@@ -100,6 +100,8 @@ struct Matrix {
         cols = rows_of(t.size(1), what);
         if (cols > 1 && t.stride(1) != 1) refuse(what, "must have contiguous columns");
         ld = rows > 1 ? t.stride(0) : cols;
+        // (an expanded row has a stride of 0, which the library takes for dense rows)
+        if (ld < cols) refuse(what, "must have rows of its own (an expanded or strided view whose rows overlap)");
         data = t.data_ptr();
     }
     void same(const Matrix& o, const char* what) const {
