@@ -36,3 +36,46 @@ def test_rows_that_overlap_in_part_and_a_single_row_of_any_stride():
         bd.add_rmsnorm_fwd(z(256).as_strided((4, 64), (32, 1)), z(4, 64))
     with pytest.raises(bd.BdattnError, match="GPU"):             # nothing else to refuse: a row is dense whatever its stride
         bd.add_rmsnorm_fwd(z(64).as_strided((1, 64), (0, 1)), z(1, 64))
+
+
+def window_operands(segments):
+    q, k = z(2, 3, 128), z(2, 9, 128)
+    t = {"q": q, "k": k, "v": k.clone(), "out": q.clone(), "kv_len": z(2, dtype=torch.int32), "key_mask": z(9, dtype=torch.float32)}
+    return t if not segments else {n: [x] if n in ("q", "k", "v", "out") else x for n, x in t.items()}
+
+
+class OnGpu:
+    """A tensor of the host that says it lies on a GPU."""
+
+    def __init__(self, t, index):
+        self._t, self._index = t, index
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+    def get_device(self):
+        return self._index
+
+    @property
+    def is_cuda(self):
+        return True
+
+
+def test_segments_refuse_tensors_of_the_host(monkeypatch):
+    monkeypatch.setattr(bd, "sdpa_fwd", lambda *a, **k: pytest.fail("an address of the host went to the library"))
+    for host in ("q", "k", "v", "out", "kv_len", "key_mask", None):
+        t = window_operands(True)
+        if host is not None:               # all others on a GPU
+            for name, x in t.items():
+                if name != host:
+                    t[name] = [OnGpu(x[0], 0)] if isinstance(x, list) else OnGpu(x, 0)
+        with pytest.raises(bd.BdattnError, match="not on the GPU"):
+            bd.sdpa_window_fwd(*(t[n] for n in ("q", "k", "v", "out")), 2, window=4, kv_len=t["kv_len"], key_mask=t["key_mask"])
+
+
+def test_segments_refuse_tensors_of_different_gpus(monkeypatch):
+    monkeypatch.setattr(bd, "sdpa_fwd", lambda *a, **k: pytest.fail("the library was asked"))
+    for other in ("k", "v", "out", "kv_len", "key_mask"):
+        t = {n: [OnGpu(x[0], int(n == other))] if isinstance(x, list) else OnGpu(x, int(n == other)) for n, x in window_operands(True).items()}
+        with pytest.raises(bd.BdattnError, match="different GPUs"):
+            bd.sdpa_window_fwd(*(t[n] for n in ("q", "k", "v", "out")), 2, window=4, kv_len=t["kv_len"], key_mask=t["key_mask"])
