@@ -676,15 +676,6 @@ def _vector(t, n, what):
     return t.data_ptr()
 
 
-def _one_gpu(tensors):
-    """The tensors' addresses go to kernels of one GPU."""
-    devices = {t.get_device() for t in tensors if t is not None}
-    if -1 in devices:
-        raise BdattnError("a tensor is not on the GPU")
-    if len(devices) > 1:
-        raise BdattnError("the tensors are on different GPUs")
-
-
 def add_rmsnorm_fwd(x, out, gain=None, *, residual=None, residual_out=None, out_scale=None, eps=1e-6, stream=None):
     """``bdattn_add_rmsnorm_fwd``: h = x (+ residual), residual_out = h, out = rmsnorm(h) * gain; with a
     ``torch.float8_e4m3fn`` out, out_scale (rows, FP32) receives the rows' scales."""
@@ -723,7 +714,8 @@ def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, nu
         w = _pack_window(window, sinks, _addr(kv_len))
     except struct.error as e:
         raise TypeError(str(e)) from None
-    _one_gpu([t for x in lists for t in x] + [kv_len, key_mask])
+    tensors = [t for x in lists for t in x] + [kv_len, key_mask]
+    (_binding or _load_binding()).one_gpu(-1, *(t.get_device() for t in tensors if t is not None))
     sdpa_fwd(q, k, v, out, num_heads, mask_mode=MASK_CAUSAL, key_mask=key_mask, softmax_scale=softmax_scale,
              num_kv_heads=num_kv_heads, stream=stream, _window=w)
 

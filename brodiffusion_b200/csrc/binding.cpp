@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -77,15 +78,21 @@ int code(const at::Tensor& t, const char* what) {
         default: refuse(what, "has an unsupported dtype");
     }
 }
-// All of a call's tensors lie on one GPU.
+// A call's tensors (their GPUs' numbers, -1: the host) lie on one GPU, and that is the current one, whose stream,
+// kernels and sizes the call takes.  current: its number, -1: looked up.
+void one_gpu(int current, const int* gpus, int n) {
+    for (int i = 0; i < n; ++i)
+        if (gpus[i] < 0) refuse("a tensor is not on the GPU");
+    for (int i = 1; i < n; ++i)
+        if (gpus[i] != gpus[0]) refuse("the tensors are on different GPUs");
+    if (current < 0) current = c10::cuda::current_device();
+    if (n > 0 && gpus[0] != current) refuse("the tensors are not on the current GPU");
+}
 void on_gpu(std::initializer_list<const at::Tensor*> all) {
-    const at::Tensor* first = nullptr;
-    for (const at::Tensor* t : all) {
-        if (t == nullptr) continue;
-        if (!t->is_cuda()) refuse("a tensor is not on the GPU");
-        if (first == nullptr) first = t;
-        else if (t->get_device() != first->get_device()) refuse("the tensors are on different GPUs");
-    }
+    int gpus[16], n = 0;
+    for (const at::Tensor* t : all)
+        if (t != nullptr) gpus[n++] = t->is_cuda() ? static_cast<int>(t->get_device()) : -1;
+    one_gpu(-1, gpus, n);
 }
 
 // A 2-D tensor with contiguous columns; the stride of a single row may be anything.
@@ -280,6 +287,24 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
 }
 
+// (current, gpus...): one_gpu, for the calls that Python makes
+PyObject* one_gpu_entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    int gpus[16];
+    if (n < 1 || n > 17) {
+        PyErr_SetString(PyExc_TypeError, "1 to 17 arguments are needed");
+        return nullptr;
+    }
+    try {
+        for (Py_ssize_t i = 1; i < n; ++i) gpus[i - 1] = integer(args[i]);
+        one_gpu(integer(args[0]), gpus, static_cast<int>(n - 1));
+        Py_RETURN_NONE;
+    } catch (const Refusal&) {
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
 PyObject* set_error(PyObject*, PyObject* type) {
     Py_INCREF(type);
     Py_XDECREF(g_error);
@@ -293,6 +318,7 @@ PyMethodDef methods[] = {
     {"add_rmsnorm", fast(entry<add_rmsnorm, 8>), METH_FASTCALL, "bdattn_add_rmsnorm_fwd"},
     {"linear_act", fast(entry<linear_act, 10>), METH_FASTCALL, "bdattn_linear_act_fwd"},
     {"sdpa_window", fast(entry<sdpa_window, 12>), METH_FASTCALL, "bdattn_sdpa_window_fwd"},
+    {"one_gpu", fast(one_gpu_entry), METH_FASTCALL, "refuses tensors of the host, of different GPUs, of another than the current one"},
     {"set_error", set_error, METH_O, "the exception of a refused call"},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -79,3 +79,16 @@ def test_segments_refuse_tensors_of_different_gpus(monkeypatch):
         t = {n: [OnGpu(x[0], int(n == other))] if isinstance(x, list) else OnGpu(x, int(n == other)) for n, x in window_operands(True).items()}
         with pytest.raises(bd.BdattnError, match="different GPUs"):
             bd.sdpa_window_fwd(*(t[n] for n in ("q", "k", "v", "out")), 2, window=4, kv_len=t["kv_len"], key_mask=t["key_mask"])
+
+
+def test_tensors_of_another_gpu_than_the_current_one_are_refused():
+    """What the calls ask about the GPUs of their tensors (the current one's number ahead of theirs; -1 is the host)."""
+    one_gpu = (bd._binding or bd._load_binding()).one_gpu
+    assert one_gpu(0, 0, 0, 0) is None and one_gpu(3, 3) is None
+    for gpus, reason in (((0, 1, 1), "current GPU"), ((1, 0), "current GPU"), ((0, 0, 1), "different GPUs"), ((0, 0, -1), "not on the GPU"),
+                         ((0, -1, 0), "not on the GPU")):
+        with pytest.raises(bd.BdattnError, match=reason):
+            one_gpu(*gpus)
+    for bad in ((), ("0", 0), (0, None)):
+        with pytest.raises(TypeError):
+            one_gpu(*bad)
