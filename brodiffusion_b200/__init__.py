@@ -694,6 +694,8 @@ def sdpa_window_fwd(q, k, v, out, num_heads, *, window, sinks=0, kv_len=None, nu
         return
     lists = [x if isinstance(x, (list, tuple)) else (x,) for x in (q, k, v, out)]
     first, batch = lists[0][0], _rows2d(lists[0][0])[4]
+    if num_heads < 1 or first.shape[-1] % num_heads != 0:
+        raise BdattnError("the width of q must be a multiple of num_heads")
     for x, heads in zip(lists, (num_heads, num_kv_heads or num_heads, num_kv_heads or num_heads, num_heads)):
         for t in x:
             if t.dtype is not first.dtype or _rows2d(t)[4] != batch:

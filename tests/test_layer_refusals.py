@@ -92,3 +92,12 @@ def test_tensors_of_another_gpu_than_the_current_one_are_refused():
     for bad in ((), ("0", 0), (0, None)):
         with pytest.raises(TypeError):
             one_gpu(*bad)
+
+
+def test_segments_refuse_heads_that_do_not_divide_the_width():
+    """264 columns are no 32 heads; the same call without segments refuses them too."""
+    q, k = z(1, 3, 264), z(1, 9, 264)
+    for args in (([q], [k], [k], [q]), (q, k, k, q)):
+        for heads in (32, 5, 0, -1):
+            with pytest.raises(bd.BdattnError, match="num_heads"):
+                bd.sdpa_window_fwd(*args, heads, window=4)
