@@ -9,9 +9,16 @@
 namespace bdattn {
 
 // x * sigmoid(k): GELU's tanh form is x sigmoid(2 u) with u = sqrt(2 / pi) (x + 0.044715 x^3), since
-// (1 + tanh u) / 2 = sigmoid(2 u); SiLU is x sigmoid(x).  `t` is -k log2(e); beyond 2^126 the reciprocal's
-// result would be flushed to zero anyway, and the product of x with an infinite exponential's is 0.
-__device__ __forceinline__ float times_sigmoid(float x, float t) { return __fdividef(x, 1.0f + fast_exp2(fminf(t, 126.0f))); }
+// (1 + tanh u) / 2 = sigmoid(2 u); SiLU is x sigmoid(x).  `t` is -k log2(e), at most 126: the
+// approximate quotient is 0 for divisors beyond 2^126.
+__device__ __forceinline__ float times_sigmoid(float x, float t) { return __fdividef(x, 1.0f + fast_exp2(t)); }
+// The larger of both; NaN stays.  Below `least` an activation is within 2e-36 of 0, and x itself over 2^126 is not: -1e38
+// would come out as -1.2.
+__device__ __forceinline__ float at_least(float x, float least) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(least));
+    return y;
+}
 
 template <int N>
 __device__ __forceinline__ void activate(float (&f)[N], int act) {
@@ -19,12 +26,18 @@ __device__ __forceinline__ void activate(float (&f)[N], int act) {
 #pragma unroll
         for (int i = 0; i < N; ++i) f[i] = gelu_exact(f[i]);
     } else if (act == kActGeluTanh) {
-        // -2 sqrt(2 / pi) log2(e) (x + 0.044715 x^3)
+        // -2 sqrt(2 / pi) log2(e) (x + 0.044715 x^3), 125.97 at -10
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = times_sigmoid(f[i], f[i] * fmaf(f[i] * f[i], -0.10294324f, -2.3022082f));
+        for (int i = 0; i < N; ++i) {
+            const float x = at_least(f[i], -10.0f);
+            f[i] = times_sigmoid(x, x * fmaf(x * x, -0.10294324f, -2.3022082f));
+        }
     } else if (act == kActSilu) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = times_sigmoid(f[i], f[i] * -1.44269504f);
+        for (int i = 0; i < N; ++i) {
+            const float x = at_least(f[i], -87.0f);
+            f[i] = times_sigmoid(x, x * -1.44269504f);
+        }
     }
 }
 

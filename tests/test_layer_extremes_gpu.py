@@ -1,0 +1,35 @@
+"""A layer's operators at the ends of the range of their types, against their formulas in 64 bits."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, E4M3 = torch.bfloat16, torch.float8_e4m3fn
+
+
+# Kernels: few rows, a tile over a cluster, single tiles, pairs (tests/layer_shapes.py).
+@pytest.mark.parametrize("M,N,K", [(2, 64, 64), (12, 64, 64), (17, 64, 1280), (129, 1288, 648), (900, 2432, 648)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_activations_of_large_sums(bd, M, N, K, act, fp8):
+    """act(z) of a large negative z is 0 and of a large positive one z, up to the largest sums that FP32 holds."""
+    K = K // 16 * 16
+    z = torch.tensor([-3e38, -1e38, -1e37, -3e35, -1e30, -1e20, -1e9, -1e4, -200.0, -100.0, -89.0, -88.0, -87.0, -20.0, -12.0, -10.0, -9.0,
+                      0.0, 9.0, 12.0, 88.0, 200.0, 1e4, 1e20, 1e30, 3e38], device="cuda").to(BF16)
+    bias = z[torch.arange(N, device="cuda") % len(z)].contiguous()
+    x = torch.zeros(M, K, device="cuda", dtype=BF16)
+    w = torch.zeros(N, K, device="cuda", dtype=BF16)
+    if fp8:
+        x, w = x.to(E4M3), w.to(E4M3)
+    y = torch.full((M, N), 7.0, device="cuda", dtype=BF16)
+    bd.linear_act_fwd(x, w, bias, y, act=act)
+    b = bias.double()
+    u = {"silu": b, "gelu": b, "gelu_tanh": 2 * (2 / torch.pi) ** 0.5 * (b + 0.044715 * b ** 3)}[act]
+    ref = b * (torch.special.ndtr(b) if act == "gelu" else torch.sigmoid(u))
+    # the output's rounding, the activation's own error (4e-6 |z| where its slope is not flat, which it is below -20), and
+    # values below the smallest normal of BF16 and FP32
+    bound = 2.0 ** -8 * ref.abs() + torch.where(b < -20, 0.0, 4e-6 * b.abs()) + 1e-8 * (b >= -100) + 1e-30
+    assert ((y.double() - ref).abs() <= bound).all(), (y.double() - ref).abs().amax(0)
+    nan = torch.full((N,), float("nan"), device="cuda", dtype=BF16)
+    bd.linear_act_fwd(x, w, nan, y, act=act)
+    assert torch.isnan(y).all()
