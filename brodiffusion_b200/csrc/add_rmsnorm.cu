@@ -7,6 +7,7 @@
 // threads between the one read and the one write.
 #include <cuda_fp8.h>
 
+#include <cfloat>
 #include <type_traits>
 
 #include "sdpa_internal.h"
@@ -37,6 +38,12 @@ __device__ __forceinline__ void block_sum_max(float& s, float& m, float* red) {
         s += red[w];
         m = fmaxf(m, red[32 + w]);
     }
+}
+
+// The scale of a row's values of 8 bits.  The maximum of |h g| does not know of NaN, nor of an infinity under a gain of 0, but the
+// sum of squares does.  (A maximum that keeps NaN costs the row an instruction a value: 16384 x 5120 105.3 us, this way 104.1.)
+__device__ __forceinline__ float row_scale(float ss, float top, float inv) {
+    return ss <= FLT_MAX ? top * inv * (1.0f / kE4m3Max) : __uint_as_float(0x7fffffffu);
 }
 
 __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
@@ -190,7 +197,7 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) add_rm
         }
         float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
         if constexpr (kFp8) {
-            const float scale = top * inv * (1.0f / kE4m3Max);
+            const float scale = row_scale(ss, top, inv);
             if (exists && me == 0) a.out_scale[now] = scale;
             inv *= scale > 0.0f ? 1.0f / scale : 1.0f;
         }
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_wide_kernel(const __grid_con
     block_sum_max(ss, top, red);
     float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
     if constexpr (kFp8) {
-        const float scale = top * inv * (1.0f / kE4m3Max);
+        const float scale = row_scale(ss, top, inv);
         if (threadIdx.x == 0) a.out_scale[row] = scale;
         inv *= scale > 0.0f ? 1.0f / scale : 1.0f;
     }
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_any_kernel(const __grid_cons
     }
     block_sum_max(ss, top, red);
     const float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
-    const float scale = top * inv * (1.0f / kE4m3Max);
+    const float scale = row_scale(ss, top, inv);
     const float mul = scale > 0.0f ? 1.0f / scale : 1.0f;
     if (kFp8 && threadIdx.x == 0) a.out_scale[row] = scale;
     for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {

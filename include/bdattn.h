@@ -536,7 +536,7 @@ int bdattn_add_row_bias(void* y, const void* bias, int rows, int cols, long long
  *   y = h * rsqrt(mean(h^2) + eps) * gain,
  *   out = y rounded to dtype (out_dtype = dtype), or, with out_dtype E4M3,
  *   out_scale[row] = max|y| / 448 and out = e4m3(y / out_scale[row]) (a row of zeros
- *   has scale 0; a row with a value that is not finite has scale NaN).
+ *   has scale 0; a row of x + residual with a value, or a sum of squares, that is not finite in FP32 has scale NaN).
  * The norm is that of the unrounded sum.  x, residual, residual_out (rows, cols) of
  * dtype BF16 / F16; residual, residual_out and gain may be NULL; gain_dtype F32 or
  * dtype.  residual_out may be residual or x (same ld), out may be x or residual

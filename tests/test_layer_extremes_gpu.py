@@ -33,3 +33,36 @@ def test_activations_of_large_sums(bd, M, N, K, act, fp8):
     nan = torch.full((N,), float("nan"), device="cuda", dtype=BF16)
     bd.linear_act_fwd(x, w, nan, y, act=act)
     assert torch.isnan(y).all()
+
+
+def norm(bd, x, residual=None, gain=None, eps=1e-6, skip=0):
+    """(values of 8 bits times their scale, scale, values); skip: elements that the rows lie off 16 bytes."""
+    rows, cols = x.shape
+    wide = lambda t: torch.nn.functional.pad(t, (skip, 8 - skip)) if skip else t
+    cut = lambda t: t[:, skip:skip + cols]
+    q = cut(wide(torch.zeros(rows, cols, device="cuda")).to(E4M3))
+    scale = torch.full((rows,), 7.0, device="cuda")
+    bd.add_rmsnorm_fwd(cut(wide(x)), q, gain, residual=None if residual is None else cut(wide(residual)), out_scale=scale, eps=eps)
+    return q.double() * scale.double()[:, None], scale, q
+
+
+# Kernels: a row to eight lanes, to a warp, to a CTA, wide rows read twice; rows off 16 bytes; tensors off by different numbers
+# of elements (the last column count)
+WIDTHS = [(4, 64, 0), (4, 512, 0), (200, 1024, 0), (3, 5120, 0), (300, 6000, 0), (2, 20000, 0), (4, 519, 3), (300, 5001, 3), (2, 20001, 5)]
+
+
+@pytest.mark.parametrize("rows,cols,skip", WIDTHS)
+@pytest.mark.parametrize("off", [False, True])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("gain", [0.0, 1.0])
+def test_rows_with_a_value_that_is_not_finite_have_scale_nan(bd, rows, cols, skip, off, value, gain):
+    """Whatever gain stands at the value's column."""
+    x = torch.ones(rows, cols, device="cuda", dtype=BF16)
+    for i, c in enumerate((0, cols // 2, cols - 1)):
+        x[i % rows, c] = value
+    bad = ~torch.isfinite(x).all(1)
+    w = torch.ones(cols, device="cuda", dtype=BF16)
+    w[[0, cols // 2, cols - 1]] = gain
+    r = torch.zeros(rows, cols + 5, device="cuda", dtype=BF16)[:, 5:] if off else None
+    got, scale, q = norm(bd, x, r, w, skip=skip)
+    assert torch.isnan(scale[bad]).all() and ((scale[~bad] * 448 - 1).abs() < 1e-5).all()
