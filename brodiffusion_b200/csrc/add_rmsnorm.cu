@@ -40,10 +40,24 @@ __device__ __forceinline__ void block_sum_max(float& s, float& m, float* red) {
     }
 }
 
-// The scale of a row's values of 8 bits.  The maximum of |h g| does not know of NaN, nor of an infinity under a gain of 0, but the
-// sum of squares does.  (A maximum that keeps NaN costs the row an instruction a value: 16384 x 5120 105.3 us, this way 104.1.)
-__device__ __forceinline__ float row_scale(float ss, float top, float inv) {
-    return ss <= FLT_MAX ? top * inv * (1.0f / kE4m3Max) : __uint_as_float(0x7fffffffu);
+// The scale of a row's values of 8 bits, and the factor that takes h g to them.
+// The maximum of |h g| does not know of NaN, nor of an infinity under a gain of 0, but the sum of squares does.  (A maximum that
+// keeps NaN costs the row an instruction a value: 16384 x 5120 105.3 us, this way 104.1.)  A row of zeros has scale 0 with
+// an eps of 0 too, where the root is infinite.  448 / top is beyond FP32 for the tiniest rows: these go through `lift`
+// times their values, which is uniform over a row and 1 for all others.
+struct RowScale {
+    float scale, factor, lift;
+};
+__device__ __forceinline__ RowScale row_scale(float ss, float top, float inv) {
+    RowScale r;
+    r.scale = !(ss <= FLT_MAX) ? __uint_as_float(0x7fffffffu) : top == 0.0f ? 0.0f : top * inv * (1.0f / kE4m3Max);
+    r.factor = r.scale > 0.0f ? inv * (1.0f / r.scale) : inv;
+    r.lift = 1.0f;
+    if (top < 0x1p-100f) {
+        r.lift = 0x1p100f;
+        r.factor = top > 0.0f ? kE4m3Max / (top * 0x1p100f) : 0.0f;
+    }
+    return r;
 }
 
 __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
@@ -197,9 +211,16 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) add_rm
         }
         float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
         if constexpr (kFp8) {
-            const float scale = row_scale(ss, top, inv);
-            if (exists && me == 0) a.out_scale[now] = scale;
-            inv *= scale > 0.0f ? 1.0f / scale : 1.0f;
+            const RowScale rs = row_scale(ss, top, inv);
+            if (exists && me == 0) a.out_scale[now] = rs.scale;
+            inv = rs.factor;
+            if (rs.lift != 1.0f) {
+#pragma unroll
+                for (int v = 0; v < kV; ++v) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[v][i] *= rs.lift;
+                }
+            }
         }
 #pragma unroll
         for (int v = 0; v < kV; ++v) {
@@ -243,18 +264,19 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_wide_kernel(const __grid_con
         }
     }
     block_sum_max(ss, top, red);
-    float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
+    float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps), lift = 1.0f;
     if constexpr (kFp8) {
-        const float scale = row_scale(ss, top, inv);
-        if (threadIdx.x == 0) a.out_scale[row] = scale;
-        inv *= scale > 0.0f ? 1.0f / scale : 1.0f;
+        const RowScale rs = row_scale(ss, top, inv);
+        if (threadIdx.x == 0) a.out_scale[row] = rs.scale;
+        inv = rs.factor;
+        lift = rs.lift;
     }
     for (int c = static_cast<int>(threadIdx.x) * 8 - s; c < a.cols; c += 8192) {
         float h[8], g[8];
         sum(c, h, g);
         if (a.residual_out != nullptr) norm_store<kBf16, kShift>(reinterpret_cast<uint16_t*>(a.residual_out) + row * a.ldro, c, a.cols, h);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] *= g[i] * inv;
+        for (int i = 0; i < 8; ++i) h[i] = kFp8 ? h[i] * g[i] * lift * inv : h[i] * (g[i] * inv);
         if constexpr (kFp8) norm_store_e4m3<kShift>(reinterpret_cast<uint8_t*>(a.out) + row * a.ldo, c, a.cols, h);
         else norm_store<kBf16, kShift>(reinterpret_cast<uint16_t*>(a.out) + row * a.ldo, c, a.cols, h);
     }
@@ -279,18 +301,17 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_any_kernel(const __grid_cons
     }
     block_sum_max(ss, top, red);
     const float inv = rsqrtf(ss / static_cast<float>(a.cols) + a.eps);
-    const float scale = row_scale(ss, top, inv);
-    const float mul = scale > 0.0f ? 1.0f / scale : 1.0f;
-    if (kFp8 && threadIdx.x == 0) a.out_scale[row] = scale;
+    const RowScale rs = row_scale(ss, top, inv);
+    if (kFp8 && threadIdx.x == 0) a.out_scale[row] = rs.scale;
     for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
         float h = load1<kBf16>(a.x, xo + c);
         if (a.residual != nullptr) h += load1<kBf16>(a.residual, ro + c);
         if (a.residual_out != nullptr) store1<kBf16>(a.residual_out, row * a.ldro + c, h);
-        const float y = h * inv * gain(c);
         if constexpr (kFp8)
-            reinterpret_cast<uint8_t*>(a.out)[row * a.ldo + c] = __nv_cvt_float_to_fp8(y * mul, __NV_SATFINITE, __NV_E4M3);
+            reinterpret_cast<uint8_t*>(a.out)[row * a.ldo + c] =
+                __nv_cvt_float_to_fp8(h * gain(c) * rs.lift * rs.factor, __NV_SATFINITE, __NV_E4M3);
         else
-            store1<kBf16>(a.out, row * a.ldo + c, y);
+            store1<kBf16>(a.out, row * a.ldo + c, h * inv * gain(c));
     }
 }
 

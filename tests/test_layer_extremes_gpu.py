@@ -66,3 +66,32 @@ def test_rows_with_a_value_that_is_not_finite_have_scale_nan(bd, rows, cols, ski
     r = torch.zeros(rows, cols + 5, device="cuda", dtype=BF16)[:, 5:] if off else None
     got, scale, q = norm(bd, x, r, w, skip=skip)
     assert torch.isnan(scale[bad]).all() and ((scale[~bad] * 448 - 1).abs() < 1e-5).all()
+
+
+@pytest.mark.parametrize("rows,cols,skip", WIDTHS)
+@pytest.mark.parametrize("off", [False, True])
+@pytest.mark.parametrize("size,gain", [(4e-37, 1.0), (1e-35, 1.0), (1e-20, 1e-17), (1e-30, 1.0), (1e-33, 0.5)])
+def test_rows_of_tiny_values_in_8_bits(bd, rows, cols, skip, off, size, gain):
+    """y = h g / sqrt(mean h^2 + eps) is representable, down to 1e-34 here, and its 8 bits are those of larger rows."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    # (magnitudes of 0.5 to 2 times the size: the smallest, 2e-37, is a normal number, as FP32 arithmetic here flushes others)
+    x = ((0.5 + 1.5 * torch.rand(rows, cols, device="cuda", generator=g)) * size).to(BF16)
+    x *= torch.where(torch.rand(rows, cols, device="cuda", generator=g) < 0.5, -1, 1)
+    x[:, 1] = 0
+    w = torch.full((cols + 1,), gain, device="cuda", dtype=torch.float32)[1:]
+    r = torch.zeros(rows, cols + 5, device="cuda", dtype=BF16)[:, 5:] if off else None
+    got, scale, q = norm(bd, x, r, w, skip=skip)
+    y = x.double() * w.double() / torch.sqrt(x.double().square().mean(1, keepdim=True) + 1e-6)
+    assert ((scale.double() - y.abs().amax(1) / 448).abs() <= 1e-5 * y.abs().amax(1) / 448).all()
+    # e4m3 rounding, 2^-4 of a value from 2^-6 on (all but the zeros are above 448 / 4)
+    assert ((got - y).abs() <= (2.0 ** -4 + 2e-5) * y.abs()).all()
+    assert (q[:, 1].float() == 0).all()
+
+
+@pytest.mark.parametrize("rows,cols,skip", WIDTHS)
+def test_rows_of_zeros_without_an_epsilon_have_scale_0(bd, rows, cols, skip):
+    x = torch.ones(rows, cols, device="cuda", dtype=BF16)
+    x[::2] = 0
+    got, scale, q = norm(bd, x, eps=0.0, skip=skip)
+    assert (scale[::2] == 0).all() and (q[::2].float() == 0).all()
+    assert ((scale[1::2] * 448 - 1).abs() < 1e-5).all() and (q[1::2].float() == 448).all()
