@@ -113,7 +113,8 @@ __device__ __forceinline__ void norm_store_e4m3(void* row, int c, int cols, cons
             if (c + i >= 0 && c + i < cols) p[i] = static_cast<uint8_t>(w[i >> 2] >> (8 * (i & 3)));
     }
 }
-// Eight gains from element c on (on 16 bytes without kShift).
+// Eight gains from element c on (on 16 bytes without kShift).  Not through the read-only path: the kernel before this one may
+// write them, and still run when this one is resident.
 template <bool kBf16, bool kShift>
 __device__ __forceinline__ void norm_gains(const AddRmsNormArgs& a, int c, float (&g)[8]) {
     if (a.gain == nullptr) {
@@ -121,12 +122,12 @@ __device__ __forceinline__ void norm_gains(const AddRmsNormArgs& a, int c, float
         for (int i = 0; i < 8; ++i) g[i] = 1.0f;
     } else if (a.gain_is_f32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = !kShift || (c + i >= 0 && c + i < a.cols) ? __ldg(reinterpret_cast<const float*>(a.gain) + c + i) : 0.0f;
+        for (int i = 0; i < 8; ++i) g[i] = !kShift || (c + i >= 0 && c + i < a.cols) ? reinterpret_cast<const float*>(a.gain)[c + i] : 0.0f;
     } else if (kShift) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = c + i >= 0 && c + i < a.cols ? load1<kBf16>(a.gain, c + i) : 0.0f;
     } else {
-        norm_wide<kBf16>(__ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.gain) + c)), g);
+        norm_wide<kBf16>(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.gain) + c), g);
     }
 }
 
@@ -188,10 +189,10 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) add_rm
         for (int v = 0; v < kV; ++v) {
             const int c = (me + v * team) * 8 - s;
             if (exists && c < a.cols) {
-                if (a.residual_out != nullptr)
-                    norm_store<kBf16, kShift>(reinterpret_cast<uint16_t*>(a.residual_out) + now * a.ldro, c, a.cols, y[v]);
                 float g[8];
                 norm_gains<kBf16, kShift>(a, c, g);
+                if (a.residual_out != nullptr)
+                    norm_store<kBf16, kShift>(reinterpret_cast<uint16_t*>(a.residual_out) + now * a.ldro, c, a.cols, y[v]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     y[v][i] *= g[i];
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_any_kernel(const __grid_cons
     const long long row = blockIdx.x;
     const long long xo = row * a.ldx, ro = row * a.ldr;
     auto gain = [&](int c) {
-        return a.gain == nullptr ? 1.0f : a.gain_is_f32 ? __ldg(reinterpret_cast<const float*>(a.gain) + c) : load1<kBf16>(a.gain, c);
+        return a.gain == nullptr ? 1.0f : a.gain_is_f32 ? reinterpret_cast<const float*>(a.gain)[c] : load1<kBf16>(a.gain, c);
     };
     float ss = 0.0f, top = 0.0f;
     for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {

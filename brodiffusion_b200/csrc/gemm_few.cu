@@ -158,7 +158,7 @@ gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
         if (m >= p.M || n >= p.N) continue;
         float f[1] = {0.0f};
         for (int k = 0; k < a.parts; ++k) f[0] += parts_s[k][i];
-        if (kFp8) f[0] *= (p.x_scale != nullptr ? load_scale(p.x_scale + m) : 1.0f) * (p.w_scale != nullptr ? __ldg(p.w_scale + n) : 1.0f);
+        if (kFp8) f[0] *= (p.x_scale != nullptr ? load_scale(p.x_scale + m) : 1.0f) * (p.w_scale != nullptr ? load_scale(p.w_scale + n) : 1.0f);
         if (p.bias != nullptr) f[0] += layer_ld16<kBf16>(p.bias, n);
         activate(f, p.act);
         if (p.gate != nullptr) f[0] *= layer_ld16<kBf16>(p.gate, n);

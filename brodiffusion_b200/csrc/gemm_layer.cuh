@@ -53,8 +53,8 @@ __device__ __forceinline__ float2 layer_pair(uint32_t w) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// A row's scale.  Not through the read-only path: the kernel before this one writes it, and may still run when
-// this one is resident.
+// A scale.  Not through the read-only path: the kernel before this one may write it, and still run when this one is
+// resident.
 __device__ __forceinline__ float load_scale(const float* p) {
     float v;
     asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
@@ -65,7 +65,7 @@ __device__ __forceinline__ float load_scale(const float* p) {
 template <bool kBf16>
 __device__ __forceinline__ void layer_columns(const GemmProblem& p, float* cols, int n, int i, long long column, bool on) {
     cols[i] = on && p.bias != nullptr ? layer_ld16<kBf16>(p.bias, column) : 0.0f;
-    cols[n + i] = on && p.w_scale != nullptr ? __ldg(p.w_scale + column) : 1.0f;
+    cols[n + i] = on && p.w_scale != nullptr ? load_scale(p.w_scale + column) : 1.0f;
     cols[2 * n + i] = on && p.gate != nullptr ? layer_ld16<kBf16>(p.gate, column) : 1.0f;
 }
 

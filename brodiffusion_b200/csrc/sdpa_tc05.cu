@@ -329,7 +329,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     const int c = lane + 32 * w;
-                    mv[w] = c < ti.valid ? __ldg(a.key_mask + ti.kbase + c) : 0.0f;
+                    mv[w] = c < ti.valid ? a.key_mask[ti.kbase + c] : 0.0f;
                 }
                 const bool seen = __any_sync(0xffffffffu, mv[0] != 0.0f || mv[1] != 0.0f || mv[2] != 0.0f || mv[3] != 0.0f);
                 bool hidden = false;
@@ -524,7 +524,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const int c = 4 * lane + w;
-                        mv[w] = c < tm.valid ? __ldg(a.key_mask + tm.kbase + c) : 1.0f;
+                        mv[w] = c < tm.valid ? a.key_mask[tm.kbase + c] : 1.0f;
                     }
 #pragma unroll
                     for (int w = 0; w < 4; ++w) mbits[w] = __ballot_sync(0xffffffffu, mv[w] != 0.0f);

@@ -213,7 +213,7 @@ sdpa_few_kernel(const __grid_constant__ CUtensorMap tmK0, const __grid_constant_
             key0 += key_w;
             // which of the warp's keys exist and are let through by the key mask, one to a lane
             bool on = lane < 16 * KT && key_w + lane < n;
-            if (a.key_mask != nullptr && on) on = __ldg(a.key_mask + key0 + lane) != 0.0f;
+            if (a.key_mask != nullptr && on) on = a.key_mask[key0 + lane] != 0.0f;
             const uint32_t live = __ballot_sync(0xffffffffu, on);
             // A slot may pass from one group of warps to another.  That the slot's last user has released it says that its last
             // copy had landed: without this wait a group that is ahead could find the phase before that copy

@@ -14,7 +14,8 @@
 namespace bdattn {
 
 // Keys of batch item b.  The lengths lie in device memory, where the host cannot check them: one outside
-// [0, Lk] counts as the nearer end.  (Not read through the read-only path: the kernel before this one may write them.)
+// [0, Lk] counts as the nearer end.  (Neither they nor the key mask are read through the read-only path: the kernel before
+// this one may write them.)
 __device__ __forceinline__ int window_keys(const int* kv_len, int batch, int lk) {
     if (kv_len == nullptr) return lk;
     int n;
@@ -72,7 +73,7 @@ __device__ __noinline__ void window_row(const SdpaWindowArgs& a, int batch, int 
         const int begin = part ? span.win_begin : 0, end = part ? span.win_end : span.sink_end;
         for (int j0 = begin; j0 < end; j0 += 32) {
             const int j = j0 + lane;
-            const bool on = j < end && (a.key_mask == nullptr || __ldg(a.key_mask + j) != 0.0f);
+            const bool on = j < end && (a.key_mask == nullptr || a.key_mask[j] != 0.0f);
             const uint32_t seen = __ballot_sync(0xffffffffu, on);
             if (seen == 0) continue;
             float s = -INFINITY;
