@@ -59,7 +59,7 @@ class CausalLayer:
 
     def forward(self, stream, cache, cos, sin):
         """``stream`` (B, L, D): the hidden states of L new tokens of every sequence, updated in place.  Their K and V go
-        behind the cache's rows."""
+        behind the cache's rows.  A call that raises leaves the cache's lengths as they were (the stream may be half updated)."""
         import torch
         B, L, D = stream.shape
         w, nh, nkv, hd = self.w, self.nh, self.nkv, self.hd
@@ -83,18 +83,27 @@ class CausalLayer:
             bd.rmsnorm_rope([job(k, cache.k[b, cache.filled[b]:cache.filled[b] + L], "k_gain", b) for b in group], nkv, hd, eps=self.eps)
         for b in range(B):
             cache.v[b, cache.filled[b]:cache.filled[b] + L].copy_(v[b])
-            cache.filled[b] += L
         cache.lengths += L
-        att = new(B, L, nh * hd)
-        # (no row behind the longest sequence is looked at)
-        most = max(cache.filled)
-        bd.sdpa_window_fwd(q, cache.k[:, :most], cache.v[:, :most], att, nh, window=self.window, sinks=self.sinks,
-                           num_kv_heads=nkv, kv_len=cache.lengths)
-        branch = new(B * L, D)
-        bd.linear_act_fwd(att.view(B * L, -1), w["wo"], None, branch)
+        try:
+            self._behind_the_cache(rows, q, cache, max(cache.filled) + L)
+        except BaseException:
+            cache.lengths -= L               # the rows behind the lengths are nobody's
+            raise
+        cache.filled[:] = [n + L for n in cache.filled]
+        return stream
+
+    def _behind_the_cache(self, rows, q, cache, most):
+        """Attention over the first ``most`` rows of the cache (no row behind the longest sequence is looked at) and what follows."""
+        import torch
+        w, D = self.w, rows.shape[1]
+        new = lambda *shape: torch.empty(*shape, device=rows.device, dtype=rows.dtype)
+        att = new(q.shape)
+        bd.sdpa_window_fwd(q, cache.k[:, :most], cache.v[:, :most], att, self.nh, window=self.window, sinks=self.sinks,
+                           num_kv_heads=self.nkv, kv_len=cache.lengths)
+        branch = new(len(rows), D)
+        bd.linear_act_fwd(att.view(len(rows), -1), w["wo"], None, branch)
 
         x8, xs = self._rows8(branch, w["norm2"], residual=rows, residual_out=rows)
-        hidden = new(B * L, w["w_up"].shape[0])
+        hidden = new(len(rows), w["w_up"].shape[0])
         bd.linear_act_fwd(x8, self.w_up, w.get("b_up"), hidden, act=self.act, x_scale=xs, w_scale=self.w_up_scale)
         bd.linear_act_fwd(hidden, w["w_down"], w.get("b_down"), rows, residual=rows)
-        return stream
