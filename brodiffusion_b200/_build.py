@@ -22,13 +22,21 @@ NVCC_FLAGS = [
 BINDING_PATH = os.path.join(PKG_DIR, "_binding.so")
 
 
-def build_binding(force: bool = False) -> str:
+def build_binding(force: bool = False):
+    """Compile ``_binding.so``; without a torch that has CUDA there is nothing to bind (None), and the library stands alone."""
     src = os.path.join(CSRC, "binding.cpp")
     header = os.path.join(PKG_DIR, "..", "include", "bdattn.h")
     if not force and os.path.exists(BINDING_PATH) and os.path.getmtime(BINDING_PATH) >= max(map(os.path.getmtime, (src, header))):
         return BINDING_PATH
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ModuleNotFoundError as e:
+        if e.name != "torch":
+            raise
+        return None
+    if torch.version.cuda is None:
+        return None
     from torch.utils import cpp_extension
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
