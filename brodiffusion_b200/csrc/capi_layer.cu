@@ -85,6 +85,8 @@ int bdattn_add_rmsnorm_fwd(const bdattn_add_rmsnorm_params* p, bdattn_stream_t s
     const bool fp8 = p->out_dtype == BDATTN_E4M3;
     if (!fp8 && p->out_dtype != p->dtype) return fail("%s: out_dtype must be dtype or E4M3 (got %d)", op, p->out_dtype);
     if (p->rows < 0 || p->cols < 1) return fail("%s: rows must be >= 0 and cols >= 1 (got %d and %d)", op, p->rows, p->cols);
+    // (a thread's column goes on by 8192 past the last one)
+    if (p->cols > INT32_MAX - 8192) return fail("%s: more than 2^31 - 8193 columns (got %d)", op, p->cols);
     if (p->rows == 0) return 0;
     if (p->x == nullptr || p->out == nullptr) return fail("%s: x/out is null", op);
     if (fp8 && p->out_scale == nullptr) return fail("%s: E4M3 output needs out_scale", op);

@@ -540,7 +540,7 @@ int bdattn_add_row_bias(void* y, const void* bias, int rows, int cols, long long
  * The norm is that of the unrounded sum.  x, residual, residual_out (rows, cols) of
  * dtype BF16 / F16; residual, residual_out and gain may be NULL; gain_dtype F32 or
  * dtype.  residual_out may be residual or x (same ld), out may be x or residual
- * where its dtype is theirs.  Any cols >= 1, any alignment of the element type and any ld >= cols;
+ * where its dtype is theirs.  Any cols from 1 to 2^31 - 8193, any alignment of the element type and any ld >= cols;
  * rows of 16-byte alignment with cols and ld multiples of 8 are the fast ones. */
 typedef struct bdattn_add_rmsnorm_params {
     int dtype;

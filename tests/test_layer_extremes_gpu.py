@@ -95,3 +95,13 @@ def test_rows_of_zeros_without_an_epsilon_have_scale_0(bd, rows, cols, skip):
     got, scale, q = norm(bd, x, eps=0.0, skip=skip)
     assert (scale[::2] == 0).all() and (q[::2].float() == 0).all()
     assert ((scale[1::2] * 448 - 1).abs() < 1e-5).all() and (q[1::2].float() == 448).all()
+
+
+@pytest.mark.parametrize("cols", [2 ** 31 - 1, 2 ** 31 - 8192])
+@pytest.mark.parametrize("out_dtype", ["BF16", "E4M3"])
+def test_rows_whose_columns_pass_32_bits_are_refused(bd, cols, out_dtype):
+    """(By the host, ahead of the addresses: nothing is launched.)"""
+    p = bd.AddRmsNormParams(dtype=bd.BF16, rows=1, cols=cols, out_dtype=getattr(bd, out_dtype))
+    assert bd.lib().bdattn_add_rmsnorm_fwd(p, None) == -1 and "columns" in bd.last_error()
+    p.cols = 2 ** 31 - 8193
+    assert bd.lib().bdattn_add_rmsnorm_fwd(p, None) == -1 and "null" in bd.last_error()
