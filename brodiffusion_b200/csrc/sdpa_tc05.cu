@@ -8,8 +8,9 @@
 //   warp  8    : issues the Q.K^T MMAs (one lane), owns the TMEM allocation
 //   warp  9    : TMA producer for Q, K and V tiles (one lane)
 //   warp  10   : issues the P.V MMAs (one lane)
-//   warp  11   : idle (it completes the third warpgroup, so that registers can be moved
-//                to the softmax warpgroups with setmaxnreg)
+//   warp  11   : with a window, and lengths or a key mask: takes what hidden rows of a V tile hold out of it
+//                (hide_rows); otherwise idle (it completes the third warpgroup, so that registers can
+//                be moved to the softmax warpgroups with setmaxnreg)
 //   warps 12-15: only with per-key scale vectors (kScale): multiply the rows of a K or V
 //                tile in shared memory by their factors before the MMAs read it, 32
 //                rows each
@@ -164,6 +165,59 @@ __device__ __forceinline__ void setmaxnreg_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// With a window: whether a call has rows that no query may see.
+template <int kHooks>
+__device__ __forceinline__ bool hides_rows(const SdpaDevArgsWindow& a) { return kHooks >= 1 || a.w.kv_len != nullptr; }
+template <int kHooks>
+__device__ __forceinline__ bool hides_rows(const SdpaDevArgs&) { return false; }
+// Writes zeros over the rows of the V tiles that no query may see, from key `keys` on or under the key mask, and hands the
+// tiles on from v_full to v_ready: a warp by itself, which walks all tiles in order (it sees every phase of the barriers
+// it waits on).  A lane has the rows `lane` + 32 w; which of them are hidden is looked up a tile ahead.
+// Not inlined: with this code beside it the softmax code came out slower whether this ran or not (prompts of 2 x 1536 tokens, 24 heads
+// of 128, a masked start and window 300: 37.8 us, 39.4 with code that never ran).
+template <class C, int kHooks>
+__device__ __noinline__ void hide_rows(const SdpaDevArgsWindow& a, uint8_t* smem_v, uint64_t* v_full, uint64_t* v_ready,
+                                       const uint16_t* tile_list, int n_kv, int n_sink, int skip, int keys) {
+    const int lane = threadIdx.x & 31;
+    uint32_t hidden = 0;          // bit w: row lane + 32 w
+    auto look = [&](int j) {
+        hidden = 0;
+        if (j >= n_kv) return;
+        const int entry = tile_list != nullptr ? tile_list[j] : j >= n_sink ? j + skip : j;
+        const TileInfo ti = kv_tile(a, tile_list != nullptr ? entry & (kPartTile - 1) : entry);
+        const bool masked = kHooks >= 1 && a.key_mask != nullptr && (tile_list == nullptr || (entry & kPartTile) != 0);
+        if (!masked && keys - ti.kbase >= ti.valid) return;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int c = lane + 32 * w;
+            if (c < ti.valid && (ti.kbase + c >= keys || (masked && a.key_mask[ti.kbase + c] == 0.0f))) hidden |= 1u << w;
+        }
+    };
+    look(0);
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int j = 0; j < n_kv; ++j) {
+        if (!mbar_wait_warp(&v_full[slot], phase)) return;
+        if (__any_sync(0xffffffffu, hidden != 0)) {
+            // the pieces of a row in an order of the lane's own: eight rows of an access fall into different banks
+            uint8_t* const tile = smem_v + slot * C::kTileBytes + lane * 128;
+#pragma unroll 1
+            for (int w = 0; w < 4; ++w) {
+                if ((hidden >> w) & 1u) {
+#pragma unroll
+                    for (int i = 0; i < 8 * C::kChunks; ++i)
+                        *reinterpret_cast<uint4*>(tile + w * 4096 + (i >> 3) * kChunkBytes + (((i & 7) ^ (lane & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+            fence_proxy_async_smem();      // the MMA reads the tile through the async proxy
+            __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&v_ready[slot]);
+        if (++slot == C::kVStages) { slot = 0; phase ^= 1; }
+        look(j + 1);
+    }
+}
+
 // HOOKS: 0 = none; 1 = key_mask only; 2 = key_mask and the per-row softmax statistics; 3 = a logit
 // bias besides (slower softmax path); 4 = a bias of a few rows, read without shared memory (launch_hd).
 // SCALE: key_scale / val_scale are applied to the K / V tiles in shared memory by
@@ -173,8 +227,11 @@ __device__ __forceinline__ void setmaxnreg_dec() {
 // kMixed: some CTAs of the launch have one query tile (launch_t); without it every CTA has two.
 // kWindow: causal with a sliding window and visible first keys (sdpa_window.cuh).  A CTA visits the key tiles that
 // some row of it sees, those of the sinks and those of the window, and nothing between; a column that a row does not see is
-// hidden by its number in the tiles at the ends.  A weight of zero times a value that is not finite is NaN: rows that
-// come out so, though their weights are finite, are worked out again from the visible keys alone.
+// hidden by its number in the tiles at the ends.  A weight of zero times a value that is not finite is NaN.  Rows of V that no
+// query may see, behind the length or under the key mask, can hold anything: they become zeros in shared memory (hide_rows), and
+// the outputs do not depend on them (prompts of 2 x 1536 tokens with NaN in such rows: 4 to 40 ms, this way 16 to 67 us; with numbers
+// in them 16 to 63 us without it).  Rows that some queries see and others do not stay: query rows that come out so,
+// though their weights are finite, are worked out again from the visible keys alone.
 template <int HD, bool kBf16, int kHooks, bool kScale, bool kMixed, bool kWindow = false>
 __global__ void __launch_bounds__(Roles<kScale>::kThreads, 1)
 sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant__ CUtensorMap tmQ1,
@@ -202,7 +259,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
     uint64_t* k_ready = k_empty + KS;    // [KS] tile landed and, where needed, scaled (kScale)
     uint64_t* v_full = k_ready + KS;     // [VS]
     uint64_t* v_empty = v_full + VS;     // [VS]
-    uint64_t* v_ready = v_empty + VS;    // [VS]
+    uint64_t* v_ready = v_empty + VS;    // [VS] the same; with kWindow the tile's hidden rows are zeros
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(v_ready + VS);
     uint16_t* tile_list = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(bars) + C::kBarBytes);   // [kMaxListed]
 
@@ -253,7 +310,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
         for (int i = 0; i < VS; ++i) {
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
-            mbar_init(&v_ready[i], 4);
+            mbar_init(&v_ready[i], kWindow ? 1 : 4);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 1);
@@ -877,7 +934,7 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
             // -------------------------------------------------- P.V issuer
             constexpr uint32_t idesc_pv = make_idesc_f16(kBf16 ? 1 : 0, kBM, HD, 0, 1);
             const uint32_t v_base = smem_u32(smem_v);
-            uint64_t* const v_rdy = kScale ? v_ready : v_full;
+            uint64_t* const v_rdy = kScale || (kWindow && hides_rows<kHooks>(a)) ? v_ready : v_full;
             int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -944,6 +1001,10 @@ sdpa_tc05_kernel(const __grid_constant__ CUtensorMap tmQ0, const __grid_constant
                 }
             }
             __syncwarp();
+        } else if (kWindow && warp == 11) {
+            if constexpr (kWindow)
+                if (hides_rows<kHooks>(a))
+                    hide_rows<C, kHooks>(a, smem_v, v_full, v_ready, listed ? tile_list : nullptr, n_kv, n_sink, skip, q_offset + a.lq_total);
         } else if (kScale && warp >= 12) {
             // ------------------------------------------- K / V row scaling
             // The four warps walk the K and V tiles in order (they see every phase of the barriers they
