@@ -216,10 +216,11 @@ struct Rows {
         batch = d == 3 ? rows_of(t.size(0), what) : 1;
         rows = rows_of(t.size(d - 2), what);
         cols = rows_of(t.size(d - 1), what);
-        if (t.stride(d - 1) != 1) refuse(what, "must have contiguous columns");
-        ld = t.stride(d - 2);
-        stride = d == 3 ? t.stride(0) : 0;
-        if (batch > 1 && stride == 0) refuse(what, "has the same memory for several batch items");     // (0 stands for dense ones)
+        if (cols > 1 && t.stride(d - 1) != 1) refuse(what, "must have contiguous columns");
+        // (the strides of a single row and a single item may be anything; 0 stands for dense items)
+        ld = rows > 1 ? t.stride(d - 2) : cols;
+        stride = batch > 1 ? t.stride(0) : 0;
+        if (batch > 1 && stride == 0) refuse(what, "has the same memory for several batch items");
         data = t.data_ptr();
     }
 };
