@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) add_rm
     constexpr int kSide = kTeam > 0 ? 128 / (kTeam > 0 ? kTeam : 1) : 1;       // rows side by side
     const int team = kTeam > 0 ? kTeam : static_cast<int>(blockDim.x);
     const int me = kTeam > 0 ? static_cast<int>(threadIdx.x) & (kTeam - 1) : static_cast<int>(threadIdx.x);
-    if (gridDim.x <= 148) dependents_may_launch();
+    if (a.one_wave) dependents_may_launch();
     wait_for_prior_grid();
     auto shift_of = [&](long long row) { return kShift ? static_cast<int>((a.shift + row * a.ldx) & 7) : 0; };
     uint4 x[kV], r[kV];
@@ -348,6 +348,7 @@ cudaError_t launch_norm(AddRmsNormArgs a, cudaStream_t stream) {
     auto go = [&](auto kern, int side, int threads) {
         const int most = resident_ctas(reinterpret_cast<const void*>(kern), threads);
         const long long ctas = (a.rows + side - 1) / side;
+        a.one_wave = ctas <= sm_count();
         return launch_dependent(kern, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(threads), 0, stream, a);
     };
     auto pick = [&](auto shift) {

@@ -75,7 +75,6 @@ gemm_few_kernel(const __grid_constant__ GemmFewArgs a) {
     if (a.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     dependents_may_launch();
     // While the kernel before this one ends, the first weights come into the L2.
-    // While the kernel before this one ends, the first weights come into the L2.
     if (lane < 16 && n > 0) {
         const uint16_t* const at = a.w + static_cast<long long>(min(n0 + lane, p.N - 1)) * a.ldw + first * 64;
 #pragma unroll

@@ -251,6 +251,7 @@ struct AddRmsNormArgs {
     long long ldx, ldr, ldro, ldo;
     float eps;
     int shift;                 // set by the launch: elements that x lies off 16 bytes
+    bool one_wave;             // set by the launch: no more CTAs than SMs
 };
 cudaError_t launch_add_rmsnorm(const AddRmsNormArgs& a, bool bf16, bool fp8, cudaStream_t stream);
 
