@@ -1,8 +1,9 @@
 // The calls of a decoding step from Python: torch tensors to the parameter structures of include/bdattn.h.
-// A step of a layer makes eight calls whose kernels take 2 to 6 us; shapes, strides and pointers
-// looked up as Python attributes took half of the host's time for one (add_rmsnorm_fwd of one row 4.2 -> 2.5 us a call,
+// A step of a layer makes seven of these calls, and two of rmsnorm_rope for every four sequences, with kernels of 2 to 6 us;
+// shapes, strides and pointers looked up as Python attributes took half of the host's time for one (add_rmsnorm_fwd of one row 4.2 -> 2.5 us a call,
 // linear_act_fwd 4.9 -> 2.9, sdpa_window_fwd 6.2 -> 3.3; the launch itself is 2.3).  What is checked here is what the library
-// cannot see: that the tensors fit one another.  Everything else it refuses itself.
+// cannot see: that the tensors fit one another, that rows and items are memory of their own, and that all of it lies on the
+// current GPU.  Everything else it refuses itself.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>

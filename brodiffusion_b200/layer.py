@@ -11,7 +11,9 @@ prefix layers in front of a denoiser, put together as such a layer uses them.
     stream           <- linear_act_fwd  (16-bit down projection, the residual in its epilogue)
 
 A call takes any number of new tokens of every sequence: a whole prompt, a chunk of it, one
-token.  Torch provides memory only; nothing is kept between calls but the weights and the cache.
+token.  Torch provides memory, the copy of V's new rows into the cache (one a sequence) and the addition to the lengths; nothing
+is kept between calls but the weights and the cache.  Where the new rows go and the RoPE positions are numbers of the host, so a
+captured call would write the same rows again: of the calls above only the attention follows lengths on the device.
 """
 from __future__ import annotations
 

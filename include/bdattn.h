@@ -603,8 +603,10 @@ int bdattn_linear_act_fwd(const bdattn_linear_act_params* p, bdattn_stream_t str
  *   j <= P  and  (window == 0  or  j > P - window  or  j < sinks)  and  key_mask[j] != 0
  * (window counts the query's own key).  A query that sees nothing, one before the first key included,
  * gives zeros.  What masked places hold reaches no output, infinities and NaN included, and rows
- * past kv_len[b] need not be initialised.
- *   p       as for bdattn_sdpa_fwd: segments, strides, batch, grouped heads, key_mask, softmax_scale;
+ * past kv_len[b] need not be initialised.  (A row of V that some queries of a prompt see and others do not, with a value that is
+ * not finite, costs time: the output rows that it would spoil are worked out one by one.)
+ *   p       as for bdattn_sdpa_fwd: segments, strides, batch, grouped heads, key_mask (one row for all
+ *           batch items), softmax_scale;
  *           mask_mode must be CAUSAL; no per-key scales and no fused query norm / RoPE
  *   kv_len  batch ints in device memory, read by the kernel (a captured graph follows their
  *           growth); a value outside [0, Lk] counts as the nearer end
