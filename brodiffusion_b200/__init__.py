@@ -22,7 +22,8 @@ __all__ = [
     "ROPE_INTERLEAVED", "ROPE_HALF_SPLIT", "SdpaParams", "NormRopeJob", "sdpa_fwd",
     "rmsnorm_rope", "linear_attn_relu_fwd", "rope_tables_flux", "rope_tables_qwen", "RopeSegment", "device_status", "last_error",
     "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd", "WindowParams", "sdpa_window_fwd", "LinearActParams",
-    "linear_act_fwd",
+    "linear_act_fwd", "SandwichNormParams", "sandwich_norm_fwd", "LinearW4Params", "w4_bytes", "w4_pack", "linear_w4_fwd",
+    "Cache4", "Cache4Params", "Cache4Rows", "SdpaCache4Params", "cache4_append", "cache4_read", "sdpa_cache4_fwd",
 ]
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 16
@@ -139,6 +140,59 @@ class LinearActParams(C.Structure):
     ]
 
 
+class SandwichNormParams(C.Structure):
+    """Mirror of ``bdattn_sandwich_norm_params`` (include/bdattn.h)."""
+    _fields_ = [
+        ("dtype", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("residual_out", C.c_void_p),
+        ("post_gain", C.c_void_p), ("gain", C.c_void_p), ("gain_dtype", C.c_int),
+        ("gate", C.c_void_p), ("gates", C.c_int), ("gate_ld", C.c_longlong), ("residual_scale", C.c_float),
+        ("out", C.c_void_p), ("out_dtype", C.c_int), ("out_scale", C.c_void_p),
+        ("x_ld", C.c_longlong), ("residual_ld", C.c_longlong), ("residual_out_ld", C.c_longlong),
+        ("out_ld", C.c_longlong), ("eps", C.c_float),
+    ]
+
+
+class LinearW4Params(C.Structure):
+    """Mirror of ``bdattn_linear_w4_params`` (include/bdattn.h)."""
+    _fields_ = [
+        ("dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("group", C.c_int),
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("gate", C.c_void_p), ("residual", C.c_void_p),
+        ("y", C.c_void_p), ("act", C.c_int),
+        ("x_ld", C.c_longlong), ("residual_ld", C.c_longlong), ("y_ld", C.c_longlong),
+    ]
+
+
+class Cache4Params(C.Structure):
+    """Mirror of ``bdattn_cache4`` (include/bdattn.h)."""
+    _fields_ = [
+        ("dtype", C.c_int), ("batch", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("group", C.c_int),
+        ("rows", C.c_int),
+        ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("codes_batch_stride", C.c_longlong), ("codes_head_stride", C.c_longlong),
+        ("scales_batch_stride", C.c_longlong), ("scales_head_stride", C.c_longlong),
+    ]
+
+
+class Cache4Rows(C.Structure):
+    """Mirror of ``bdattn_cache4_rows`` (include/bdattn.h)."""
+    _fields_ = [
+        ("rows", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_ld", C.c_longlong), ("v_ld", C.c_longlong), ("k_batch_stride", C.c_longlong),
+        ("v_batch_stride", C.c_longlong), ("kv_len", C.c_void_p),
+    ]
+
+
+class SdpaCache4Params(C.Structure):
+    """Mirror of ``bdattn_sdpa_cache4_params`` (include/bdattn.h)."""
+    _fields_ = [
+        ("num_heads", C.c_int), ("q_rows", C.c_int), ("q", C.c_void_p), ("o", C.c_void_p),
+        ("q_ld", C.c_longlong), ("o_ld", C.c_longlong), ("q_batch_stride", C.c_longlong),
+        ("o_batch_stride", C.c_longlong), ("window", C.c_int), ("sinks", C.c_int),
+        ("kv_len", C.c_void_p), ("key_mask", C.c_void_p), ("softmax_scale", C.c_float),
+    ]
+
+
 _FORMATS = {C.c_int: "i", C.c_longlong: "q", C.c_float: "f", C.c_void_p: "P", C.c_size_t: "N"}
 
 
@@ -239,6 +293,15 @@ def lib():
         L.bdattn_sdpa_window_fwd.argtypes = [C.POINTER(SdpaParams), C.POINTER(WindowParams), C.c_void_p]
         L.bdattn_linear_act_fwd.argtypes = [C.POINTER(LinearActParams), C.c_void_p]
         L.bdattn_add_rmsnorm_fwd.argtypes = [C.POINTER(AddRmsNormParams), C.c_void_p]
+        L.bdattn_sandwich_norm_fwd.argtypes = [C.POINTER(SandwichNormParams), C.c_void_p]
+        L.bdattn_w4_bytes.restype = C.c_size_t
+        L.bdattn_w4_bytes.argtypes = [C.c_int] * 3
+        L.bdattn_w4_pack.argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                     C.c_void_p]
+        L.bdattn_linear_w4_fwd.argtypes = [C.POINTER(LinearW4Params), C.c_void_p]
+        L.bdattn_cache4_append.argtypes = [C.POINTER(Cache4Params), C.POINTER(Cache4Rows), C.c_void_p]
+        L.bdattn_cache4_read.argtypes = [C.POINTER(Cache4Params), C.POINTER(Cache4Rows), C.c_void_p]
+        L.bdattn_sdpa_cache4_fwd.argtypes = [C.POINTER(Cache4Params), C.POINTER(SdpaCache4Params), C.c_void_p]
         # The same entry points for this module's own calls, which pass packed structures (bytes) as pointers
         for name in ("sdpa_fwd", "sdpa_fwd_allgather", "sdpa_fwd_allgather_multicast", "mgpu_sdpa_fwd_headsharded",
                      "sdpa_traced_fwd", "rmsnorm_rope", "qkvo_fwd", "qkvo_fwd_static", "qkv_norm_rope_fwd",
@@ -733,3 +796,77 @@ def linear_act_fwd(x, w, bias, y, *, act="none", gate=None, residual=None, x_sca
         raise BdattnError(f"unknown activation {act!r} (one of {', '.join(ACTIVATIONS)})")
     (_binding or _load_binding()).linear_act(x, w, bias, y, code, gate, residual, x_scale, w_scale,
                                              None if stream is None else stream.cuda_stream)
+
+
+def sandwich_norm_fwd(x, residual, residual_out, post_gain=None, *, gate=None, residual_scale=1.0, gain=None, out=None,
+                      out_scale=None, eps=1e-6, stream=None):
+    """``bdattn_sandwich_norm_fwd``: h = residual_scale * residual + gate * rmsnorm(x) * post_gain, residual_out = h,
+    out = rmsnorm(h) * gain (None: left out; e4m3 with out_scale as in ``add_rmsnorm_fwd``).  gate: (cols), or (n, cols)
+    with a vector for each rows / n rows."""
+    (_binding or _load_binding()).sandwich_norm(x, residual, residual_out, post_gain, gate, residual_scale, gain, out, out_scale, eps,
+                                                None if stream is None else stream.cuda_stream)
+
+
+def w4_bytes(rows, cols, group) -> int:
+    """Bytes of a packed (rows, cols) matrix of 4-bit weights."""
+    return int(lib().bdattn_w4_bytes(rows, cols, group))
+
+
+def w4_pack(codes, scales, packed, *, group, stream=None):
+    """``bdattn_w4_pack``: codes (N, K / 2) uint8, two columns a byte with the even one in the low half, and scales
+    (N, ceil(K / group), 2), the (step, low) pairs of w = low + step * code, into packed (``w4_bytes`` uint8)."""
+    (_binding or _load_binding()).w4_pack(codes, scales, packed, group, None if stream is None else stream.cuda_stream)
+
+
+def linear_w4_fwd(x, w, bias, y, *, group, act="none", gate=None, residual=None, stream=None):
+    """``bdattn_linear_w4_fwd``: y = residual + gate * act(x @ W.T + bias) with W packed by ``w4_pack`` (of pairs of the type
+    of x).  act: a key of ``ACTIVATIONS``."""
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        raise BdattnError(f"unknown activation {act!r} (one of {', '.join(ACTIVATIONS)})")
+    (_binding or _load_binding()).linear_w4(x, w, bias, y, group, code, gate, residual,
+                                            None if stream is None else stream.cuda_stream)
+
+
+class Cache4:
+    """K and V of a cache in 4 bits (``bdattn_cache4``): codes (B, heads, rows, head_dim / 2) uint8 and (step, low) pairs
+    (B, heads, rows, head_dim / group, 2) of the activations' dtype."""
+    __slots__ = ("k_codes", "v_codes", "k_scales", "v_scales")
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
+
+    @classmethod
+    def empty(cls, batch, num_kv_heads, rows, head_dim, group, dtype, device="cuda"):
+        import torch
+        codes = lambda: torch.empty(batch, num_kv_heads, rows, head_dim // 2, device=device, dtype=torch.uint8)
+        scales = lambda: torch.empty(batch, num_kv_heads, rows, head_dim // group, 2, device=device, dtype=dtype)
+        return cls(codes(), codes(), scales(), scales())
+
+    @property
+    def rows(self):
+        return self.k_codes.shape[2]
+
+    def first(self, rows):
+        """The cache's first rows, the same memory."""
+        return Cache4(*(getattr(self, n)[:, :, :rows] for n in self.__slots__))
+
+
+def cache4_append(k, v, cache, *, kv_len=None, stream=None):
+    """``bdattn_cache4_append``: the L rows of k and v, (B, L, heads * head_dim) or (L, ...), to the places n - L .. n - 1 of the
+    cache, n = kv_len[b] (INT32 on the device, the new rows counted) or all of its rows."""
+    (_binding or _load_binding()).cache4_append(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, k, v, kv_len,
+                                                None if stream is None else stream.cuda_stream)
+
+
+def cache4_read(cache, k_out, v_out, *, kv_len=None, stream=None):
+    """``bdattn_cache4_read``: the values that the places n - L .. n - 1 of the cache stand for, in 16 bits."""
+    (_binding or _load_binding()).cache4_read(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, k_out, v_out, kv_len,
+                                              None if stream is None else stream.cuda_stream)
+
+
+def sdpa_cache4_fwd(q, cache, out, num_heads, *, window=0, sinks=0, kv_len=None, key_mask=None, softmax_scale=0.0, stream=None):
+    """``bdattn_sdpa_cache4_fwd``: ``sdpa_window_fwd`` over a cache in 4 bits.  q and out: (B, L, num_heads * head_dim), or
+    (L, ...) for a cache of one item."""
+    (_binding or _load_binding()).sdpa_cache4(cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, q, out, num_heads, window, sinks,
+                                              kv_len, key_mask, softmax_scale, None if stream is None else stream.cuda_stream)

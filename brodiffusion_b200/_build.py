@@ -4,6 +4,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
@@ -13,9 +14,10 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "--use_fast_math",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-Xptxas", "-v",
 ]
+UNITS = ["bdattn_lib", "bdattn_lib4"]      # translation units
 
 
 # The Python module of the calls of a decoding step (csrc/binding.cpp): torch tensors in, the library's entry points out.
@@ -73,12 +75,24 @@ def build(force: bool = False, verbose: bool = False) -> str:
         build_binding()
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, "-o", LIB_PATH, os.path.join(CSRC, "bdattn_lib.cu")]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    log = res.stdout + res.stderr
+    log, failed = "", False
+    with tempfile.TemporaryDirectory() as d:
+        # the units side by side, then one library of them
+        objects = [os.path.join(d, u + ".o") for u in UNITS]
+        cmds = [[nvcc, *NVCC_FLAGS, "-c", "-o", o, os.path.join(CSRC, u + ".cu")] for u, o in zip(UNITS, objects)]
+        running = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
+        for cmd, p in zip(cmds, running):
+            out = p.communicate()[0]
+            log += " ".join(cmd) + "\n" + out
+            failed = failed or p.returncode != 0
+        if not failed:
+            cmd = [nvcc, *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objects]
+            res = subprocess.run(cmd, capture_output=True, text=True)
+            log += " ".join(cmd) + "\n" + res.stdout + res.stderr
+            failed = res.returncode != 0
     with open(os.path.join(PKG_DIR, "build.log"), "w") as f:
-        f.write(" ".join(cmd) + "\n" + log)
-    if res.returncode != 0:
+        f.write(log)
+    if failed:
         sys.stderr.write(log)
         raise RuntimeError("nvcc failed building libbdattn.so")
     if verbose:

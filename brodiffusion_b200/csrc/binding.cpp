@@ -272,6 +272,222 @@ PyObject* sdpa_window(PyObject* const* a) {
     return done(bdattn_sdpa_window_fwd(&p, &w, stream_of(a[11])));
 }
 
+// (x, residual, residual_out, post_gain, gate, residual_scale, gain, out, out_scale, eps, stream)
+PyObject* sandwich_norm(PyObject* const* a) {
+    const at::Tensor &x = tensor(a[0], "x"), &residual = tensor(a[1], "residual"), &residual_out = tensor(a[2], "residual_out");
+    const at::Tensor *post = optional(a[3], "post_gain"), *gate = optional(a[4], "gate"), *gain = optional(a[6], "gain"),
+                     *out = optional(a[7], "out"), *scale = optional(a[8], "out_scale");
+    const float residual_scale = real(a[5]), eps = real(a[9]);
+    const Matrix mx(x, "x"), mr(residual, "residual"), ms(residual_out, "residual_out");
+    mr.same(mx, "residual");
+    ms.same(mx, "residual_out");
+    Matrix mo, mg;
+    if (out != nullptr) (mo = Matrix(*out, "out")).same(mx, "out");
+    typed(&residual, x.scalar_type(), "residual");
+    typed(&residual_out, x.scalar_type(), "residual_out");
+    typed(gate, x.scalar_type(), "gate");
+    typed(scale, at::kFloat, "out_scale");
+    if (gain != nullptr && post != nullptr) typed(gain, post->scalar_type(), "gain");
+    if (gate != nullptr) {
+        if (gate->dim() == 1) {
+            mg.data = vector(gate, mx.cols, "gate");
+            mg.rows = 1;
+            mg.ld = mx.cols;
+        } else {
+            mg = Matrix(*gate, "gate");
+            if (mg.cols != mx.cols || mg.rows < 1) refuse("gate must have a row at least and the columns of x");
+        }
+    }
+    bdattn_sandwich_norm_params p{};
+    p.dtype = code(x, "x");
+    p.rows = mx.rows;
+    p.cols = mx.cols;
+    p.x = mx.data;
+    p.x_ld = mx.ld;
+    p.residual = mr.data;
+    p.residual_ld = mr.ld;
+    p.residual_out = ms.data;
+    p.residual_out_ld = ms.ld;
+    p.post_gain = vector(post, mx.cols, "post_gain");
+    p.gain = vector(gain, mx.cols, "gain");
+    p.gain_dtype = post != nullptr ? code(*post, "post_gain") : gain != nullptr ? code(*gain, "gain") : BDATTN_F32;
+    p.gate = mg.data;
+    p.gates = mg.rows;
+    p.gate_ld = mg.ld;
+    p.residual_scale = residual_scale;
+    p.out = mo.data;
+    p.out_ld = mo.ld;
+    p.out_dtype = out != nullptr ? code(*out, "out") : p.dtype;
+    p.out_scale = static_cast<float*>(vector(scale, mx.rows, "out_scale"));
+    p.eps = eps;
+    on_gpu({&x, &residual, &residual_out, post, gate, gain, out, scale});
+    return done(bdattn_sandwich_norm_fwd(&p, stream_of(a[10])));
+}
+
+// (codes, scales, packed, group, stream)
+PyObject* w4_pack(PyObject* const* a) {
+    const at::Tensor &codes = tensor(a[0], "codes"), &scales = tensor(a[1], "scales"), &packed = tensor(a[2], "packed");
+    const int group = integer(a[3]);
+    typed(&codes, at::kByte, "codes");
+    typed(&packed, at::kByte, "packed");
+    if (scales.scalar_type() != at::kBFloat16 && scales.scalar_type() != at::kHalf) refuse("scales must be BF16 or F16");
+    const Matrix mc(codes, "codes");
+    if (group != 32 && group != 64 && group != 128) refuse("group must be 32, 64 or 128");
+    if (mc.rows < 1 || mc.cols < 1 || mc.cols > INT32_MAX / 2) refuse("codes must have rows, and less than 2^31 columns of 4 bits");
+    const int K = 2 * mc.cols, groups = (mc.cols - 1) / (group / 2) + 1;
+    if (scales.dim() != 3 || scales.size(0) != mc.rows || scales.size(1) != groups || scales.size(2) != 2 || scales.stride(2) != 1 ||
+        (groups > 1 && scales.stride(1) != 2) || (mc.rows > 1 && scales.stride(0) < 2ll * groups))
+        refuse("scales must be (rows, groups, 2) with dense rows of their own");
+    if (packed.dim() != 1 || static_cast<size_t>(packed.size(0)) != bdattn_w4_bytes(mc.rows, K, group) || (packed.size(0) > 1 && packed.stride(0) != 1))
+        refuse("packed must be dense, of w4_bytes(rows, columns, group) bytes");
+    on_gpu({&codes, &scales, &packed});
+    return done(bdattn_w4_pack(mc.data, mc.ld, scales.data_ptr(), mc.rows > 1 ? scales.stride(0) : 2ll * groups, packed.data_ptr(), mc.rows, K, group,
+                               stream_of(a[4])));
+}
+
+// (x, w, bias, y, group, act, gate, residual, stream)
+PyObject* linear_w4(PyObject* const* a) {
+    const at::Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &y = tensor(a[3], "y");
+    const at::Tensor *bias = optional(a[2], "bias"), *gate = optional(a[6], "gate"), *residual = optional(a[7], "residual");
+    const int group = integer(a[4]), act = integer(a[5]);
+    const Matrix mx(x, "x"), my(y, "y");
+    if (my.rows != mx.rows) refuse("y must have the rows of x");
+    Matrix mr;
+    if (residual != nullptr) (mr = Matrix(*residual, "residual")).same(my, "residual");
+    typed(&w, at::kByte, "w");
+    typed(&x, y.scalar_type(), "x");
+    typed(bias, y.scalar_type(), "bias");
+    typed(gate, y.scalar_type(), "gate");
+    typed(residual, y.scalar_type(), "residual");
+    if (w.dim() != 1 || static_cast<size_t>(w.size(0)) != bdattn_w4_bytes(my.cols, mx.cols, group) || (w.size(0) > 1 && w.stride(0) != 1) || w.size(0) == 0)
+        refuse("w must be dense, of w4_bytes(columns of y, columns of x, group) bytes");
+    bdattn_linear_w4_params p{};
+    p.dtype = code(y, "y");
+    p.M = mx.rows;
+    p.N = my.cols;
+    p.K = mx.cols;
+    p.group = group;
+    p.x = mx.data;
+    p.x_ld = mx.ld;
+    p.w = w.data_ptr();
+    p.bias = vector(bias, my.cols, "bias");
+    p.gate = vector(gate, my.cols, "gate");
+    p.residual = mr.data;
+    p.residual_ld = mr.ld;
+    p.y = my.data;
+    p.y_ld = my.ld;
+    p.act = act;
+    on_gpu({&x, &w, &y, bias, gate, residual});
+    return done(bdattn_linear_w4_fwd(&p, stream_of(a[8])));
+}
+
+// A cache of four tensors: (B, heads, rows, bytes) codes and (B, heads, rows, groups, 2) scales, rows of a head dense.
+struct Cache4 {
+    const at::Tensor *k_codes, *v_codes, *k_scales, *v_scales;
+    bdattn_cache4 c{};
+    explicit Cache4(PyObject* const* a) {
+        k_codes = &tensor(a[0], "k_codes");
+        v_codes = &tensor(a[1], "v_codes");
+        k_scales = &tensor(a[2], "k_scales");
+        v_scales = &tensor(a[3], "v_scales");
+        typed(k_codes, at::kByte, "k_codes");
+        typed(v_codes, at::kByte, "v_codes");
+        typed(v_scales, k_scales->scalar_type(), "v_scales");
+        if (k_codes->dim() != 4 || k_scales->dim() != 5) refuse("codes must be (batch, heads, rows, bytes), scales (batch, heads, rows, groups, 2)");
+        if (k_codes->sizes() != v_codes->sizes() || k_scales->sizes() != v_scales->sizes()) refuse("K and V of the cache have other shapes");
+        for (int d = 0; d < 3; ++d)
+            if (k_codes->size(d) != k_scales->size(d)) refuse("codes and scales of the cache have other shapes");
+        const int64_t bytes = k_codes->size(3), groups = k_scales->size(3);
+        if (groups < 1 || bytes < 1 || 2 * bytes % groups != 0 || k_scales->size(4) != 2) refuse("scales must be a pair for every group of a row");
+        c.dtype = code(*k_scales, "k_scales");
+        c.batch = rows_of(k_codes->size(0), "the cache");
+        c.num_kv_heads = rows_of(k_codes->size(1), "the cache");
+        c.rows = rows_of(k_codes->size(2), "the cache");
+        c.head_dim = rows_of(2 * bytes, "the cache");
+        c.group = static_cast<int>(2 * bytes / groups);
+        // strides of dimensions of one are anything
+        auto strides = [&](const at::Tensor& k, const at::Tensor& v, int64_t row, long long* head, long long* batch) {
+            for (const at::Tensor* t : {&k, &v}) {
+                if (t->size(2) > 1 && t->stride(2) != row) refuse("rows of a head of the cache must be dense");
+                if (t->stride(t->dim() - 1) != 1 && t->size(t->dim() - 1) > 1) refuse("rows of a head of the cache must be dense");
+                if (t->dim() == 5 && t->size(3) > 1 && t->stride(3) != 2) refuse("rows of a head of the cache must be dense");
+            }
+            if ((c.num_kv_heads > 1 && k.stride(1) != v.stride(1)) || (c.batch > 1 && k.stride(0) != v.stride(0)))
+                refuse("K and V of the cache have other strides");
+            *head = c.num_kv_heads > 1 ? k.stride(1) : c.rows * row;
+            *batch = c.batch > 1 ? k.stride(0) : c.num_kv_heads * *head;
+            if (*head == 0 || *batch == 0) refuse("heads and batch items of the cache must be memory of their own");
+        };
+        strides(*k_codes, *v_codes, bytes, &c.codes_head_stride, &c.codes_batch_stride);
+        strides(*k_scales, *v_scales, 2 * groups, &c.scales_head_stride, &c.scales_batch_stride);
+        c.k_codes = k_codes->data_ptr();
+        c.v_codes = v_codes->data_ptr();
+        c.k_scales = k_scales->data_ptr();
+        c.v_scales = v_scales->data_ptr();
+    }
+};
+
+// (k_codes, v_codes, k_scales, v_scales, k, v, kv_len, stream)
+template <bool kAppend>
+PyObject* cache4_rows(PyObject* const* a) {
+    const Cache4 cache(a);
+    const at::Tensor &k = tensor(a[4], "k"), &v = tensor(a[5], "v");
+    const at::Tensor* kv_len = optional(a[6], "kv_len");
+    typed(&k, cache.k_scales->scalar_type(), "k");
+    typed(&v, cache.k_scales->scalar_type(), "v");
+    typed(kv_len, at::kInt, "kv_len");
+    const Rows mk(k, "k"), mv(v, "v");
+    if (mv.rows != mk.rows || mv.cols != mk.cols || mv.batch != mk.batch) refuse("v must have the shape of k");
+    if (mk.batch != cache.c.batch || mk.cols != static_cast<int64_t>(cache.c.num_kv_heads) * cache.c.head_dim)
+        refuse("k and v must have the cache's batch and heads");
+    if (mk.ld < mk.cols || mv.ld < mv.cols) refuse("k and v must have rows of their own");
+    bdattn_cache4_rows r{};
+    r.rows = mk.rows;
+    r.k = mk.data;
+    r.v = mv.data;
+    r.k_ld = mk.ld;
+    r.v_ld = mv.ld;
+    r.k_batch_stride = mk.stride;
+    r.v_batch_stride = mv.stride;
+    r.kv_len = static_cast<const int*>(vector(kv_len, cache.c.batch, "kv_len"));
+    on_gpu({cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, &k, &v, kv_len});
+    return done(kAppend ? bdattn_cache4_append(&cache.c, &r, stream_of(a[7])) : bdattn_cache4_read(&cache.c, &r, stream_of(a[7])));
+}
+
+// (k_codes, v_codes, k_scales, v_scales, q, out, num_heads, window, sinks, kv_len, key_mask, softmax_scale, stream)
+PyObject* sdpa_cache4(PyObject* const* a) {
+    const Cache4 cache(a);
+    const at::Tensor &q = tensor(a[4], "q"), &out = tensor(a[5], "out");
+    const int heads = integer(a[6]), window = integer(a[7]), sinks = integer(a[8]);
+    const at::Tensor *kv_len = optional(a[9], "kv_len"), *mask = optional(a[10], "key_mask");
+    const float scale = real(a[11]);
+    typed(&q, cache.k_scales->scalar_type(), "q");
+    typed(&out, cache.k_scales->scalar_type(), "out");
+    typed(kv_len, at::kInt, "kv_len");
+    typed(mask, at::kFloat, "key_mask");
+    const Rows mq(q, "q"), mo(out, "out");
+    if (mo.rows != mq.rows || mo.cols != mq.cols || mo.batch != mq.batch) refuse("out must have the shape of q");
+    if (mq.batch != cache.c.batch || heads < 1 || mq.cols != static_cast<int64_t>(heads) * cache.c.head_dim)
+        refuse("q must have the cache's batch and num_heads heads of its width");
+    if (mq.ld < mq.cols || mo.ld < mo.cols) refuse("q and out must have rows of their own");
+    bdattn_sdpa_cache4_params p{};
+    p.num_heads = heads;
+    p.q_rows = mq.rows;
+    p.q = mq.data;
+    p.o = mo.data;
+    p.q_ld = mq.ld;
+    p.o_ld = mo.ld;
+    p.q_batch_stride = mq.stride;
+    p.o_batch_stride = mo.stride;
+    p.window = window;
+    p.sinks = sinks;
+    p.kv_len = static_cast<const int*>(vector(kv_len, cache.c.batch, "kv_len"));
+    p.key_mask = static_cast<const float*>(vector(mask, cache.c.rows, "key_mask"));
+    p.softmax_scale = scale;
+    on_gpu({cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, &q, &out, kv_len, mask});
+    return done(bdattn_sdpa_cache4_fwd(&cache.c, &p, stream_of(a[12])));
+}
+
 template <PyObject* (*kCall)(PyObject* const*), int kArgs>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != kArgs) {
@@ -320,6 +536,12 @@ PyMethodDef methods[] = {
     {"add_rmsnorm", fast(entry<add_rmsnorm, 8>), METH_FASTCALL, "bdattn_add_rmsnorm_fwd"},
     {"linear_act", fast(entry<linear_act, 10>), METH_FASTCALL, "bdattn_linear_act_fwd"},
     {"sdpa_window", fast(entry<sdpa_window, 12>), METH_FASTCALL, "bdattn_sdpa_window_fwd"},
+    {"sandwich_norm", fast(entry<sandwich_norm, 11>), METH_FASTCALL, "bdattn_sandwich_norm_fwd"},
+    {"w4_pack", fast(entry<w4_pack, 5>), METH_FASTCALL, "bdattn_w4_pack"},
+    {"linear_w4", fast(entry<linear_w4, 9>), METH_FASTCALL, "bdattn_linear_w4_fwd"},
+    {"cache4_append", fast(entry<cache4_rows<true>, 8>), METH_FASTCALL, "bdattn_cache4_append"},
+    {"cache4_read", fast(entry<cache4_rows<false>, 8>), METH_FASTCALL, "bdattn_cache4_read"},
+    {"sdpa_cache4", fast(entry<sdpa_cache4, 13>), METH_FASTCALL, "bdattn_sdpa_cache4_fwd"},
     {"one_gpu", fast(one_gpu_entry), METH_FASTCALL, "refuses tensors of the host, of different GPUs, of another than the current one"},
     {"set_error", set_error, METH_O, "the exception of a refused call"},
     {nullptr, nullptr, 0, nullptr},

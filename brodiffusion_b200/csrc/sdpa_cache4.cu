@@ -1,0 +1,458 @@
+// Causal attention over a cache in 4 bits (cache4.cu), with a sliding window and first keys that stay visible.
+//   s_ij = scale * sum_g step_K[j, g] (sum_{c in g} q_ic u_jc) + low_K[j, g] (sum_{c in g} q_ic)
+//   o_i  = (sum_j p_ij step_V[j, g] (u_j - 8) + sum_j p_ij (low_V[j, g] + 8 step_V[j, g])) / sum_j p_ij,   p_ij = exp(s_ij - max)
+// (with u as it is, both sums would be some ten times the output of many keys, and the roundings of the first in proportion: fp16
+// outputs of 8000 keys were off by 5.3e-4, with u - 8 by 2.4e-4, of which 2.1e-4 are the outputs' own).
+// The codes enter mma.sync as exact FP16 integers (four_bit.cuh); steps and lows are applied to FP32 scores and to the
+// FP32 weights ahead of their one rounding, to FP16.  What a call costs is reading the visible rows once, 4 + 32 / group bits
+// a value: the query heads that share a K/V head, and the new tokens, are the (eight or sixteen) columns of a product whose rows are
+// sixteen keys, or sixteen columns of V.  A warp takes sixteen keys at a time, straight from memory to registers, with the next
+// sixteen on their way, and has a running maximum, sum and accumulator of its own; these meet in shared memory, then in
+// distributed shared memory, where every CTA of a head's cluster finishes its share of the rows.
+#include "four_bit.cuh"
+#include "sdpa_window.cuh"
+
+namespace bdattn {
+namespace {
+
+constexpr int kC4MaxSplit = 16;
+
+__device__ __forceinline__ uint32_t c4_transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void c4_store_cluster(uint32_t addr, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void c4_store_cluster(uint32_t addr, float2 v) {
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
+}
+// 2^e for e in [-126, 127]
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+template <int HD, int W, int NR>
+struct Cache4Cfg {
+    static constexpr int kRows = 8 * NR, kLd = HD + 4, kMergeRows = kRows + kC4MaxSplit - 1;
+    static constexpr int kSmem = (W * kRows * (kLd + 2) + kMergeRows * (kLd + 2)) * 4;
+};
+
+// HD: 64 or 128.  G: groups of a row.  W: warps.  NR: query rows in eights.  kCtas: CTAs of an SM.
+template <int HD, int G, bool kBf16, int W, int NR, int kCtas>
+__global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid_constant__ SdpaCache4Args a) {
+    using C = Cache4Cfg<HD, W, NR>;
+    constexpr int S = HD / 32, kPer = S / G, kRows = C::kRows;
+    extern __shared__ float c4_smem[];
+    float* const o_warp = c4_smem;                                          // [W][kRows][kLd]
+    float* const o_cta = o_warp + W * kRows * C::kLd;                       // [kMergeRows][kLd]
+    float2* const ml_warp = reinterpret_cast<float2*>(o_cta + C::kMergeRows * C::kLd);     // [W][kRows]
+    float2* const ml_cta = ml_warp + W * kRows;                             // [kMergeRows]
+
+    const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const int split = a.split, part = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int unit = static_cast<int>(blockIdx.x) / split, kv_head = unit / a.row_tiles, row0 = unit % a.row_tiles * kRows;
+    const int batch = blockIdx.y, rows = min(kRows, a.lq * a.kv_group - row0);
+    // (waited for ahead of the first store into a peer's shared memory: it has to run by then)
+    if (split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    dependents_may_launch();
+    wait_for_prior_grid();
+
+    const int n_keys = window_keys(a.kv_len, batch, a.c.rows), first_pos = n_keys - a.lq;      // of query 0
+    const int pos_lo = first_pos + row0 / a.kv_group, pos_hi = first_pos + (row0 + rows - 1) / a.kv_group;
+    const WindowSpan span = window_span(pos_lo, pos_hi, a.window, a.sinks);
+    // steps of sixteen keys: those of the sinks, then those of the window, from the sixteen in which it begins
+    const int sink_steps = (span.sink_end + 15) / 16, win0 = span.win_begin & ~15;
+    const int steps = sink_steps + (span.win_end > span.win_begin ? (span.win_end - win0 + 15) / 16 : 0);
+
+    // The queries in FP16, a power of two from where the largest of a row is in [2^14, 2^15): what that rounds is 2^-35 of
+    // the largest.  This lane has row g's columns 32 s + 8 q + 0..7 as the pairs of codes8, those of the odd pairs over 16.
+    uint32_t qf[NR][S][4];
+    float qs[NR][G][2], sl2[NR][2];       // of columns 2 q and 2 q + 1: sums over a group, factor of the scores
+    int pos[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        const int r = row0 + min(nr * 8 + g, rows - 1), i = r / a.kv_group;
+        const uint16_t* const qp = reinterpret_cast<const uint16_t*>(a.q) + batch * a.q_bs + i * a.q_ld +
+                                   static_cast<long long>(kv_head * a.kv_group + r % a.kv_group) * HD + q * 8;
+        float f[S][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const uint4 v = load16(qp + s * 32);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 p = layer_pair<kBf16>(w[e]);
+                f[s][2 * e] = p.x;
+                f[s][2 * e + 1] = p.y;
+                top = fmaxf(top, fmaxf(fabsf(p.x), fabsf(p.y)));
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // (zeros, and rows that are not finite, stay as they are)
+        const int up = top > 0.0f && top <= FLT_MAX ? min(100, 141 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
+        const float lift = pow2(up), lift16 = pow2(up - 4);
+        float sum[G];
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+            sum[gi] = 0.0f;
+#pragma unroll
+            for (int s = gi * kPer; s < (gi + 1) * kPer; ++s) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[gi] += f[s][e] * lift;
+            }
+            sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 1);
+            sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 2);
+            // the codes count 2^-24 each
+            sum[gi] *= 0x1p-24f;
+        }
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float l = (e & 1) ? lift16 : lift;
+                qf[nr][s][e] = pack2<false>(f[s][e] * l, f[s][e + 4] * l);
+            }
+        }
+        const float down = pow2(-up) * (0x1p24f * a.scale * 1.4426950408889634f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int from = (2 * q + h) * 4;
+            sl2[nr][h] = __shfl_sync(0xffffffffu, down, from);
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) qs[nr][gi][h] = __shfl_sync(0xffffffffu, sum[gi], from);
+            pos[nr][h] = first_pos + (row0 + min(nr * 8 + 2 * q + h, rows - 1)) / a.kv_group;
+        }
+    }
+
+    const uint8_t* const kc_base = a.c.k_codes + batch * a.c.codes_bs + kv_head * a.c.codes_hs + q * 4 * S;
+    const uint8_t* const vc_base = a.c.v_codes + batch * a.c.codes_bs + kv_head * a.c.codes_hs + g * 2 * S;
+    const uint16_t* const ks_base = a.c.k_scales + batch * a.c.scales_bs + kv_head * a.c.scales_hs;
+    const uint16_t* const vs_base = a.c.v_scales + batch * a.c.scales_bs + kv_head * a.c.scales_hs;
+    uint32_t kc[2][S], vc[4][S / 2], ks[2][G], vs[2][G];
+    auto fetch = [&](int step) {
+        const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
+        // (keys behind the last row are read as that one; nobody sees them)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const long long key = min(key0 + g + 8 * h, a.c.rows - 1);
+            load_words_once<S>(kc_base + key * (HD / 2), kc[h]);
+            load_words_once<G>(ks_base + key * (2 * G), ks[h]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const long long key = min(key0 + 2 * q + (e & 1) + 8 * (e >> 1), a.c.rows - 1);
+            load_words_once<S / 2>(vc_base + key * (HD / 2), vc[e]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_words_once<G>(vs_base + min(key0 + g + 8 * h, a.c.rows - 1) * static_cast<long long>(2 * G), vs[h]);
+    };
+
+    // Transposed accumulators: lane (g, q) has columns of V (rows of a product) in the tiles 2 s (columns 32 s + 4 g and + 2) and
+    // 2 s + 1 (+ 1 and + 3, sixteen times them), for the query rows 2 q and 2 q + 1; lows, maxima and sums for its own keys.
+    float m[NR][2], l[NR][2], o[NR][2 * S][4], lo[NR][G][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            m[nr][h] = -INFINITY;
+            l[nr][h] = 0.0f;
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * S; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.0f;
+    }
+    int v_exp = -1000;           // the steps of V count 2^-v_exp each: the largest so far is in [2^14, 2^15) then
+    const int stride = W * split;
+    int step = part * W + warp;
+    if (step < steps) fetch(step);
+    for (; step < steps; step += stride) {
+        const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
+        const int begin = step < sink_steps ? 0 : span.win_begin, end = step < sink_steps ? span.sink_end : span.win_end;
+        // scores
+        float s[NR][4];
+        float2 vstep[2][G];
+        {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.0f;
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+                float d[NR][4] = {};
+#pragma unroll
+                for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
+                    uint32_t u[2][4];
+                    codes8<true>(kc[0][i], u[0]);
+                    codes8<true>(kc[1][i], u[1]);
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr) {
+                        mma16<false>(d[nr], u[0][0], u[1][0], u[0][2], u[1][2], qf[nr][i][0], qf[nr][i][2]);
+                        mma16<false>(d[nr], u[0][1], u[1][1], u[0][3], u[1][3], qf[nr][i][1], qf[nr][i][3]);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 p = layer_pair<kBf16>(ks[h][gi]);
+                    vstep[h][gi] = layer_pair<kBf16>(vs[h][gi]);
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr) {
+                        s[nr][2 * h] = fmaf(p.x, d[nr][2 * h], fmaf(p.y, qs[nr][gi][0], s[nr][2 * h]));
+                        s[nr][2 * h + 1] = fmaf(p.x, d[nr][2 * h + 1], fmaf(p.y, qs[nr][gi][1], s[nr][2 * h + 1]));
+                    }
+                }
+            }
+        }
+        uint32_t vw[4][S / 2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int i = 0; i < S / 2; ++i) vw[e][i] = vc[e][i];
+        }
+        if (step + stride < steps) fetch(step + stride);
+
+        // what is seen of the sixteen keys; all of it in most steps
+        const bool whole = a.key_mask == nullptr && key0 >= begin && key0 + 16 <= end && key0 + 15 <= pos_lo &&
+                           (a.window == 0 || pos_hi - key0 < a.window || key0 + 16 <= a.sinks);
+        if (!whole) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = key0 + g + 8 * h;
+                bool on = key >= begin && key < end;
+                if (on && a.key_mask != nullptr) on = load_scale(a.key_mask + key) != 0.0f;
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const bool seen = on && key <= pos[nr][c] && (a.window == 0 || pos[nr][c] - key < a.window || key < a.sinks);
+                        if (!seen) s[nr][2 * h + c] = -INFINITY;
+                    }
+                }
+                // what hidden rows hold counts for nothing
+                if (!on) {
+#pragma unroll
+                    for (int gi = 0; gi < G; ++gi) vstep[h][gi] = make_float2(0.0f, 0.0f);
+                }
+            }
+        }
+        // a new largest step of V
+        {
+            float top = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int gi = 0; gi < G; ++gi) top = fmaxf(top, vstep[h][gi].x <= FLT_MAX ? vstep[h][gi].x : 0.0f);
+            }
+            const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127 - 14;
+            if (e > v_exp) {
+                const float f = v_exp < e - 126 ? 0.0f : pow2(v_exp - e);
+                v_exp = e;
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+                    for (int i = 0; i < 2 * S; ++i) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[nr][i][x] *= f;
+                    }
+                }
+            }
+        }
+        const float v_lift = pow2(min(127, -v_exp));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+                vstep[h][gi].y = fmaf(8.0f, vstep[h][gi].x, vstep[h][gi].y);
+                vstep[h][gi].x *= v_lift;
+            }
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            float top[2] = {fmaxf(s[nr][0], s[nr][2]), fmaxf(s[nr][1], s[nr][3])};
+            // a new largest score is rare after the first steps
+            if (__any_sync(0xffffffffu, top[0] > m[nr][0] || top[1] > m[nr][1])) {
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], x));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], x));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float now = fmaxf(m[nr][h], top[h]);
+                    const float alpha = now == -INFINITY ? 1.0f : fast_exp2((m[nr][h] - now) * sl2[nr][h]);
+                    m[nr][h] = now;
+                    l[nr][h] *= alpha;
+#pragma unroll
+                    for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < 2 * S; ++i) {
+                        o[nr][i][h] *= alpha;
+                        o[nr][i][2 + h] *= alpha;
+                    }
+                }
+            }
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float ref = m[nr][e & 1] == -INFINITY ? 0.0f : m[nr][e & 1];
+                p[e] = fast_exp2((s[nr][e] - ref) * sl2[nr][e & 1]);
+                l[nr][e & 1] += p[e];
+            }
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) {
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 v = vstep[e >> 1][gi];
+                    w[e] = p[e] * v.x;
+                    float add = p[e] * v.y;
+                    if (!whole && p[e] == 0.0f) w[e] = add = 0.0f;          // (a row that this query does not see may be NaN)
+                    lo[nr][gi][e & 1] += add;
+                }
+                const uint32_t b0 = c4_transpose8(pack2<false>(w[0], w[1])), b1 = c4_transpose8(pack2<false>(w[2], w[3]));
+#pragma unroll
+                for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
+                    // four columns of two keys: the halves of a word of each
+                    const uint32_t sel = (i & 1) ? 0x7632 : 0x5410;
+                    const uint32_t w0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), w1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
+                    uint32_t u0[4], u1[4];
+                    codes8<true>(w0, u0);
+                    codes8<true>(w1, u1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        u0[e] = (e & 1) ? less_eight<true>(u0[e]) : less_eight<false>(u0[e]);
+                        u1[e] = (e & 1) ? less_eight<true>(u1[e]) : less_eight<false>(u1[e]);
+                    }
+                    mma16<false>(o[nr][2 * i], u0[0], u0[2], u1[0], u1[2], b0, b1);
+                    mma16<false>(o[nr][2 * i + 1], u0[1], u0[3], u1[1], u1[3], b0, b1);
+                }
+            }
+        }
+    }
+    // the warps' sums, whole: over the lanes' keys, the lows and the powers of two put in
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) {
+                l[nr][h] += __shfl_xor_sync(0xffffffffu, l[nr][h], x);
+#pragma unroll
+                for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] += __shfl_xor_sync(0xffffffffu, lo[nr][gi][h], x);
+            }
+        }
+    }
+    const float v_down = pow2(max(-126, v_exp));
+    float* const mine = o_warp + warp * kRows * C::kLd;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = nr * 8 + 2 * q + h;
+            // the maximum in units of log2, the same for all warps of the row
+            if (g == 0) ml_warp[warp * kRows + r] = make_float2(m[nr][h] == -INFINITY ? -INFINITY : m[nr][h] * sl2[nr][h], l[nr][h]);
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const float low = lo[nr][s / kPer][h];
+                *reinterpret_cast<float4*>(mine + r * C::kLd + 32 * s + 4 * g) =
+                    make_float4(fmaf(o[nr][2 * s][h] * 0x1p24f, v_down, low), fmaf(o[nr][2 * s + 1][h] * 0x1p20f, v_down, low),
+                                fmaf(o[nr][2 * s][2 + h] * 0x1p24f, v_down, low), fmaf(o[nr][2 * s + 1][2 + h] * 0x1p20f, v_down, low));
+            }
+        }
+    }
+    __syncthreads();
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    // The CTA's sums go to the CTAs that finish the rows: row r to CTA r % split, in whose place
+    // part * ceil(kRows / split) + r / split it lies.
+    constexpr int kUnits = HD / 4;
+    const int per = (kRows + split - 1) / split;
+    for (int u = threadIdx.x; u < rows * kUnits; u += W * 32) {
+        const int r = u / kUnits, c = (u % kUnits) * 4;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, ml_warp[w * kRows + r].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float2 t = ml_warp[w * kRows + r];
+            const float f = fast_exp2(t.x - ref);
+            const float4 v = *reinterpret_cast<const float4*>(o_warp + (w * kRows + r) * C::kLd + c);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+            sum = fmaf(f, t.y, sum);
+        }
+        const int place = part * per + r / split;
+        if (split > 1) {
+            c4_store_cluster(mapa(smem_u32(o_cta + place * C::kLd + c), r % split), acc);
+            if (c == 0) c4_store_cluster(mapa(smem_u32(ml_cta + place), r % split), make_float2(top, sum));
+        } else {
+            *reinterpret_cast<float4*>(o_cta + place * C::kLd + c) = acc;
+            if (c == 0) ml_cta[place] = make_float2(top, sum);
+        }
+    }
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+    for (int u = threadIdx.x; u < per * kUnits; u += W * 32) {
+        const int x = u / kUnits, r = part + x * split, c = (u % kUnits) * 4;
+        if (r >= rows) break;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float top = -INFINITY, sum = 0.0f;
+        for (int k = 0; k < split; ++k) top = fmaxf(top, ml_cta[k * per + x].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int k = 0; k < split; ++k) {
+            const float2 t = ml_cta[k * per + x];
+            const float4 v = *reinterpret_cast<const float4*>(o_cta + (k * per + x) * C::kLd + c);
+            const float f = fast_exp2(t.x - ref);
+            acc.x = fmaf(f, v.x, acc.x);
+            acc.y = fmaf(f, v.y, acc.y);
+            acc.z = fmaf(f, v.z, acc.z);
+            acc.w = fmaf(f, v.w, acc.w);
+            sum = fmaf(f, t.y, sum);
+        }
+        // (a sum that is NaN makes the row NaN)
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int i = (row0 + r) / a.kv_group, head = kv_head * a.kv_group + (row0 + r) % a.kv_group;
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + batch * a.o_bs + i * a.o_ld + static_cast<long long>(head) * HD + c) =
+            make_uint2(pack2<kBf16>(acc.x * inv, acc.y * inv), pack2<kBf16>(acc.z * inv, acc.w * inv));
+    }
+}
+
+template <int HD, int G, bool kBf16, int W, int NR, int kCtas>
+cudaError_t go_cache4(SdpaCache4Args a, int split, cudaStream_t stream) {
+    using C = Cache4Cfg<HD, W, NR>;
+    const auto kern = sdpa_cache4_kernel<HD, G, kBf16, W, NR, kCtas>;
+    cudaError_t e = set_max_smem_once(kern, C::kSmem);
+    if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    a.split = split;
+    const dim3 grid(static_cast<unsigned>(split * a.c.kv_heads * a.row_tiles), static_cast<unsigned>(a.batch));
+    return launch_dependent_cluster(kern, grid, dim3(W * 32), C::kSmem, stream, dim3(split), a);
+}
+
+template <int HD, int G, bool kBf16>
+cudaError_t pick_cache4(SdpaCache4Args a, cudaStream_t stream) {
+    const int nr = a.lq * static_cast<long long>(a.kv_group) <= 8 ? 1 : 2;
+    a.row_tiles = static_cast<int>((static_cast<long long>(a.lq) * a.kv_group + 8 * nr - 1) / (8 * nr));
+    const long long units = static_cast<long long>(a.batch) * a.c.kv_heads * a.row_tiles;
+    const long long seen = a.window > 0 ? static_cast<long long>(a.window) + a.sinks + a.lq - 1 : a.c.rows;
+    const long long steps = ((seen < a.c.rows ? seen : a.c.rows) + 15) / 16;
+    int split = 1;
+    while (split < 8 && units * split * 2 <= 3 * sm_count() && steps >= 8 * split) split *= 2;
+    return nr == 1 ? go_cache4<HD, G, kBf16, 4, 1, 3>(a, split, stream) : go_cache4<HD, G, kBf16, 4, 2, 2>(a, split, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_sdpa_cache4(const SdpaCache4Args& a, bool bf16, cudaStream_t stream) {
+    auto go = [&](auto b) {
+        constexpr bool kB = decltype(b)::value;
+        const int groups = a.c.head_dim / a.c.group;
+        if (a.c.head_dim == 64) return groups == 1 ? pick_cache4<64, 1, kB>(a, stream) : pick_cache4<64, 2, kB>(a, stream);
+        return groups == 1 ? pick_cache4<128, 1, kB>(a, stream) : groups == 2 ? pick_cache4<128, 2, kB>(a, stream) : pick_cache4<128, 4, kB>(a, stream);
+    };
+    return bf16 ? go(std::true_type{}) : go(std::false_type{});
+}
+
+}  // namespace bdattn

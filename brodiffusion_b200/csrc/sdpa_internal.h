@@ -1,6 +1,8 @@
 // Internal launch interfaces shared by the C-ABI layer and the kernels.
 #pragma once
 
+#include <cstdint>
+
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -254,6 +256,72 @@ struct AddRmsNormArgs {
     bool one_wave;             // set by the launch: no more CTAs than SMs
 };
 cudaError_t launch_add_rmsnorm(const AddRmsNormArgs& a, bool bf16, bool fp8, cudaStream_t stream);
+
+// The norms behind a block and ahead of the next one, with gate, scale and addition between them.
+struct SandwichNormArgs {
+    const void* x;
+    const void* residual;
+    void* residual_out;
+    const void* post_gain;     // cols values, or null
+    const void* gain;          // cols values, or null
+    int gain_is_f32;           // both
+    const void* gate;          // vectors of cols values, or null: row r has vector r / gate_rows
+    int gate_rows;
+    void* out;                 // or null
+    float* out_scale;          // e4m3 output: rows values; else null
+    int rows, cols;
+    long long ldx, ldr, ldro, ldo, ldg;
+    float residual_scale, eps;
+    int shift;                 // set by the launch: elements that x lies off 16 bytes
+    bool one_wave;             // set by the launch: no more CTAs than SMs
+};
+cudaError_t launch_sandwich_norm(const SandwichNormArgs& a, bool bf16, cudaStream_t stream);
+
+// A layer's product with 4-bit weights (one problem: M, N, K, C, ldc, bias, act, gate, residual, ldr), and their packing.
+struct W4PackArgs {
+    const uint8_t* codes;      // (N, K / 2)
+    const void* scales;        // (N, groups, 2) of 16 bits
+    void* packed;
+    int N, K, group, k_tiles;
+    long long codes_ld, scales_ld;
+};
+cudaError_t launch_w4_linear(const GemmProblem& p, const void* x, long long ldx, const void* w, int group, bool bf16, cudaStream_t stream);
+cudaError_t launch_w4_pack(const W4PackArgs& a, cudaStream_t stream);
+
+// A cache in 4 bits: rows of heads behind one another, strides of batch items and heads in bytes (codes) and 16-bit units.
+struct Cache4Dev {
+    uint8_t* k_codes;
+    uint8_t* v_codes;
+    uint16_t* k_scales;
+    uint16_t* v_scales;
+    long long codes_bs, codes_hs, scales_bs, scales_hs;
+    int rows, kv_heads, head_dim, group;
+};
+// Rows n - n_rows + i of every item, n its length.
+struct Cache4RowsArgs {
+    Cache4Dev c;
+    const void* k;
+    const void* v;
+    long long k_ld, v_ld, k_bs, v_bs;
+    int n_rows;
+    long long items;           // batch * n_rows * kv_heads * 2
+    const int* kv_len;
+};
+cudaError_t launch_cache4_append(const Cache4RowsArgs& a, bool bf16, cudaStream_t stream);
+cudaError_t launch_cache4_read(const Cache4RowsArgs& a, bool bf16, cudaStream_t stream);
+// Causal attention over it.
+struct SdpaCache4Args {
+    Cache4Dev c;
+    const void* q;
+    void* o;
+    long long q_ld, o_ld, q_bs, o_bs;
+    int lq, kv_group, window, sinks, batch;
+    float scale;
+    const float* key_mask;
+    const int* kv_len;
+    int split, row_tiles;      // set by the launch
+};
+cudaError_t launch_sdpa_cache4(const SdpaCache4Args& a, bool bf16, cudaStream_t stream);
 
 // Elementwise helpers.
 cudaError_t launch_add_inplace(void* y, const void* x, long long n, bool bf16, cudaStream_t stream);

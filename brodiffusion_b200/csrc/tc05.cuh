@@ -24,9 +24,12 @@ enum : int {
     kStatusBadArgs = 2,       // device-side argument check failed
 };
 
-// Per-device status word (one copy per device that loads the module).  The
-// library is built as a single translation unit, so this definition is the
-// only one.
+// Per-device status word (one copy per device that loads the module).  The kernels that
+// set it are one translation unit (bdattn_lib.cu), so this definition is the only one; the unit of the
+// kernels without a wait (bdattn_lib4.cu) has a word of its own that nobody sets.
+#ifdef BDATTN_UNIT_WITHOUT_WAITS
+static
+#endif
 __device__ int g_device_status = 0;
 
 // ------------------------------------------------------------ host helpers

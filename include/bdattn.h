@@ -620,6 +620,142 @@ typedef struct bdattn_window_params {
 
 int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_params* w, bdattn_stream_t stream);
 
+/* ------------------------------------------- the same layer in 4 bits
+ * Values in groups of 32, 64 or 128 of a row, each with a step and a lowest value of the activations' type (a
+ * pair: step, then low):  x = low + step * u,  u in 0..15.  No operator rounds a value that it reads: codes meet the other
+ * operand as integers, steps and lows are applied to FP32 sums.
+ *
+ * bdattn_sandwich_norm_fwd: what stands between two blocks of a layer with norms on both sides of each,
+ *   b = x * rsqrt(mean(x^2) + eps) * post_gain,
+ *   h = residual_scale * residual + gate[group of rows] * b   in FP32,  residual_out = h rounded to dtype,
+ *   y = h * rsqrt(mean(h^2) + eps) * gain,  out and out_scale from y as in bdattn_add_rmsnorm_fwd.
+ * x is the block's output, residual the stream; gate: `gates` vectors of cols values, of which row r has number
+ * r / (rows / gates) (batch items with a modulation each); post_gain, gain, gate and out may be NULL (out: the last block;
+ * gain goes with out).  Both norms are of unrounded values.  A sum of squares that is not finite in FP32 gives NaN.
+ * residual_out may be residual or x, out may be x or residual where its dtype is theirs (same ld).  Sizes, strides and
+ * alignments as for bdattn_add_rmsnorm_fwd. */
+typedef struct bdattn_sandwich_norm_params {
+    int dtype;
+    int rows;              /* 0: nothing is done */
+    int cols;
+    const void* x;
+    const void* residual;
+    void* residual_out;
+    const void* post_gain;
+    const void* gain;
+    int gain_dtype;        /* of both gains: F32 or dtype */
+    const void* gate;      /* of dtype */
+    int gates;             /* divides rows */
+    long long gate_ld;     /* 0 => cols */
+    float residual_scale;
+    void* out;
+    int out_dtype;
+    float* out_scale;      /* rows values; E4M3 output only */
+    long long x_ld;        /* 0 => cols */
+    long long residual_ld;
+    long long residual_out_ld;
+    long long out_ld;
+    float eps;
+} bdattn_sandwich_norm_params;
+
+int bdattn_sandwich_norm_fwd(const bdattn_sandwich_norm_params* p, bdattn_stream_t stream);
+
+/* bdattn_linear_w4_fwd: bdattn_linear_act_fwd for few rows against 4-bit weights,
+ *   Y[m, n] = residual[m, n] + gate[n] * act(sum_k X[m, k] W[n, k] + bias[n]),
+ * W packed by bdattn_w4_pack (once, at load) into bdattn_w4_bytes(N, K, group) bytes, 16-byte aligned: tiles of 16 rows x 128
+ * columns, codes in the order of the kernel's lanes, pairs behind them.  X (M, K), Y, residual (M, N), bias and gate (N) of
+ * dtype BF16 / F16, the pairs of the weights too; bias, gate and residual may be NULL; residual may be Y (same ld).  K and x_ld
+ * are multiples of 8, X is 16-byte aligned; any N.  Meant for up to 64 rows, which read W once; more rows
+ * read it again for each 64.  A row of X with a value that is not finite (BF16: of 2^63 and more) comes out not finite; BF16 values below 2^-57 may count as
+ * zeros.
+ * bdattn_w4_pack: codes (N, K / 2 bytes, row stride codes_ld bytes) hold two columns a byte, the even one in the low half;
+ * scales (N, ceil(K / group), 2) the pairs, row stride scales_ld values; a last group may be short. */
+typedef struct bdattn_linear_w4_params {
+    int dtype;
+    int M;                 /* 0: nothing is done */
+    int N;
+    int K;
+    int group;             /* 32, 64 or 128 */
+    const void* x;
+    const void* w;
+    const void* bias;
+    const void* gate;
+    const void* residual;
+    void* y;
+    int act;               /* BDATTN_ACT_* */
+    long long x_ld;        /* 0 => K */
+    long long residual_ld; /* 0 => N */
+    long long y_ld;        /* 0 => N */
+} bdattn_linear_w4_params;
+
+size_t bdattn_w4_bytes(int N, int K, int group);
+int bdattn_w4_pack(const void* codes, long long codes_ld, const void* scales, long long scales_ld, void* packed, int N, int K,
+                   int group, bdattn_stream_t stream);
+int bdattn_linear_w4_fwd(const bdattn_linear_w4_params* p, bdattn_stream_t stream);
+
+/* A cache of K and V in 4 bits: (batch, num_kv_heads, rows, head_dim / 2) bytes of codes and (batch, num_kv_heads, rows,
+ * head_dim / group, 2) pairs of dtype, for K and V each, rows of a head dense.  A group of a new row x is held as
+ *   low = min x,  step = (max x - min x) / 15 rounded to dtype,  u = round((x - low) / step) up to 15 (0 where step is 0);
+ * a group with a value that is not finite has NaN for both and is NaN.  Steps below 2^-126 count as 0.  The
+ * codes of a row lie in the order of the attention kernel's lanes (bdattn_cache4_read gives the values back); rows can be
+ * moved, copied and left out as they are.  head_dim 64 or 128, group 32, 64 or 128 up to it; codes 16-byte aligned with
+ * strides that are multiples of 16, scales aligned to a row's pairs.
+ *
+ * bdattn_cache4_append: row i of the r->rows new ones of item b goes to place n - r->rows + i, n = kv_len[b] (kv_len NULL: all
+ * rows of the cache): kv_len counts the new rows already, as for the attention behind it.  A place before the
+ * first row is not written.  bdattn_cache4_read: the same places back as low + step * u, rounded once (to the largest finite
+ * value where a rounded step takes it beyond); zeros from before the first row.  k, v (batch, r->rows, num_kv_heads * head_dim) of dtype, 16-byte aligned with strides that are multiples of 8.
+ *
+ * bdattn_sdpa_cache4_fwd: bdattn_sdpa_window_fwd over such a cache: the same rule of what is seen, the same treatment of
+ * kv_len, key_mask and rows that nobody sees (they may hold anything).  One query segment. */
+typedef struct bdattn_cache4 {
+    int dtype;
+    int batch;
+    int num_kv_heads;
+    int head_dim;
+    int group;
+    int rows;
+    void* k_codes;
+    void* v_codes;
+    void* k_scales;
+    void* v_scales;
+    long long codes_batch_stride;    /* bytes; 0 => num_kv_heads * codes_head_stride */
+    long long codes_head_stride;     /* bytes; 0 => rows * head_dim / 2 */
+    long long scales_batch_stride;   /* values; 0 => num_kv_heads * scales_head_stride */
+    long long scales_head_stride;    /* values; 0 => rows * head_dim / group * 2 */
+} bdattn_cache4;
+
+typedef struct bdattn_cache4_rows {
+    int rows;              /* of every batch item; 0: nothing is done */
+    void* k;               /* append reads, read writes them */
+    void* v;
+    long long k_ld;        /* 0 => num_kv_heads * head_dim */
+    long long v_ld;
+    long long k_batch_stride;        /* 0 => rows * ld */
+    long long v_batch_stride;
+    const int* kv_len;     /* or NULL */
+} bdattn_cache4_rows;
+
+typedef struct bdattn_sdpa_cache4_params {
+    int num_heads;
+    int q_rows;
+    const void* q;         /* (batch, q_rows, num_heads * head_dim) */
+    void* o;
+    long long q_ld;        /* 0 => num_heads * head_dim */
+    long long o_ld;
+    long long q_batch_stride;        /* 0 => q_rows * ld */
+    long long o_batch_stride;
+    int window;            /* >= 0; 0: unbounded */
+    int sinks;             /* >= 0 */
+    const int* kv_len;     /* or NULL */
+    const float* key_mask; /* cache rows, 0 = masked; or NULL */
+    float softmax_scale;   /* <= 0 => 1 / sqrt(head_dim) */
+} bdattn_sdpa_cache4_params;
+
+int bdattn_cache4_append(const bdattn_cache4* c, const bdattn_cache4_rows* r, bdattn_stream_t stream);
+int bdattn_cache4_read(const bdattn_cache4* c, const bdattn_cache4_rows* r, bdattn_stream_t stream);
+int bdattn_sdpa_cache4_fwd(const bdattn_cache4* c, const bdattn_sdpa_cache4_params* p, bdattn_stream_t stream);
+
 /* Y = a*Y + b*X over n dense elements, in place: the device side of the
  * prefix KV cache operations QwenImage21PrefixCache::scale_kv (brotensor
  * scale_inplace, x = NULL and b = 0) and ::blend_from (brotensor axpby_inplace
