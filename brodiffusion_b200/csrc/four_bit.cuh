@@ -2,7 +2,7 @@
 //
 // The codes go to the tensor core as they lie.  Among the low bits of a BF16 or FP16 the integer n (below 2^8, 2^11) is
 // the number n * 2^-133, or n * 2^-24: below the smallest normal exactly so, and the first binade above continues it.  A mask
-// makes two operands of a word: the nibbles 0 and 4 as they are and, BF16, 1 and 5 times 16.  So a word of eight codes costs
+// makes two operands of a word: the nibbles 0 and 4 as they are, 1 and 5 times 16.  So a word of eight codes costs
 // five instructions, no code is rounded, and the steps are applied to sums in FP32.  What meets them carries the
 // power of two that brings the products back to the middle of FP32's range.
 #pragma once
@@ -16,22 +16,15 @@
 
 namespace bdattn {
 
-// The eight codes of a word as four pairs (j, j + 4).  kSixteen: those of 1 and 3 are sixteen times theirs, which saves two
-// shifts where the other operand can carry 1 / 16.
-template <bool kSixteen>
+// The eight codes of a word as four pairs (j, j + 4); those of 1 and 3 are sixteen times theirs.
 __device__ __forceinline__ void codes8(uint32_t w, uint32_t (&r)[4]) {
     r[0] = w & 0x000f000fu;
+    r[1] = w & 0x00f000f0u;
     r[2] = (w >> 8) & 0x000f000fu;
-    if constexpr (kSixteen) {
-        r[1] = w & 0x00f000f0u;
-        r[3] = (w >> 8) & 0x00f000f0u;
-    } else {
-        r[1] = (w >> 4) & 0x000f000fu;
-        r[3] = (w >> 12) & 0x000f000fu;
-    }
+    r[3] = (w >> 8) & 0x00f000f0u;
 }
 
-// FP16 codes (in units of 2^-24, kSixteen: 2^-20) less eight: exact below the smallest normal too.
+// FP16 codes (in units of 2^-24, those of codes8's odd pairs, kSixteen: 2^-20) less eight: exact below the smallest normal too.
 template <bool kSixteen>
 __device__ __forceinline__ uint32_t less_eight(uint32_t u) {
     uint32_t r;

@@ -182,8 +182,8 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
                 for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
                     uint32_t u[2][4];
-                    codes8<true>(kc[0][i], u[0]);
-                    codes8<true>(kc[1][i], u[1]);
+                    codes8(kc[0][i], u[0]);
+                    codes8(kc[1][i], u[1]);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
                         mma16<false>(d[nr], u[0][0], u[1][0], u[0][2], u[1][2], qf[nr][i][0], qf[nr][i][2]);
@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                     const uint32_t sel = (i & 1) ? 0x7632 : 0x5410;
                     const uint32_t w0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), w1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
                     uint32_t u0[4], u1[4];
-                    codes8<true>(w0, u0);
-                    codes8<true>(w1, u1);
+                    codes8(w0, u0);
+                    codes8(w1, u1);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         u0[e] = (e & 1) ? less_eight<true>(u0[e]) : less_eight<false>(u0[e]);

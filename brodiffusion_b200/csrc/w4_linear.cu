@@ -2,7 +2,7 @@
 //   C[m, n] = residual + gate * act(sum_k X[m, k] W[n, k] + bias),  W[n, k] = low[n, g] + step[n, g] u[n, k],  g = k / group
 // as  sum_g step[n, g] (sum_{k in g} X u) + low[n, g] (sum_{k in g} X):  the codes u enter mma.sync as exact small integers
 // (four_bit.cuh), the sums of X come from the same instruction with ones for weights, and step and low are applied to
-// FP32 sums every 32 columns, so that nothing is rounded but X, W as they are given and the result.
+// FP32 sums of a group, so that nothing is rounded but X, W as they are given and the result.
 //
 // What a call of few rows costs is reading W once, 4 + 32 / group bits a value.  Packed weights (w4_pack_kernel) are tiles of 16 rows x 128
 // columns in the order in which a warp's lanes want them: 16 bytes a lane for each eight of its rows, the steps and
@@ -16,6 +16,13 @@ constexpr int kW4MaxParts = 8;
 
 __host__ __device__ constexpr int w4_tile_bytes(int group) { return 1024 + 16 * (128 / group) * 4; }
 
+// BF16 pairs times a power of two.
+__device__ __forceinline__ uint32_t times_pow2(uint32_t v, uint32_t by) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(by));
+    return r;
+}
+
 struct W4Args {
     GemmProblem p;          // M, N, K, C, bias, act, gate, residual
     const uint16_t* x;
@@ -25,9 +32,9 @@ struct W4Args {
 };
 
 // kGroups: groups of a tile's 128 columns.  W: warps, each with K tiles of its own.  T: row tiles of a CTA.  NR: rows of X in
-// eights.
-template <bool kBf16, int kGroups, int W, int T, int NR>
-__global__ void __launch_bounds__(W * 32) w4_linear_kernel(const __grid_constant__ W4Args a) {
+// eights.  D: K tiles of a warp in flight, with the columns of X that go with them.  kCtas: CTAs of an SM.
+template <bool kBf16, int kGroups, int W, int T, int NR, int D, int kCtas>
+__global__ void __launch_bounds__(W * 32, kCtas) w4_few_kernel(const __grid_constant__ W4Args a) {
     extern __shared__ float w4_sums[];      // [W][16 T x 8 NR], then [parts][16 T x 8 NR]
     constexpr int kOut = 16 * T * 8 * NR, kTile = w4_tile_bytes(128 / kGroups);
     const GemmProblem& p = a.p;
@@ -38,70 +45,72 @@ __global__ void __launch_bounds__(W * 32) w4_linear_kernel(const __grid_constant
     const uint8_t* wp[T];
 #pragma unroll
     for (int t = 0; t < T; ++t)      // (a row tile that does not exist is read as the last one: its sums go nowhere)
-        wp[t] = a.w + static_cast<long long>(min(tile0 + t, n_tiles - 1)) * a.k_tiles * kTile;
+        wp[t] = a.w + (static_cast<long long>(min(tile0 + t, n_tiles - 1)) * a.k_tiles + first) * kTile;
     if (a.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     dependents_may_launch();
+    // While the kernel before this one ends, the first weights come into the L2.
+    if (lane * 128 < kTile) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+                if (first + i * step < a.k_tiles) asm volatile("prefetch.global.L2 [%0];" ::"l"(wp[t] + static_cast<long long>(i) * step * kTile + lane * 128));
+        }
+    }
     wait_for_prior_grid();
 
     const uint16_t* xp[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) xp[r] = a.x + min(m0 + r * 8 + g, p.M - 1) * a.ldx + q * 8;
 
-    uint4 wv[T][2];
-    uint32_t sv[T][2][kGroups];
-    auto fetch = [&](int kt) {
-#pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const uint8_t* const at = wp[t] + static_cast<long long>(kt) * kTile;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                wv[t][h] = load16_once(at + h * 512 + lane * 16);
-                load_words_once<kGroups>(at + 1024 + (g + 8 * h) * 4 * kGroups, sv[t][h]);
-            }
-        }
-    };
-    float y[T][NR][4] = {};
-    if (first < a.k_tiles) fetch(first);
-    for (int kt = first; kt < a.k_tiles; kt += step) {
-        uint32_t w[T][2][4], sc[T][2][kGroups];
+    uint4 wv[D][T][2], xv[D][4][NR];
+    uint32_t sv[D][T][2][kGroups];
+    int next = first;                // the K tile that is fetched next
+    auto fetch = [&](int i) {
 #pragma unroll
         for (int t = 0; t < T; ++t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                w[t][h][0] = wv[t][h].x; w[t][h][1] = wv[t][h].y; w[t][h][2] = wv[t][h].z; w[t][h][3] = wv[t][h].w;
-#pragma unroll
-                for (int i = 0; i < kGroups; ++i) sc[t][h][i] = sv[t][h][i];
+                wv[i][t][h] = load16_once(wp[t] + h * 512 + lane * 16);
+                load_words_once<kGroups>(wp[t] + 1024 + (g + 8 * h) * 4 * kGroups, sv[i][t][h]);
             }
+            wp[t] += static_cast<long long>(step) * kTile;
         }
-        if (kt + step < a.k_tiles) fetch(kt + step);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            // eight columns of X a lane, in the pairs of codes8
-            const int c = kt * 128 + s * 32;
-            uint32_t b[NR][4];
+            const int c = next * 128 + s * 32;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                xv[i][s][r] = make_uint4(0u, 0u, 0u, 0u);
+                if (c + q * 8 < p.K) xv[i][s][r] = load16(xp[r] + c);
+            }
+        }
+        next += step;
+    };
+    float y[T][NR][4] = {};
+    auto products = [&](int i) {
+#pragma unroll
+        for (int gi = 0; gi < kGroups; ++gi) {
+            constexpr int kPer = 4 / kGroups;
+            // sums of X over the group's columns, in the places of their rows of C: a product with ones
             float xs[NR][4];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (c + q * 8 < p.K) v = load16(xp[r] + c);
-                b[r][0] = __byte_perm(v.x, v.z, 0x5410);
-                b[r][1] = __byte_perm(v.x, v.z, 0x7632);
-                b[r][2] = __byte_perm(v.y, v.w, 0x5410);
-                b[r][3] = __byte_perm(v.y, v.w, 0x7632);
-                if constexpr (kBf16) {
-                    // 2^64, and 2^60 where the codes are sixteen times theirs: exact, beyond FP32 from |x| = 2^63 on
-                    const __nv_bfloat162 up = __float2bfloat162_rn(0x1p64f), up16 = __float2bfloat162_rn(0x1p60f);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        __nv_bfloat162& f = reinterpret_cast<__nv_bfloat162&>(b[r][i]);
-                        f = __hmul2(f, (i & 1) ? up16 : up);
-                    }
-                }
-                // sums of X over the 32 columns, in the places of their rows of C
-                constexpr uint32_t kOne = kBf16 ? 0x3f803f80u : 0x3c003c00u, kOdd = kBf16 ? 0x41804180u : kOne;
                 xs[r][0] = xs[r][1] = xs[r][2] = xs[r][3] = 0.0f;
-                mma16<kBf16>(xs[r], kOne, kOne, kOne, kOne, b[r][0], b[r][2]);
-                mma16<kBf16>(xs[r], kOdd, kOdd, kOdd, kOdd, b[r][1], b[r][3]);
+#pragma unroll
+                for (int s = gi * kPer; s < (gi + 1) * kPer; ++s) {
+                    uint4& v = xv[i][s][r];
+                    if constexpr (kBf16) {
+                        // 2^64, and 2^60 where the codes are sixteen times theirs: exact, beyond FP32 from |x| = 2^63 on
+                        v.x = times_pow2(v.x, 0x5f805f80u);
+                        v.y = times_pow2(v.y, 0x5f805f80u);
+                        v.z = times_pow2(v.z, 0x5d805d80u);
+                        v.w = times_pow2(v.w, 0x5d805d80u);
+                    }
+                    constexpr uint32_t kOne = kBf16 ? 0x3f803f80u : 0x3c003c00u, kOdd = kBf16 ? 0x41804180u : kOne;
+                    mma16<kBf16>(xs[r], kOne, kOne, kOne, kOne, v.x, v.y);
+                    mma16<kBf16>(xs[r], kOdd, kOdd, kOdd, kOdd, v.z, v.w);
+                }
                 if constexpr (kBf16) {
                     xs[r][0] *= 0x1p-64f;
                     xs[r][1] *= 0x1p-64f;
@@ -109,23 +118,48 @@ __global__ void __launch_bounds__(W * 32) w4_linear_kernel(const __grid_constant
             }
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                uint32_t u[2][4];
-                float2 sl[2];
+                // (two sums, half as long a chain of products each; FP16: X cannot carry the 1 / 16 of the odd pairs)
+                float d[NR][4] = {}, e[NR][4] = {};
+#pragma unroll
+                for (int s = gi * kPer; s < (gi + 1) * kPer; ++s) {
+                    uint32_t u[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint4& w = wv[i][t][h];
+                        codes8(s == 0 ? w.x : s == 1 ? w.y : s == 2 ? w.z : w.w, u[h]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        const uint4& v = xv[i][s][r];
+                        mma16<kBf16>(d[r], u[0][0], u[1][0], u[0][2], u[1][2], v.x, v.y);
+                        mma16<kBf16>(e[r], u[0][1], u[1][1], u[0][3], u[1][3], v.z, v.w);
+                    }
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    codes8<kBf16>(w[t][h][s], u[h]);
-                    sl[h] = layer_pair<kBf16>(sc[t][h][s * kGroups / 4]);
-                    sl[h].x *= kBf16 ? 0x1p69f : 0x1p24f;
-                }
+                    float2 sl = layer_pair<kBf16>(sv[i][t][h][gi]);
+                    sl.x *= kBf16 ? 0x1p69f : 0x1p24f;
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    float d[4] = {};
-                    mma16<kBf16>(d, u[0][0], u[1][0], u[0][2], u[1][2], b[r][0], b[r][2]);
-                    mma16<kBf16>(d, u[0][1], u[1][1], u[0][3], u[1][3], b[r][1], b[r][3]);
+                    for (int r = 0; r < NR; ++r) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        y[t][r][e] = fmaf(d[e], sl[e >> 1].x, fmaf(xs[r][e & 1], sl[e >> 1].y, y[t][r][e]));
+                        for (int c = 0; c < 2; ++c) {
+                            const float f = kBf16 ? d[r][2 * h + c] + e[r][2 * h + c] : fmaf(e[r][2 * h + c], 0.0625f, d[r][2 * h + c]);
+                            y[t][r][2 * h + c] = fmaf(f, sl.x, fmaf(xs[r][c], sl.y, y[t][r][2 * h + c]));
+                        }
+                    }
                 }
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+        if (next < a.k_tiles) fetch(i);
+    for (int kt = first; kt < a.k_tiles; kt += D * step) {
+#pragma unroll
+        for (int i = 0; i < D; ++i) {
+            if (kt + i * step < a.k_tiles) {
+                products(i);
+                if (next < a.k_tiles) fetch(i);
             }
         }
     }
@@ -182,7 +216,12 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const W4PackArgs a) {
             const int lane = (at >> 2) & 31, s = at & 3;
             const long long row = row0 + (lane >> 2) + 8 * (at >> 7), col = kt * 128ll + s * 32 + (lane & 3) * 8;
             if (row < a.N && col < a.K)
-                for (int b = 0; b < 4; ++b) v |= static_cast<uint32_t>(a.codes[row * a.codes_ld + col / 2 + b]) << (8 * b);
+                for (int b = 0; b < 4; ++b) {
+                    // columns 2 b and 2 b + 1 are the pair 0, 2, 1, 3 of codes8: those of a product lie side by side in X
+                    const int pair = (b & 1) * 2 + (b >> 1);
+                    const uint32_t two = a.codes[row * a.codes_ld + col / 2 + b];
+                    v |= (two & 15u) << (4 * pair) | (two >> 4) << (16 + 4 * pair);
+                }
         } else {
             const int groups = 128 / a.group, j = at - 256;
             const long long row = row0 + j / groups, grp = static_cast<long long>(kt) * groups + j % groups;
@@ -195,9 +234,9 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const W4PackArgs a) {
     }
 }
 
-template <bool kBf16, int kGroups, int W, int T, int NR>
-cudaError_t go_w4(const W4Args& a, cudaStream_t stream) {
-    const auto kern = w4_linear_kernel<kBf16, kGroups, W, T, NR>;
+template <bool kBf16, int kGroups, int W, int T, int NR, int D, int kCtas>
+cudaError_t go_w4_few(const W4Args& a, cudaStream_t stream) {
+    const auto kern = w4_few_kernel<kBf16, kGroups, W, T, NR, D, kCtas>;
     const int smem = (W + a.parts) * 16 * T * 8 * NR * 4;
     const cudaError_t e = set_max_smem_once(kern, smem);
     if (e != cudaSuccess) return e;
@@ -206,19 +245,43 @@ cudaError_t go_w4(const W4Args& a, cudaStream_t stream) {
     return launch_dependent_cluster(kern, grid, dim3(W * 32), smem, stream, dim3(a.parts), a);
 }
 
+// Which kernel: the one whose CTAs all run at once (n of them to an SM) with the fewest tiles to a warp behind one another, so
+// that nearly all of W is on its way at the same time; K over a cluster where that takes it.  Few tiles: a row tile to a CTA, both of a
+// warp's K tiles in registers (1368 x 1291, one row 2.3 us, two row tiles to a CTA 2.7; 2560 x 1280 2.5 and 2.7).  More:
+// two row tiles to a CTA of eight warps, two or three CTAs to an SM (2560 x 2560 over three CTAs 2.9, over two 3.9, whole 4.1; 10240 x 2560
+// whole 5.8, over two 8.3), and of four warps, five CTAs to an SM, for the rest (5120 x 5120 over four 6.0, over two CTAs of eight warps
+// 6.8; 20480 x 5120 15.3, 15.6).
 template <bool kBf16, int kGroups>
 cudaError_t pick_w4(W4Args a, cudaStream_t stream) {
-    const int tiles = (a.p.N - 1) / 16 + 1;
-    auto parts = [&](int w, int t) {
-        int n = 1;
-        while (n < kW4MaxParts && (tiles + t - 1) / t * n * 2 <= 4 * sm_count() && a.k_tiles >= 2 * n * w) n *= 2;
-        return n;
+    const int sms = sm_count(), tiles = (a.p.N - 1) / 16 + 1, pairs = (tiles + 1) / 2, kt = a.k_tiles;
+    // the fewest CTAs to a cluster with which a warp has no more than `most` K tiles, if `ctas` such clusters fit `room` CTAs; or 0
+    auto split = [&](int ctas, long long room, int warps, int most) {
+        for (int p = 1; p <= kW4MaxParts && p * static_cast<long long>(ctas) <= room; ++p)
+            if ((kt - 1) / (warps * p) + 1 <= most) return p;
+        return 0;
     };
-    a.parts = parts(8, 2);
-    if (a.p.M <= 8) return go_w4<kBf16, kGroups, 8, 2, 1>(a, stream);
-    if (a.p.M <= 16) return go_w4<kBf16, kGroups, 8, 2, 2>(a, stream);
-    if (a.p.M <= 32) return go_w4<kBf16, kGroups, 8, 2, 4>(a, stream);
-    return go_w4<kBf16, kGroups, 8, 1, 8>(a, stream);
+    // as many as there is room for with two K tiles to a warp
+    auto spread = [&](int ctas, long long room, int warps) {
+        int p = 1;
+        while (p < kW4MaxParts && (p * 2) * static_cast<long long>(ctas) <= room && kt >= warps * p * 4) p *= 2;
+        return p;
+    };
+    if (a.p.M <= 8) {
+        if ((a.parts = split(tiles, 2ll * sms, 8, 2)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 1, 2, 2>(a, stream);
+        if ((a.parts = split(pairs, 2ll * sms, 8, 1)) != 0 || (a.parts = split(pairs, sms, 8, 2)) != 0)
+            return go_w4_few<kBf16, kGroups, 8, 2, 1, 1, 2>(a, stream);
+        a.parts = 1;
+        if (pairs <= 3 * sms && kt <= 24) return go_w4_few<kBf16, kGroups, 8, 2, 1, 1, 3>(a, stream);
+        a.parts = spread(pairs, 5ll * sms, 4);
+        return go_w4_few<kBf16, kGroups, 4, 2, 1, 1, 5>(a, stream);
+    }
+    if (a.p.M <= 16) {
+        if ((a.parts = split(tiles, sms, 8, 2)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 2, 1>(a, stream);
+        if ((a.parts = split(tiles, 2ll * sms, 8, 3)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 1, 2>(a, stream);
+    }
+    // more rows: sixteen a pass
+    a.parts = spread(pairs * ((a.p.M - 1) / 16 + 1), 3ll * sms, 4);
+    return go_w4_few<kBf16, kGroups, 4, 2, 2, 1, 3>(a, stream);
 }
 
 }  // namespace
