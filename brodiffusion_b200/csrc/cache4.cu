@@ -1,141 +1,204 @@
 // New rows of K and V into a cache of 4-bit groups, and rows of it back to 16 bits.
 //   group of a head's row:  low = min x,  step = (max x - min x) / 15 rounded to the storage type,
 //                           u = round((x - low) / step) in 0..15 (0 where step is 0),  value low + step u
-// A group with a value that is not finite has step and low NaN.  The quotients are IEEE ones, so that the same row has the same
-// codes wherever it is worked out.
+// A group with a value that is not finite has step and low NaN.  The quotients are rounded correctly, so that the same row has the
+// same codes wherever it is worked out (values of 16 bits lie on the border between two codes every few hundred times).
 //
 // A head's row is HD / 2 bytes of codes and a (step, low) pair for each group.  Its codes lie in the order in which the attention
 // kernel's lanes want them (S = HD / 32):
 //   K: the word of columns 32 s + 8 q + 0..7 is word q S + s       (q < 4: lanes of a key, a load of S words each)
 //   V: the half word of columns 32 s + 4 g + 0..3 is half g S + s  (g < 8: lanes of a column block)
-// Both kernels move bytes: a lane has four columns, so that a row of 128 columns is a warp's 256 bytes, and four
-// rows of heads are on their way at once.
+// Both kernels move bytes.  A lane has eight columns, so that a warp has two rows of 128 columns (four of 64) of a head, and kCacheTurns
+// such at once: reads of whole rows, writes that lie behind one another.
 #include "four_bit.cuh"
 #include "sdpa_window.cuh"
 
 namespace bdattn {
 namespace {
 
-constexpr int kCacheItems = 4;      // rows of heads in flight to a lane
+constexpr int kCacheTurns = 4;
 
-// One row of one head of K (0) or V (1): where it is in the cache and in the 16-bit tensor.
-struct CacheItem {
-    bool on;
-    int kv, pos;
-    const uint16_t* x;
-    long long codes, scales;
+// A lane's part of a call: columns 8 i .. 8 i + 7 of row `row` + turn * `rows` of K or V of a head.
+struct CacheLane {
+    int i, row, rows, place0, s, q;
+    uint16_t* x;
+    long long ld;
+    uint8_t* codes;
+    uint16_t* scales;
+    bool v;
+    __device__ __forceinline__ explicit CacheLane(const Cache4RowsArgs& a) {
+        const int lanes = a.c.head_dim / 8, lane = threadIdx.x & 31, head = blockIdx.y >> 1, b = blockIdx.z;
+        v = (blockIdx.y & 1) != 0;
+        i = lane & (lanes - 1);
+        s = i >> 2;
+        q = i & 3;
+        rows = 32 / lanes;
+        row = (static_cast<int>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * rows * kCacheTurns + lane / lanes;
+        place0 = window_keys(a.kv_len, b, a.c.rows) - a.n_rows;
+        ld = v ? a.v_ld : a.k_ld;
+        x = reinterpret_cast<uint16_t*>(const_cast<void*>(v ? a.v : a.k)) + b * (v ? a.v_bs : a.k_bs) + static_cast<long long>(head) * a.c.head_dim + 8 * i;
+        codes = (v ? a.c.v_codes : a.c.k_codes) + b * a.c.codes_bs + head * a.c.codes_hs;
+        scales = (v ? a.c.v_scales : a.c.k_scales) + b * a.c.scales_bs + head * a.c.scales_hs;
+    }
+    __device__ __forceinline__ uint8_t* codes_at(int place, int hd) const { return codes + static_cast<long long>(place) * (hd / 2); }
+    __device__ __forceinline__ uint32_t* pair_at(int place, int hd, int group) const {
+        return reinterpret_cast<uint32_t*>(scales + static_cast<long long>(place) * (2 * hd / group)) + 8 * i / group;
+    }
 };
-__device__ __forceinline__ CacheItem cache_item(const Cache4RowsArgs& a, long long item) {
-    CacheItem r;
-    r.on = item < a.items;
-    if (!r.on) item = 0;
-    r.kv = static_cast<int>(item & 1);
-    const long long row = (item >> 1) / a.c.kv_heads;
-    const int head = static_cast<int>((item >> 1) - row * a.c.kv_heads), b = static_cast<int>(row / a.n_rows), i = static_cast<int>(row - static_cast<long long>(b) * a.n_rows);
-    r.pos = window_keys(a.kv_len, b, a.c.rows) - a.n_rows + i;
-    r.x = reinterpret_cast<const uint16_t*>(r.kv ? a.v : a.k) + b * (r.kv ? a.v_bs : a.k_bs) + i * (r.kv ? a.v_ld : a.k_ld) + head * static_cast<long long>(a.c.head_dim);
-    r.codes = b * a.c.codes_bs + head * a.c.codes_hs + static_cast<long long>(r.pos) * (a.c.head_dim / 2);
-    r.scales = b * a.c.scales_bs + head * a.c.scales_hs + static_cast<long long>(r.pos) * (2 * a.c.head_dim / a.c.group);
+
+// The smaller, or larger, of two pairs of values; NaN stays.
+template <bool kBf16, bool kMax>
+__device__ __forceinline__ uint32_t extreme2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (kBf16 && kMax) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (kBf16) asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (kMax) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-// The half word of this lane's four columns 4 i .. 4 i + 3 in a row.
-__device__ __forceinline__ int half_of(int i, int kv, int S) {
-    const int s = i >> 3, g = i & 7;
-    return kv ? g * S + s : ((g >> 1) * S + s) * 2 + (g & 1);
+
+// a / b rounded to the nearest, by Markstein's correction of a * (1 / b); inv is 1 / b rounded to the nearest, the quotient neither
+// huge nor tiny.
+__device__ __forceinline__ float quotient(float a, float b, float inv) {
+    const float q = a * inv;
+    return fmaf(fmaf(-q, b, a), inv, q);
 }
 
 template <bool kBf16>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4RowsArgs a) {
-    if (gridDim.x <= 148) dependents_may_launch();
+    dependents_may_launch();
     wait_for_prior_grid();
-    const int lanes = a.c.head_dim / 4, i = threadIdx.x % lanes, per = 256 / lanes, team = a.c.group / 4;
-    const int half_k = half_of(i, 0, a.c.head_dim / 32), half_v = half_of(i, 1, a.c.head_dim / 32);
-    // (lanes that belong together are in one warp and take the same turns)
-    for (long long base = static_cast<long long>(blockIdx.x) * per * kCacheItems; base < a.items; base += static_cast<long long>(gridDim.x) * per * kCacheItems) {
-        uint2 x[kCacheItems];
-        CacheItem it[kCacheItems];
+    const CacheLane at(a);
+    const int hd = a.c.head_dim, team = a.c.group / 8;
+    uint4 x[kCacheTurns];
 #pragma unroll
-        for (int n = 0; n < kCacheItems; ++n) {
-            it[n] = cache_item(a, base + n * per + threadIdx.x / lanes);
-            x[n] = load8_once(it[n].x + 4 * i);
+    for (int n = 0; n < kCacheTurns; ++n) {
+        const int row = at.row + n * at.rows;
+        x[n] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < a.n_rows) x[n] = load16_once(at.x + row * at.ld);
+    }
+#pragma unroll
+    for (int n = 0; n < kCacheTurns; ++n) {
+        if (at.row - static_cast<int>(threadIdx.x & 31) / (hd / 8) + n * at.rows >= a.n_rows) break;          // (of the whole warp)
+        const int row = at.row + n * at.rows, place = at.place0 + row;
+        uint32_t lo2 = extreme2<kBf16, false>(extreme2<kBf16, false>(x[n].x, x[n].y), extreme2<kBf16, false>(x[n].z, x[n].w));
+        uint32_t hi2 = extreme2<kBf16, true>(extreme2<kBf16, true>(x[n].x, x[n].y), extreme2<kBf16, true>(x[n].z, x[n].w));
+        for (int o = 1; o < team; o *= 2) {
+            lo2 = extreme2<kBf16, false>(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
+            hi2 = extreme2<kBf16, true>(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
         }
+        const float low = layer_pair<kBf16>(extreme2<kBf16, false>(lo2, lo2 >> 16)).x, high = layer_pair<kBf16>(extreme2<kBf16, true>(hi2, hi2 >> 16)).x;
+        uint32_t pair = pack2<kBf16>(quotient(high - low, 15.0f, 1.0f / 15.0f), low);
+        float step = layer_pair<kBf16>(pair).x;
+        // (a value that is not finite has made one of both so)
+        if (!(step <= FLT_MAX && fabsf(low) <= FLT_MAX)) {
+            pair = kBf16 ? 0x7fc07fc0u : 0x7e007e00u;
+            step = 0.0f;
+        }
+        // 1.5 * 2^23 more than a quotient is the nearest integer in the low bits; eight of them are added up shifted, and what the
+        // rest of their bits comes to is taken off
+        constexpr float kRound = 12582912.0f;
+        constexpr uint32_t kRest = 0x4b400000u * 0x11111111u;
+        uint32_t codes = 0;
+        if (step > 0.0f) {
+            const float inv = __frcp_rn(step);
+            const uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
 #pragma unroll
-        for (int n = 0; n < kCacheItems; ++n) {
-            const float2 f0 = layer_pair<kBf16>(x[n].x), f1 = layer_pair<kBf16>(x[n].y);
-            const float f[4] = {f0.x, f0.y, f1.x, f1.y};
-            float lo = fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), hi = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
-            // (minimum and maximum leave NaN out; the sum of |x| does not, nor an infinity)
-            bool odd = !(fabsf(f[0]) + fabsf(f[1]) + fabsf(f[2]) + fabsf(f[3]) <= FLT_MAX);
-            if (odd) odd = !(fabsf(f[0]) <= FLT_MAX && fabsf(f[1]) <= FLT_MAX && fabsf(f[2]) <= FLT_MAX && fabsf(f[3]) <= FLT_MAX);
-            for (int o = 1; o < team; o *= 2) {
-                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            }
-            const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-            const uint32_t mine = (team == 32 ? 0xffffffffu : (1u << team) - 1u) << ((threadIdx.x & 31) & ~(team - 1));
-            uint32_t pair = pack2<kBf16>(__fdiv_rn(hi - lo, 15.0f), lo);
-            float step = layer_pair<kBf16>(pair).x;
-            if ((odds & mine) != 0 || !(step <= FLT_MAX)) {
-                pair = kBf16 ? 0x7fc07fc0u : 0x7e007e00u;
-                step = 0.0f;
-            }
-            uint32_t codes = 0;
-            if (step > 0.0f) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float u = fminf(rintf(__fdiv_rn(f[e] - lo, step)), 15.0f);
-                    codes |= static_cast<uint32_t>(u) << (4 * e);
+            for (int e = 3; e >= 0; --e) {
+                const float2 f = layer_pair<kBf16>(w[e]);
+                // (only steps below FP16's smallest normal are so much smaller than a fifteenth of the range that a code could be 16)
+                float u[2] = {quotient(f.x - low, step, inv), quotient(f.y - low, step, inv)};
+                if (!kBf16) {
+                    u[0] = fminf(u[0], 15.0f);
+                    u[1] = fminf(u[1], 15.0f);
                 }
+                codes = codes * 16 + __float_as_uint(u[1] + kRound);
+                codes = codes * 16 + __float_as_uint(u[0] + kRound);
             }
-            // (a place outside the cache is not written)
-            if (it[n].on && it[n].pos >= 0 && it[n].pos < a.c.rows) {
-                reinterpret_cast<uint16_t*>((it[n].kv ? a.c.v_codes : a.c.k_codes) + it[n].codes)[it[n].kv ? half_v : half_k] = static_cast<uint16_t>(codes);
-                if (i % team == 0)
-                    reinterpret_cast<uint32_t*>((it[n].kv ? a.c.v_scales : a.c.k_scales) + it[n].scales)[i / team] = pair;
+            codes -= kRest;
+        }
+        // (a place outside the cache is not written)
+        if (row < a.n_rows && place >= 0 && place < a.c.rows) {
+            const int S = hd / 32;
+            uint8_t* const p = at.codes_at(place, hd);
+            if (at.v) {
+                reinterpret_cast<uint16_t*>(p)[2 * at.q * S + at.s] = static_cast<uint16_t>(codes);
+                reinterpret_cast<uint16_t*>(p)[(2 * at.q + 1) * S + at.s] = static_cast<uint16_t>(codes >> 16);
+            } else {
+                reinterpret_cast<uint32_t*>(p)[at.q * S + at.s] = codes;
             }
+            if (at.i % team == 0) *at.pair_at(place, hd, a.c.group) = pair;
         }
     }
 }
 
 template <bool kBf16>
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4RowsArgs a) {
-    if (gridDim.x <= 148) dependents_may_launch();
+    dependents_may_launch();
     wait_for_prior_grid();
-    const int lanes = a.c.head_dim / 4, i = threadIdx.x % lanes, per = 256 / lanes, team = a.c.group / 4;
-    const int half_k = half_of(i, 0, a.c.head_dim / 32), half_v = half_of(i, 1, a.c.head_dim / 32);
-    for (long long base = static_cast<long long>(blockIdx.x) * per * kCacheItems; base < a.items; base += static_cast<long long>(gridDim.x) * per * kCacheItems) {
-        uint32_t codes[kCacheItems], pair[kCacheItems];
-        CacheItem it[kCacheItems];
+    const CacheLane at(a);
+    const int hd = a.c.head_dim, S = hd / 32;
+    uint32_t codes[kCacheTurns], pair[kCacheTurns];
 #pragma unroll
-        for (int n = 0; n < kCacheItems; ++n) {
-            it[n] = cache_item(a, base + n * per + threadIdx.x / lanes);
-            codes[n] = pair[n] = 0;              // (zeros from outside the cache)
-            if (it[n].on && it[n].pos >= 0 && it[n].pos < a.c.rows) {
-                uint16_t c;
-                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c) : "l"(reinterpret_cast<const uint16_t*>((it[n].kv ? a.c.v_codes : a.c.k_codes) + it[n].codes) + (it[n].kv ? half_v : half_k)));
-                codes[n] = c;
-                pair[n] = load4_once(reinterpret_cast<const uint32_t*>((it[n].kv ? a.c.v_scales : a.c.k_scales) + it[n].scales) + i / team);
+    for (int n = 0; n < kCacheTurns; ++n) {
+        const int row = at.row + n * at.rows, place = at.place0 + row;
+        codes[n] = pair[n] = 0;              // (zeros from outside the cache)
+        if (row < a.n_rows && place >= 0 && place < a.c.rows) {
+            const uint8_t* const p = at.codes_at(place, hd);
+            if (at.v) {
+                uint16_t c0, c1;
+                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c0) : "l"(reinterpret_cast<const uint16_t*>(p) + 2 * at.q * S + at.s));
+                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c1) : "l"(reinterpret_cast<const uint16_t*>(p) + (2 * at.q + 1) * S + at.s));
+                codes[n] = static_cast<uint32_t>(c0) | static_cast<uint32_t>(c1) << 16;
+            } else {
+                asm volatile("ld.global.u32 %0, [%1];" : "=r"(codes[n]) : "l"(reinterpret_cast<const uint32_t*>(p) + at.q * S + at.s));
             }
+            asm volatile("ld.global.u32 %0, [%1];" : "=r"(pair[n]) : "l"(at.pair_at(place, hd, a.c.group)));
         }
+    }
 #pragma unroll
-        for (int n = 0; n < kCacheItems; ++n) {
-            const float2 s = layer_pair<kBf16>(pair[n]);
-            float f[4];
+    for (int n = 0; n < kCacheTurns; ++n) {
+        const int row = at.row + n * at.rows;
+        if (row >= a.n_rows) break;
+        const float2 s = layer_pair<kBf16>(pair[n]);
+        uint32_t r[4], out[4];
+        // low + step u for the pairs (j, j + 4) of the word, rounded once by a fused multiplication and addition in 16 bits: a code behind
+        // the bits of 128 (1024) is that much more than itself
+        const uint32_t step2 = __byte_perm(pair[n], 0, 0x1010), low2 = __byte_perm(pair[n], 0, 0x3232);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t u = ((codes[n] >> (4 * e)) & 0x000f000fu) | (kBf16 ? 0x43004300u : 0x64006400u);
+            if constexpr (kBf16) asm("{.reg .b32 t; sub.rn.bf16x2 t, %1, %2; fma.rn.bf16x2 %0, t, %3, %4;}" : "=r"(r[e]) : "r"(u), "r"(0x43004300u), "r"(step2), "r"(low2));
+            else asm("{.reg .b32 t; sub.rn.f16x2 t, %1, %2; fma.rn.f16x2 %0, t, %3, %4;}" : "=r"(r[e]) : "r"(u), "r"(0x64006400u), "r"(step2), "r"(low2));
+        }
+        out[0] = __byte_perm(r[0], r[1], 0x5410);
+        out[1] = __byte_perm(r[2], r[3], 0x5410);
+        out[2] = __byte_perm(r[0], r[1], 0x7632);
+        out[3] = __byte_perm(r[2], r[3], 0x7632);
+        // (the rounded step may take the largest value past the type's range; NaN stays)
+        const float most = kBf16 ? 0x1.fep127f : 65504.0f;
+        if (fabsf(fmaf(s.x, 15.0f, s.y)) > most) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                // (the rounded step may take the largest value past the type's range; NaN stays)
-                const float v = fmaf(s.x, static_cast<float>((codes[n] >> (4 * e)) & 15u), s.y), most = kBf16 ? 0x1.fep127f : 65504.0f;
-                f[e] = v > most ? most : v < -most ? -most : v;
+                float f[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float v = fmaf(s.x, static_cast<float>((codes[n] >> (8 * e + 4 * h)) & 15u), s.y);
+                    f[h] = v > most ? most : v < -most ? -most : v;
+                }
+                out[e] = pack2<kBf16>(f[0], f[1]);
             }
-            if (it[n].on) *reinterpret_cast<uint2*>(const_cast<uint16_t*>(it[n].x) + 4 * i) = make_uint2(pack2<kBf16>(f[0], f[1]), pack2<kBf16>(f[2], f[3]));
         }
+        *reinterpret_cast<uint4*>(at.x + row * at.ld) = make_uint4(out[0], out[1], out[2], out[3]);
     }
 }
 
 template <class Kernel>
 cudaError_t launch_rows(Kernel kern, const Cache4RowsArgs& a, cudaStream_t stream) {
-    const long long per = 256 / (a.c.head_dim / 4) * kCacheItems, ctas = (a.items + per - 1) / per, most = 8ll * sm_count();
-    return launch_dependent(kern, dim3(static_cast<unsigned>(ctas < most ? ctas : most)), dim3(256), 0, stream, a);
+    const int per = 256 / a.c.head_dim * kCacheTurns;          // rows of a warp
+    const int warps = (a.n_rows - 1) / per + 1, w = warps < 8 ? warps : 8;
+    return launch_dependent(kern, dim3(static_cast<unsigned>((warps - 1) / w + 1), static_cast<unsigned>(2 * a.c.kv_heads), static_cast<unsigned>(a.batch)),
+                            dim3(32 * w), 0, stream, a);
 }
 
 }  // namespace

@@ -13,8 +13,8 @@ bool is_group(int group) { return group == 32 || group == 64 || group == 128; }
 int cache4_of(const char* op, const bdattn_cache4* c, bdattn::Cache4Dev* d) {
     if (c == nullptr) return fail("%s: cache is null", op);
     if (!is_16bit(c->dtype)) return fail("%s: dtype must be BF16 or F16 (got %d)", op, c->dtype);
-    if (c->batch < 1 || c->batch > 65535 || c->num_kv_heads < 1 || c->num_kv_heads > 65535)
-        return fail("%s: batch and num_kv_heads must be in [1, 65535] (got %d and %d)", op, c->batch, c->num_kv_heads);
+    if (c->batch < 1 || c->batch > 65535 || c->num_kv_heads < 1 || c->num_kv_heads > 32767)
+        return fail("%s: batch must be in [1, 65535], num_kv_heads in [1, 32767] (got %d and %d)", op, c->batch, c->num_kv_heads);
     if (c->head_dim != 64 && c->head_dim != 128) return fail("%s: head_dim must be 64 or 128 (got %d)", op, c->head_dim);
     if (!is_group(c->group) || c->group > c->head_dim)
         return fail("%s: group must be 32, 64 or 128 and no larger than head_dim (got %d)", op, c->group);
@@ -81,7 +81,7 @@ int cache4_rows(const char* op, const bdattn_cache4* c, const bdattn_cache4_rows
     a.v = r->v;
     a.n_rows = r->rows;
     a.kv_len = r->kv_len;
-    a.items = 2ll * c->batch * r->rows * c->num_kv_heads;
+    a.batch = c->batch;
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool bf16 = c->dtype == BDATTN_BF16;
     const cudaError_t e = append ? bdattn::launch_cache4_append(a, bf16, st) : bdattn::launch_cache4_read(a, bf16, st);

@@ -303,8 +303,7 @@ struct Cache4RowsArgs {
     const void* k;
     const void* v;
     long long k_ld, v_ld, k_bs, v_bs;
-    int n_rows;
-    long long items;           // batch * n_rows * kv_heads * 2
+    int n_rows, batch;
     const int* kv_len;
 };
 cudaError_t launch_cache4_append(const Cache4RowsArgs& a, bool bf16, cudaStream_t stream);
