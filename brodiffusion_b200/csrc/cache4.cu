@@ -18,31 +18,27 @@ namespace {
 
 constexpr int kCacheTurns = 4;
 
-// A lane's part of a call: columns 8 i .. 8 i + 7 of row `row` + turn * `rows` of K or V of a head.
+// A lane's part of a call: columns 8 i .. 8 i + 7 of row `row` + turn * kRows of K or V of a head.
+template <int HD, int kGroup>
 struct CacheLane {
-    int i, row, rows, place0, s, q;
+    static constexpr int kLanes = HD / 8, kRows = 32 / kLanes, S = HD / 32, kPairs = HD / kGroup;
+    int i, row, place0;
     uint16_t* x;
     long long ld;
     uint8_t* codes;
-    uint16_t* scales;
+    uint32_t* pairs;
     bool v;
     __device__ __forceinline__ explicit CacheLane(const Cache4RowsArgs& a) {
-        const int lanes = a.c.head_dim / 8, lane = threadIdx.x & 31, head = blockIdx.y >> 1, b = blockIdx.z;
+        const int lane = threadIdx.x & 31, head = blockIdx.y >> 1, b = blockIdx.z;
         v = (blockIdx.y & 1) != 0;
-        i = lane & (lanes - 1);
-        s = i >> 2;
-        q = i & 3;
-        rows = 32 / lanes;
-        row = (static_cast<int>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * rows * kCacheTurns + lane / lanes;
+        i = lane % kLanes;
+        row = (static_cast<int>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kRows * kCacheTurns + lane / kLanes;
         place0 = window_keys(a.kv_len, b, a.c.rows) - a.n_rows;
         ld = v ? a.v_ld : a.k_ld;
-        x = reinterpret_cast<uint16_t*>(const_cast<void*>(v ? a.v : a.k)) + b * (v ? a.v_bs : a.k_bs) + static_cast<long long>(head) * a.c.head_dim + 8 * i;
-        codes = (v ? a.c.v_codes : a.c.k_codes) + b * a.c.codes_bs + head * a.c.codes_hs;
-        scales = (v ? a.c.v_scales : a.c.k_scales) + b * a.c.scales_bs + head * a.c.scales_hs;
-    }
-    __device__ __forceinline__ uint8_t* codes_at(int place, int hd) const { return codes + static_cast<long long>(place) * (hd / 2); }
-    __device__ __forceinline__ uint32_t* pair_at(int place, int hd, int group) const {
-        return reinterpret_cast<uint32_t*>(scales + static_cast<long long>(place) * (2 * hd / group)) + 8 * i / group;
+        x = reinterpret_cast<uint16_t*>(const_cast<void*>(v ? a.v : a.k)) + b * (v ? a.v_bs : a.k_bs) + static_cast<long long>(head) * HD + 8 * i;
+        // (this lane's word of K, or its first half word of V, is at the same place in every row)
+        codes = (v ? a.c.v_codes : a.c.k_codes) + b * a.c.codes_bs + head * a.c.codes_hs + (v ? (2 * (i & 3) * S + (i >> 2)) * 2 : ((i & 3) * S + (i >> 2)) * 4);
+        pairs = reinterpret_cast<uint32_t*>((v ? a.c.v_scales : a.c.k_scales) + b * a.c.scales_bs + head * a.c.scales_hs) + 8 * i / kGroup;
     }
 };
 
@@ -64,26 +60,28 @@ __device__ __forceinline__ float quotient(float a, float b, float inv) {
     return fmaf(fmaf(-q, b, a), inv, q);
 }
 
-template <bool kBf16>
+template <bool kBf16, int HD, int kGroup>
 __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4RowsArgs a) {
     dependents_may_launch();
     wait_for_prior_grid();
-    const CacheLane at(a);
-    const int hd = a.c.head_dim, team = a.c.group / 8;
+    using Lane = CacheLane<HD, kGroup>;
+    const Lane at(a);
+    constexpr int kTeam = kGroup / 8;
     uint4 x[kCacheTurns];
 #pragma unroll
     for (int n = 0; n < kCacheTurns; ++n) {
-        const int row = at.row + n * at.rows;
+        const int row = at.row + n * Lane::kRows;
         x[n] = make_uint4(0u, 0u, 0u, 0u);
         if (row < a.n_rows) x[n] = load16_once(at.x + row * at.ld);
     }
 #pragma unroll
     for (int n = 0; n < kCacheTurns; ++n) {
-        if (at.row - static_cast<int>(threadIdx.x & 31) / (hd / 8) + n * at.rows >= a.n_rows) break;          // (of the whole warp)
-        const int row = at.row + n * at.rows, place = at.place0 + row;
+        if (at.row - static_cast<int>(threadIdx.x & 31) / Lane::kLanes + n * Lane::kRows >= a.n_rows) break;          // (of the whole warp)
+        const int row = at.row + n * Lane::kRows, place = at.place0 + row;
         uint32_t lo2 = extreme2<kBf16, false>(extreme2<kBf16, false>(x[n].x, x[n].y), extreme2<kBf16, false>(x[n].z, x[n].w));
         uint32_t hi2 = extreme2<kBf16, true>(extreme2<kBf16, true>(x[n].x, x[n].y), extreme2<kBf16, true>(x[n].z, x[n].w));
-        for (int o = 1; o < team; o *= 2) {
+#pragma unroll
+        for (int o = 1; o < kTeam; o *= 2) {
             lo2 = extreme2<kBf16, false>(lo2, __shfl_xor_sync(0xffffffffu, lo2, o));
             hi2 = extreme2<kBf16, true>(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
         }
@@ -119,46 +117,45 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4RowsArgs
         }
         // (a place outside the cache is not written)
         if (row < a.n_rows && place >= 0 && place < a.c.rows) {
-            const int S = hd / 32;
-            uint8_t* const p = at.codes_at(place, hd);
+            uint8_t* const p = at.codes + static_cast<long long>(place) * (HD / 2);
             if (at.v) {
-                reinterpret_cast<uint16_t*>(p)[2 * at.q * S + at.s] = static_cast<uint16_t>(codes);
-                reinterpret_cast<uint16_t*>(p)[(2 * at.q + 1) * S + at.s] = static_cast<uint16_t>(codes >> 16);
+                *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(codes);
+                *reinterpret_cast<uint16_t*>(p + 2 * Lane::S) = static_cast<uint16_t>(codes >> 16);
             } else {
-                reinterpret_cast<uint32_t*>(p)[at.q * S + at.s] = codes;
+                *reinterpret_cast<uint32_t*>(p) = codes;
             }
-            if (at.i % team == 0) *at.pair_at(place, hd, a.c.group) = pair;
+            if (at.i % kTeam == 0) at.pairs[static_cast<long long>(place) * Lane::kPairs] = pair;
         }
     }
 }
 
-template <bool kBf16>
+template <bool kBf16, int HD, int kGroup>
 __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4RowsArgs a) {
     dependents_may_launch();
     wait_for_prior_grid();
-    const CacheLane at(a);
-    const int hd = a.c.head_dim, S = hd / 32;
+    using Lane = CacheLane<HD, kGroup>;
+    const Lane at(a);
     uint32_t codes[kCacheTurns], pair[kCacheTurns];
 #pragma unroll
     for (int n = 0; n < kCacheTurns; ++n) {
-        const int row = at.row + n * at.rows, place = at.place0 + row;
+        const int row = at.row + n * Lane::kRows, place = at.place0 + row;
         codes[n] = pair[n] = 0;              // (zeros from outside the cache)
         if (row < a.n_rows && place >= 0 && place < a.c.rows) {
-            const uint8_t* const p = at.codes_at(place, hd);
+            const uint8_t* const p = at.codes + static_cast<long long>(place) * (HD / 2);
             if (at.v) {
                 uint16_t c0, c1;
-                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c0) : "l"(reinterpret_cast<const uint16_t*>(p) + 2 * at.q * S + at.s));
-                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c1) : "l"(reinterpret_cast<const uint16_t*>(p) + (2 * at.q + 1) * S + at.s));
+                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c0) : "l"(p));
+                asm volatile("ld.global.u16 %0, [%1];" : "=h"(c1) : "l"(p + 2 * Lane::S));
                 codes[n] = static_cast<uint32_t>(c0) | static_cast<uint32_t>(c1) << 16;
             } else {
-                asm volatile("ld.global.u32 %0, [%1];" : "=r"(codes[n]) : "l"(reinterpret_cast<const uint32_t*>(p) + at.q * S + at.s));
+                asm volatile("ld.global.u32 %0, [%1];" : "=r"(codes[n]) : "l"(p));
             }
-            asm volatile("ld.global.u32 %0, [%1];" : "=r"(pair[n]) : "l"(at.pair_at(place, hd, a.c.group)));
+            asm volatile("ld.global.u32 %0, [%1];" : "=r"(pair[n]) : "l"(at.pairs + static_cast<long long>(place) * Lane::kPairs));
         }
     }
 #pragma unroll
     for (int n = 0; n < kCacheTurns; ++n) {
-        const int row = at.row + n * at.rows;
+        const int row = at.row + n * Lane::kRows;
         if (row >= a.n_rows) break;
         const float2 s = layer_pair<kBf16>(pair[n]);
         uint32_t r[4], out[4];
@@ -200,14 +197,25 @@ cudaError_t launch_rows(Kernel kern, const Cache4RowsArgs& a, cudaStream_t strea
     return launch_dependent(kern, dim3(static_cast<unsigned>((warps - 1) / w + 1), static_cast<unsigned>(2 * a.c.kv_heads), static_cast<unsigned>(a.batch)),
                             dim3(32 * w), 0, stream, a);
 }
+template <bool kBf16, int HD, int kGroup>
+cudaError_t append_or_read(const Cache4RowsArgs& a, bool append, cudaStream_t stream) {
+    return append ? launch_rows(cache4_append_kernel<kBf16, HD, kGroup>, a, stream) : launch_rows(cache4_read_kernel<kBf16, HD, kGroup>, a, stream);
+}
+template <bool kBf16>
+cudaError_t pick_rows(const Cache4RowsArgs& a, bool append, cudaStream_t stream) {
+    const int g = a.c.group;
+    if (a.c.head_dim == 64) return g == 32 ? append_or_read<kBf16, 64, 32>(a, append, stream) : append_or_read<kBf16, 64, 64>(a, append, stream);
+    return g == 32 ? append_or_read<kBf16, 128, 32>(a, append, stream) : g == 64 ? append_or_read<kBf16, 128, 64>(a, append, stream)
+                                                                                 : append_or_read<kBf16, 128, 128>(a, append, stream);
+}
 
 }  // namespace
 
 cudaError_t launch_cache4_append(const Cache4RowsArgs& a, bool bf16, cudaStream_t stream) {
-    return launch_rows(bf16 ? cache4_append_kernel<true> : cache4_append_kernel<false>, a, stream);
+    return bf16 ? pick_rows<true>(a, true, stream) : pick_rows<false>(a, true, stream);
 }
 cudaError_t launch_cache4_read(const Cache4RowsArgs& a, bool bf16, cudaStream_t stream) {
-    return launch_rows(bf16 ? cache4_read_kernel<true> : cache4_read_kernel<false>, a, stream);
+    return bf16 ? pick_rows<true>(a, false, stream) : pick_rows<false>(a, false, stream);
 }
 
 }  // namespace bdattn
