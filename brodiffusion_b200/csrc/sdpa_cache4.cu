@@ -31,20 +31,42 @@ __device__ __forceinline__ void c4_store_cluster(uint32_t addr, float2 v) {
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-template <int HD, int W, int NR>
+template <int HD, int G, int W, int NR, int D>
 struct Cache4Cfg {
     static constexpr int kRows = 8 * NR, kLd = HD + 4, kMergeRows = kRows + kC4MaxSplit - 1;
-    static constexpr int kSmem = (W * kRows * (kLd + 2) + kMergeRows * (kLd + 2)) * 4;
+    static constexpr int kCodes = 16 * HD / 2, kScales = 16 * 4 * G, kStep = 2 * (kCodes + kScales);      // bytes of sixteen keys
+    static constexpr int kRing = W * D * kStep, kSums = W * kRows * kLd * 4;                              // (the sums lie in the ring's place)
+    static constexpr int kFirst = kRing > kSums ? kRing : kSums;
+    static constexpr int kSmem = kFirst + (kMergeRows * (kLd + 2) + W * kRows * 2) * 4;
 };
 
-// HD: 64 or 128.  G: groups of a row.  W: warps.  NR: query rows in eights.  kCtas: CTAs of an SM.
-template <int HD, int G, bool kBf16, int W, int NR, int kCtas>
+// Global to shared memory, 4, 8 or 16 bytes.
+template <int kBytes>
+__device__ __forceinline__ void c4_copy(uint32_t dst, const void* src) {
+    if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+}
+template <int kWords>
+__device__ __forceinline__ void c4_lds(const uint8_t* p, uint32_t (&w)[kWords]) {
+    if constexpr (kWords == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (kWords == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+
+// HD: 64 or 128.  G: groups of a row.  W: warps.  NR: query rows in eights.  D: steps of a warp in shared memory.  kCtas: CTAs of an SM.
+template <int HD, int G, bool kBf16, int W, int NR, int D, int kCtas>
 __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid_constant__ SdpaCache4Args a) {
-    using C = Cache4Cfg<HD, W, NR>;
+    using C = Cache4Cfg<HD, G, W, NR, D>;
     constexpr int S = HD / 32, kPer = S / G, kRows = C::kRows;
-    extern __shared__ float c4_smem[];
-    float* const o_warp = c4_smem;                                          // [W][kRows][kLd]
-    float* const o_cta = o_warp + W * kRows * C::kLd;                       // [kMergeRows][kLd]
+    extern __shared__ __align__(16) uint8_t c4_smem[];
+    float* const o_warp = reinterpret_cast<float*>(c4_smem);                // [W][kRows][kLd], once the rings are done with
+    float* const o_cta = reinterpret_cast<float*>(c4_smem + C::kFirst);     // [kMergeRows][kLd]
     float2* const ml_warp = reinterpret_cast<float2*>(o_cta + C::kMergeRows * C::kLd);     // [W][kRows]
     float2* const ml_cta = ml_warp + W * kRows;                             // [kMergeRows]
 
@@ -67,7 +89,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     // The queries in FP16, a power of two from where the largest of a row is in [2^14, 2^15): what that rounds is 2^-35 of
     // the largest.  This lane has row g's columns 32 s + 8 q + 0..7 as the pairs of codes8, those of the odd pairs over 16.
     uint32_t qf[NR][S][4];
-    float qs[NR][G][2], sl2[NR][2];       // of columns 2 q and 2 q + 1: sums over a group, factor of the scores
+    float qs[NR][2], sl2[NR][2];          // row g's sum over group q in two parts of 11 bits; factor of the scores of columns 2 q and 2 q + 1
     int pos[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -114,39 +136,46 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                 qf[nr][s][e] = pack2<false>(f[s][e] * l, f[s][e + 4] * l);
             }
         }
+        float mine = 0.0f;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) mine = q == gi ? sum[gi] : mine;
+        qs[nr][0] = __uint_as_float(__float_as_uint(mine) & 0xffffe000u);
+        qs[nr][1] = mine - qs[nr][0];
         const float down = pow2(-up) * (0x1p24f * a.scale * 1.4426950408889634f);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int from = (2 * q + h) * 4;
             sl2[nr][h] = __shfl_sync(0xffffffffu, down, from);
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) qs[nr][gi][h] = __shfl_sync(0xffffffffu, sum[gi], from);
             pos[nr][h] = first_pos + (row0 + min(nr * 8 + 2 * q + h, rows - 1)) / a.kv_group;
         }
     }
 
-    const uint8_t* const kc_base = a.c.k_codes + batch * a.c.codes_bs + kv_head * a.c.codes_hs + q * 4 * S;
-    const uint8_t* const vc_base = a.c.v_codes + batch * a.c.codes_bs + kv_head * a.c.codes_hs + g * 2 * S;
-    const uint16_t* const ks_base = a.c.k_scales + batch * a.c.scales_bs + kv_head * a.c.scales_hs;
-    const uint16_t* const vs_base = a.c.v_scales + batch * a.c.scales_bs + kv_head * a.c.scales_hs;
-    uint32_t kc[2][S], vc[4][S / 2], ks[2][G], vs[2][G];
-    auto fetch = [&](int step) {
+    // A step's keys come as they lie, sixteen bytes of codes and a key's pairs to a lane, into this warp's own part of shared
+    // memory; the pieces of V's rows change places so that the four keys that a quarter of a warp reads at once lie in different banks.
+    const uint8_t* const kc_base = a.c.k_codes + batch * a.c.codes_bs + kv_head * a.c.codes_hs;
+    const uint8_t* const vc_base = a.c.v_codes + batch * a.c.codes_bs + kv_head * a.c.codes_hs;
+    const uint16_t* const sc_base = (lane < 16 ? a.c.k_scales : a.c.v_scales) + batch * a.c.scales_bs + kv_head * a.c.scales_hs;
+    uint8_t* const ring = c4_smem + warp * D * C::kStep;
+    constexpr int kPieces = HD / 32;                // of a row
+    auto fetch = [&](int step, int slot) {
         const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
+        const uint32_t st = smem_u32(ring + slot * C::kStep);
         // (keys behind the last row are read as that one; nobody sees them)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const long long key = min(key0 + g + 8 * h, a.c.rows - 1);
-            load_words_once<S>(kc_base + key * (HD / 2), kc[h]);
-            load_words_once<G>(ks_base + key * (2 * G), ks[h]);
+        for (int i = 0; i < 16 * kPieces / 32; ++i) {
+            const int row = (lane + 32 * i) / kPieces, c = lane % kPieces;
+            const long long off = static_cast<long long>(min(key0 + row, a.c.rows - 1)) * (HD / 2) + c * 16;
+            c4_copy<16>(st + row * (HD / 2) + c * 16, kc_base + off);
+            c4_copy<16>(st + C::kCodes + row * (HD / 2) + (HD == 128 ? c ^ ((row >> 1) & 3) : c) * 16, vc_base + off);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const long long key = min(key0 + 2 * q + (e & 1) + 8 * (e >> 1), a.c.rows - 1);
-            load_words_once<S / 2>(vc_base + key * (HD / 2), vc[e]);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) load_words_once<G>(vs_base + min(key0 + g + 8 * h, a.c.rows - 1) * static_cast<long long>(2 * G), vs[h]);
+        c4_copy<4 * G>(st + 2 * C::kCodes + lane * 4 * G, sc_base + static_cast<long long>(min(key0 + (lane & 15), a.c.rows - 1)) * (2 * G));
     };
+    const uint8_t* const k_at = ring + g * (HD / 2) + q * 4 * S;
+    const uint8_t* const ks_at = ring + 2 * C::kCodes + g * 4 * G;
+    // V: lanes of odd q take the second key of a pair first, and put the halves together the other way round
+    const int odd_q = q & 1;
+    const uint8_t* const v_at = ring + C::kCodes + 2 * q * (HD / 2) + (HD == 128 ? ((g >> 1) ^ q) * 16 + (g & 1) * 8 : g * 4);
+    const uint32_t sel_low = odd_q ? 0x1054 : 0x5410, sel_high = odd_q ? 0x3276 : 0x7632;
 
     // Transposed accumulators: lane (g, q) has columns of V (rows of a product) in the tiles 2 s (columns 32 s + 4 g and + 2) and
     // 2 s + 1 (+ 1 and + 3, sixteen times them), for the query rows 2 q and 2 q + 1; lows, maxima and sums for its own keys.
@@ -164,18 +193,45 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         for (int i = 0; i < 2 * S; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.0f;
     }
     int v_exp = -1000;           // the steps of V count 2^-v_exp each: the largest so far is in [2^14, 2^15) then
+    float v_lift = 0.0f;         // 2^-v_exp
     const int stride = W * split;
-    int step = part * W + warp;
-    if (step < steps) fetch(step);
+    int step = part * W + warp, slot = 0;
+#pragma unroll
+    for (int i = 0; i < D - 1; ++i) {
+        if (step + i * stride < steps) fetch(step + i * stride, i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
     for (; step < steps; step += stride) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+        __syncwarp();            // all lanes' copies are there, and all lanes have read the slot that is filled next
+        if (step + (D - 1) * stride < steps) fetch(step + (D - 1) * stride, slot == 0 ? D - 1 : slot - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const int at = slot * C::kStep;
+        slot = slot + 1 == D ? 0 : slot + 1;
+        uint32_t kc[2][S], ks[2][G];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            c4_lds<S>(k_at + at + h * 8 * (HD / 2), kc[h]);
+            c4_lds<G>(ks_at + at + h * 8 * 4 * G, ks[h]);
+        }
         const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
         const int begin = step < sink_steps ? 0 : span.win_begin, end = step < sink_steps ? span.sink_end : span.win_end;
-        // scores
+        // scores: the lows' part by one product (this lane has those of group q), then the steps' of each group
         float s[NR][4];
-        float2 vstep[2][G];
         {
+            float low[2];
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.0f;
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w = ks[h][0];
+                if constexpr (G == 2) w = q == 1 ? ks[h][1] : w;
+                if constexpr (G == 4) w = q < 2 ? (q == 0 ? w : ks[h][1]) : q == 2 ? ks[h][2] : ks[h][3];
+                low[h] = q < G ? layer_pair<kBf16>(w).y : 0.0f;
+            }
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.0f;
+                mma8_tf32(s[nr], low[0], low[1], low[0], low[1], qs[nr][0], qs[nr][1]);
+            }
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
                 float d[NR][4] = {};
@@ -192,27 +248,25 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float2 p = layer_pair<kBf16>(ks[h][gi]);
-                    vstep[h][gi] = layer_pair<kBf16>(vs[h][gi]);
+                    const float st = layer_pair<kBf16>(ks[h][gi]).x;
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
-                        s[nr][2 * h] = fmaf(p.x, d[nr][2 * h], fmaf(p.y, qs[nr][gi][0], s[nr][2 * h]));
-                        s[nr][2 * h + 1] = fmaf(p.x, d[nr][2 * h + 1], fmaf(p.y, qs[nr][gi][1], s[nr][2 * h + 1]));
+                        s[nr][2 * h] = fmaf(st, d[nr][2 * h], s[nr][2 * h]);
+                        s[nr][2 * h + 1] = fmaf(st, d[nr][2 * h + 1], s[nr][2 * h + 1]);
                     }
                 }
             }
         }
-        uint32_t vw[4][S / 2];
+        uint32_t vp[2][G], vw[4][S / 2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int h = 0; h < 2; ++h) c4_lds<G>(ks_at + at + C::kScales + h * 8 * 4 * G, vp[h]);
 #pragma unroll
-            for (int i = 0; i < S / 2; ++i) vw[e][i] = vc[e][i];
-        }
-        if (step + stride < steps) fetch(step + stride);
+        for (int e = 0; e < 4; ++e) c4_lds<S / 2>(v_at + at + ((e >> 1) * 8 + ((e ^ odd_q) & 1)) * (HD / 2), vw[e]);
 
         // what is seen of the sixteen keys; all of it in most steps
         const bool whole = a.key_mask == nullptr && key0 >= begin && key0 + 16 <= end && key0 + 15 <= pos_lo &&
                            (a.window == 0 || pos_hi - key0 < a.window || key0 + 16 <= a.sinks);
+        float careful = 0.0f;            // the largest step of V of this lane's keys
         if (!whole) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -227,25 +281,31 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                         if (!seen) s[nr][2 * h + c] = -INFINITY;
                     }
                 }
-                // what hidden rows hold counts for nothing
-                if (!on) {
+                // what hidden rows hold counts for nothing (nor does a step that is not finite below, where some rows may not see it)
 #pragma unroll
-                    for (int gi = 0; gi < G; ++gi) vstep[h][gi] = make_float2(0.0f, 0.0f);
+                for (int gi = 0; gi < G; ++gi) {
+                    if (!on) vp[h][gi] = 0u;
+                    const float st = layer_pair<kBf16>(vp[h][gi]).x;
+                    careful = fmaxf(careful, st <= FLT_MAX ? st : 0.0f);
                 }
             }
+        } else {
+            // (in pairs of 16 bits, NaN left out; an infinity makes all rows NaN, since all see it)
+            uint32_t top = vp[0][0];
+#pragma unroll
+            for (int i = 1; i < 2 * G; ++i) {
+                if constexpr (kBf16) asm("max.bf16x2 %0, %0, %1;" : "+r"(top) : "r"(vp[i / G][i % G]));
+                else asm("max.f16x2 %0, %0, %1;" : "+r"(top) : "r"(vp[i / G][i % G]));
+            }
+            careful = fmaxf(0.0f, layer_pair<kBf16>(top).x);
         }
         // a new largest step of V
         {
-            float top = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int gi = 0; gi < G; ++gi) top = fmaxf(top, vstep[h][gi].x <= FLT_MAX ? vstep[h][gi].x : 0.0f);
-            }
-            const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127 - 14;
+            const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(careful)) >> 23) - 127 - 14;
             if (e > v_exp) {
                 const float f = v_exp < e - 126 ? 0.0f : pow2(v_exp - e);
                 v_exp = e;
+                v_lift = pow2(min(127, -v_exp));
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -254,15 +314,6 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                         for (int x = 0; x < 4; ++x) o[nr][i][x] *= f;
                     }
                 }
-            }
-        }
-        const float v_lift = pow2(min(127, -v_exp));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) {
-                vstep[h][gi].y = fmaf(8.0f, vstep[h][gi].x, vstep[h][gi].y);
-                vstep[h][gi].x *= v_lift;
             }
         }
 #pragma unroll
@@ -290,29 +341,35 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                     }
                 }
             }
-            float p[4];
+            float p[4], lifted[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float ref = m[nr][e & 1] == -INFINITY ? 0.0f : m[nr][e & 1];
                 p[e] = fast_exp2((s[nr][e] - ref) * sl2[nr][e & 1]);
+                lifted[e] = p[e] * v_lift;
                 l[nr][e & 1] += p[e];
             }
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
                 float w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 v = vstep[e >> 1][gi];
-                    w[e] = p[e] * v.x;
-                    float add = p[e] * v.y;
-                    if (!whole && p[e] == 0.0f) w[e] = add = 0.0f;          // (a row that this query does not see may be NaN)
-                    lo[nr][gi][e & 1] += add;
+                for (int h = 0; h < 2; ++h) {
+                    const float2 v = layer_pair<kBf16>(vp[h][gi]);
+                    const float mid = fmaf(8.0f, v.x, v.y);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int e = 2 * h + c;
+                        w[e] = lifted[e] * v.x;
+                        float add = p[e] * mid;
+                        if (!whole && p[e] == 0.0f) w[e] = add = 0.0f;          // (a row that this query does not see may be NaN)
+                        lo[nr][gi][c] += add;
+                    }
                 }
                 const uint32_t b0 = c4_transpose8(pack2<false>(w[0], w[1])), b1 = c4_transpose8(pack2<false>(w[2], w[3]));
 #pragma unroll
                 for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
                     // four columns of two keys: the halves of a word of each
-                    const uint32_t sel = (i & 1) ? 0x7632 : 0x5410;
+                    const uint32_t sel = (i & 1) ? sel_high : sel_low;
                     const uint32_t w0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), w1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
                     uint32_t u0[4], u1[4];
                     codes8(w0, u0);
@@ -343,6 +400,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     }
     const float v_down = pow2(max(-126, v_exp));
     float* const mine = o_warp + warp * kRows * C::kLd;
+    __syncthreads();
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -419,10 +477,10 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     }
 }
 
-template <int HD, int G, bool kBf16, int W, int NR, int kCtas>
+template <int HD, int G, bool kBf16, int W, int NR, int D, int kCtas>
 cudaError_t go_cache4(SdpaCache4Args a, int split, cudaStream_t stream) {
-    using C = Cache4Cfg<HD, W, NR>;
-    const auto kern = sdpa_cache4_kernel<HD, G, kBf16, W, NR, kCtas>;
+    using C = Cache4Cfg<HD, G, W, NR, D>;
+    const auto kern = sdpa_cache4_kernel<HD, G, kBf16, W, NR, D, kCtas>;
     cudaError_t e = set_max_smem_once(kern, C::kSmem);
     if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -440,7 +498,7 @@ cudaError_t pick_cache4(SdpaCache4Args a, cudaStream_t stream) {
     const long long steps = ((seen < a.c.rows ? seen : a.c.rows) + 15) / 16;
     int split = 1;
     while (split < 8 && units * split * 2 <= 3 * sm_count() && steps >= 8 * split) split *= 2;
-    return nr == 1 ? go_cache4<HD, G, kBf16, 4, 1, 3>(a, split, stream) : go_cache4<HD, G, kBf16, 4, 2, 2>(a, split, stream);
+    return nr == 1 ? go_cache4<HD, G, kBf16, 4, 1, 3, 3>(a, split, stream) : go_cache4<HD, G, kBf16, 4, 2, 3, 2>(a, split, stream);
 }
 
 }  // namespace
