@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     };
     const uint8_t* const k_at = ring + g * (HD / 2) + q * 4 * S;
     const uint8_t* const ks_at = ring + 2 * C::kCodes + g * 4 * G;
+    const uint8_t* const low_at = ks_at + (q < G ? q : 0) * 4;
     // V: lanes of odd q take the second key of a pair first, and put the halves together the other way round
     const int odd_q = q & 1;
     const uint8_t* const v_at = ring + C::kCodes + 2 * q * (HD / 2) + (HD == 128 ? ((g >> 1) ^ q) * 16 + (g & 1) * 8 : g * 4);
@@ -179,13 +180,13 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 
     // Transposed accumulators: lane (g, q) has columns of V (rows of a product) in the tiles 2 s (columns 32 s + 4 g and + 2) and
     // 2 s + 1 (+ 1 and + 3, sixteen times them), for the query rows 2 q and 2 q + 1; lows, maxima and sums for its own keys.
-    float m[NR][2], l[NR][2], o[NR][2 * S][4], lo[NR][G][2];
+    float m[NR][2], ref[NR][2], l[NR][2], o[NR][2 * S][4], lo[NR][G][2];          // (ref: the maximum, or 0 ahead of the first key that is seen)
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             m[nr][h] = -INFINITY;
-            l[nr][h] = 0.0f;
+            ref[nr][h] = l[nr][h] = 0.0f;
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] = 0.0f;
         }
@@ -222,10 +223,8 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             float low[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t w = ks[h][0];
-                if constexpr (G == 2) w = q == 1 ? ks[h][1] : w;
-                if constexpr (G == 4) w = q < 2 ? (q == 0 ? w : ks[h][1]) : q == 2 ? ks[h][2] : ks[h][3];
-                low[h] = q < G ? layer_pair<kBf16>(w).y : 0.0f;
+                const uint32_t w = G == 1 ? ks[h][0] : *reinterpret_cast<const uint32_t*>(low_at + at + h * 8 * 4 * G);
+                low[h] = G == 4 || q < G ? layer_pair<kBf16>(w).y : 0.0f;
             }
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
@@ -267,6 +266,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         const bool whole = a.key_mask == nullptr && key0 >= begin && key0 + 16 <= end && key0 + 15 <= pos_lo &&
                            (a.window == 0 || pos_hi - key0 < a.window || key0 + 16 <= a.sinks);
         float careful = 0.0f;            // the largest step of V of this lane's keys
+        bool odd = false;                // some of their pairs are not finite, and not all queries may see them
         if (!whole) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -285,10 +285,12 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
                 for (int gi = 0; gi < G; ++gi) {
                     if (!on) vp[h][gi] = 0u;
-                    const float st = layer_pair<kBf16>(vp[h][gi]).x;
-                    careful = fmaxf(careful, st <= FLT_MAX ? st : 0.0f);
+                    const float2 v = layer_pair<kBf16>(vp[h][gi]);
+                    careful = fmaxf(careful, v.x <= FLT_MAX ? v.x : 0.0f);
+                    odd = odd || !(fabsf(v.x) <= FLT_MAX && fabsf(v.y) <= FLT_MAX);
                 }
             }
+            odd = __any_sync(0xffffffffu, odd);
         } else {
             // (in pairs of 16 bits, NaN left out; an infinity makes all rows NaN, since all see it)
             uint32_t top = vp[0][0];
@@ -331,6 +333,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                     const float now = fmaxf(m[nr][h], top[h]);
                     const float alpha = now == -INFINITY ? 1.0f : fast_exp2((m[nr][h] - now) * sl2[nr][h]);
                     m[nr][h] = now;
+                    ref[nr][h] = now == -INFINITY ? 0.0f : now;
                     l[nr][h] *= alpha;
 #pragma unroll
                     for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] *= alpha;
@@ -344,8 +347,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             float p[4], lifted[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float ref = m[nr][e & 1] == -INFINITY ? 0.0f : m[nr][e & 1];
-                p[e] = fast_exp2((s[nr][e] - ref) * sl2[nr][e & 1]);
+                p[e] = fast_exp2((s[nr][e] - ref[nr][e & 1]) * sl2[nr][e & 1]);
                 lifted[e] = p[e] * v_lift;
                 l[nr][e & 1] += p[e];
             }
@@ -360,9 +362,15 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                     for (int c = 0; c < 2; ++c) {
                         const int e = 2 * h + c;
                         w[e] = lifted[e] * v.x;
-                        float add = p[e] * mid;
-                        if (!whole && p[e] == 0.0f) w[e] = add = 0.0f;          // (a row that this query does not see may be NaN)
-                        lo[nr][gi][c] += add;
+                        if (!odd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
+                    }
+                }
+                if (odd) {               // (zero times what is not finite: of a row that the query does not see)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v = layer_pair<kBf16>(vp[e >> 1][gi]);
+                        if (p[e] == 0.0f) w[e] = 0.0f;
+                        else lo[nr][gi][e & 1] = fmaf(p[e], fmaf(8.0f, v.x, v.y), lo[nr][gi][e & 1]);
                     }
                 }
                 const uint32_t b0 = c4_transpose8(pack2<false>(w[0], w[1])), b1 = c4_transpose8(pack2<false>(w[2], w[3]));
