@@ -86,6 +86,12 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     const int sink_steps = (span.sink_end + 15) / 16, win0 = span.win_begin & ~15;
     const int steps = sink_steps + (span.win_end > span.win_begin ? (span.win_end - win0 + 15) / 16 : 0);
 
+    // steps of which every query sees all sixteen keys: of the sinks' those below whole_sinks, of the window's [whole_first, whole_end)
+    const int whole_sinks = a.key_mask != nullptr ? 0 : min(span.sink_end, pos_lo + 1) / 16;
+    const int see_all = a.window == 0 || pos_hi < a.window ? 0 : pos_hi - a.window + 1;          // the first key that the last query's window has
+    const int whole_first = sink_steps + (max(see_all, span.win_begin) - win0 + 15) / 16;
+    const int whole_end = a.key_mask != nullptr ? 0 : sink_steps + (min(span.win_end, pos_lo + 1) - win0) / 16;
+
     // The queries in FP16, a power of two from where the largest of a row is in [2^14, 2^15): what that rounds is 2^-35 of
     // the largest.  This lane has row g's columns 32 s + 8 q + 0..7 as the pairs of codes8, those of the odd pairs over 16.
     uint32_t qf[NR][S][4];
@@ -194,7 +200,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         for (int i = 0; i < 2 * S; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.0f;
     }
     int v_exp = -1000;           // the steps of V count 2^-v_exp each: the largest so far is in [2^14, 2^15) then
-    float v_lift = 0.0f;         // 2^-v_exp
+    float v_lift = 0.0f, v_most = 0.0f;          // 2^-v_exp; the step from which on it is another
     const int stride = W * split;
     int step = part * W + warp, slot = 0;
 #pragma unroll
@@ -215,8 +221,6 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             c4_lds<S>(k_at + at + h * 8 * (HD / 2), kc[h]);
             c4_lds<G>(ks_at + at + h * 8 * 4 * G, ks[h]);
         }
-        const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
-        const int begin = step < sink_steps ? 0 : span.win_begin, end = step < sink_steps ? span.sink_end : span.win_end;
         // scores: the lows' part by one product (this lane has those of group q), then the steps' of each group
         float s[NR][4];
         {
@@ -228,12 +232,11 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             }
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-                s[nr][0] = s[nr][1] = s[nr][2] = s[nr][3] = 0.0f;
-                mma8_tf32(s[nr], low[0], low[1], low[0], low[1], qs[nr][0], qs[nr][1]);
+                mma8_tf32_first(s[nr], low[0], low[1], low[0], low[1], qs[nr][0], qs[nr][1]);
             }
 #pragma unroll
             for (int gi = 0; gi < G; ++gi) {
-                float d[NR][4] = {};
+                float d[NR][4];
 #pragma unroll
                 for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
                     uint32_t u[2][4];
@@ -241,7 +244,8 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                     codes8(kc[1][i], u[1]);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
-                        mma16<false>(d[nr], u[0][0], u[1][0], u[0][2], u[1][2], qf[nr][i][0], qf[nr][i][2]);
+                        if (i == gi * kPer) mma16_first<false>(d[nr], u[0][0], u[1][0], u[0][2], u[1][2], qf[nr][i][0], qf[nr][i][2]);
+                        else mma16<false>(d[nr], u[0][0], u[1][0], u[0][2], u[1][2], qf[nr][i][0], qf[nr][i][2]);
                         mma16<false>(d[nr], u[0][1], u[1][1], u[0][3], u[1][3], qf[nr][i][1], qf[nr][i][3]);
                     }
                 }
@@ -263,11 +267,12 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         for (int e = 0; e < 4; ++e) c4_lds<S / 2>(v_at + at + ((e >> 1) * 8 + ((e ^ odd_q) & 1)) * (HD / 2), vw[e]);
 
         // what is seen of the sixteen keys; all of it in most steps
-        const bool whole = a.key_mask == nullptr && key0 >= begin && key0 + 16 <= end && key0 + 15 <= pos_lo &&
-                           (a.window == 0 || pos_hi - key0 < a.window || key0 + 16 <= a.sinks);
+        const bool whole = step < whole_sinks || (step >= whole_first && step < whole_end);
         float careful = 0.0f;            // the largest step of V of this lane's keys
         bool odd = false;                // some of their pairs are not finite, and not all queries may see them
         if (!whole) {
+            const int begin = step < sink_steps ? 0 : span.win_begin, end = step < sink_steps ? span.sink_end : span.win_end;
+            const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int key = key0 + g + 8 * h;
@@ -301,20 +306,19 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             }
             careful = fmaxf(0.0f, layer_pair<kBf16>(top).x);
         }
-        // a new largest step of V
-        {
+        // a new largest step of V is rare after the first keys
+        if (__any_sync(0xffffffffu, careful >= v_most)) {
             const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(careful)) >> 23) - 127 - 14;
-            if (e > v_exp) {
-                const float f = v_exp < e - 126 ? 0.0f : pow2(v_exp - e);
-                v_exp = e;
-                v_lift = pow2(min(127, -v_exp));
+            const float f = v_exp < e - 126 ? 0.0f : pow2(v_exp - e);
+            v_exp = e;
+            v_lift = pow2(min(127, -v_exp));
+            v_most = e < 112 ? pow2(max(-126, e + 15)) : INFINITY;
 #pragma unroll
-                for (int nr = 0; nr < NR; ++nr) {
+            for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
-                    for (int i = 0; i < 2 * S; ++i) {
+                for (int i = 0; i < 2 * S; ++i) {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) o[nr][i][x] *= f;
-                    }
+                    for (int x = 0; x < 4; ++x) o[nr][i][x] *= f;
                 }
             }
         }
