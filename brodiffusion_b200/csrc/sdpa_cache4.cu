@@ -60,7 +60,8 @@ __device__ __forceinline__ void c4_lds(const uint8_t* p, uint32_t (&w)[kWords]) 
 }
 
 // HD: 64 or 128.  G: groups of a row.  W: warps.  NR: query rows in eights.  D: steps of a warp in shared memory.  kCtas: CTAs of an SM.
-template <int HD, int G, bool kBf16, int W, int NR, int D, int kCtas>
+// kMask: with a key mask (without one, looking for it took 3 % of a call).
+template <int HD, int G, bool kBf16, bool kMask, int W, int NR, int D, int kCtas>
 __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid_constant__ SdpaCache4Args a) {
     using C = Cache4Cfg<HD, G, W, NR, D>;
     constexpr int S = HD / 32, kPer = S / G, kRows = C::kRows;
@@ -86,11 +87,11 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     const int sink_steps = (span.sink_end + 15) / 16, win0 = span.win_begin & ~15;
     const int steps = sink_steps + (span.win_end > span.win_begin ? (span.win_end - win0 + 15) / 16 : 0);
 
-    // steps of which every query sees all sixteen keys: of the sinks' those below whole_sinks, of the window's [whole_first, whole_end)
-    const int whole_sinks = a.key_mask != nullptr ? 0 : min(span.sink_end, pos_lo + 1) / 16;
+    // steps of which every query sees all sixteen keys, but for the key mask: of the sinks' those below whole_sinks, of the window's [whole_first, whole_end)
+    const int whole_sinks = min(span.sink_end, pos_lo + 1) / 16;
     const int see_all = a.window == 0 || pos_hi < a.window ? 0 : pos_hi - a.window + 1;          // the first key that the last query's window has
     const int whole_first = sink_steps + (max(see_all, span.win_begin) - win0 + 15) / 16;
-    const int whole_end = a.key_mask != nullptr ? 0 : sink_steps + (min(span.win_end, pos_lo + 1) - win0) / 16;
+    const int whole_end = sink_steps + (min(span.win_end, pos_lo + 1) - win0) / 16;
 
     // The queries in FP16, a power of two from where the largest of a row is in [2^14, 2^15): what that rounds is 2^-35 of
     // the largest.  This lane has row g's columns 32 s + 8 q + 0..7 as the pairs of codes8, those of the odd pairs over 16.
@@ -215,6 +216,9 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         asm volatile("cp.async.commit_group;" ::: "memory");
         const int at = slot * C::kStep;
         slot = slot + 1 == D ? 0 : slot + 1;
+        const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
+        float mask = 1.0f;
+        if (kMask) mask = load_scale(a.key_mask + min(key0 + (lane & 15), a.c.rows - 1));
         uint32_t kc[2][S], ks[2][G];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -267,17 +271,16 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         for (int e = 0; e < 4; ++e) c4_lds<S / 2>(v_at + at + ((e >> 1) * 8 + ((e ^ odd_q) & 1)) * (HD / 2), vw[e]);
 
         // what is seen of the sixteen keys; all of it in most steps
-        const bool whole = step < whole_sinks || (step >= whole_first && step < whole_end);
+        const uint32_t live = kMask ? __ballot_sync(0xffffffffu, mask != 0.0f) : 0xffffffffu;      // the sixteen twice
+        const bool whole = (step < whole_sinks || (step >= whole_first && step < whole_end)) && live == 0xffffffffu;
         float careful = 0.0f;            // the largest step of V of this lane's keys
         bool odd = false;                // some of their pairs are not finite, and not all queries may see them
         if (!whole) {
             const int begin = step < sink_steps ? 0 : span.win_begin, end = step < sink_steps ? span.sink_end : span.win_end;
-            const int key0 = step < sink_steps ? step * 16 : win0 + (step - sink_steps) * 16;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int key = key0 + g + 8 * h;
-                bool on = key >= begin && key < end;
-                if (on && a.key_mask != nullptr) on = load_scale(a.key_mask + key) != 0.0f;
+                const bool on = key >= begin && key < end && ((live >> (g + 8 * h)) & 1u) != 0;
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 template <int HD, int G, bool kBf16, int W, int NR, int D, int kCtas>
 cudaError_t go_cache4(SdpaCache4Args a, int split, cudaStream_t stream) {
     using C = Cache4Cfg<HD, G, W, NR, D>;
-    const auto kern = sdpa_cache4_kernel<HD, G, kBf16, W, NR, D, kCtas>;
+    const auto kern = a.key_mask != nullptr ? sdpa_cache4_kernel<HD, G, kBf16, true, W, NR, D, kCtas> : sdpa_cache4_kernel<HD, G, kBf16, false, W, NR, D, kCtas>;
     cudaError_t e = set_max_smem_once(kern, C::kSmem);
     if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -503,14 +506,30 @@ cudaError_t go_cache4(SdpaCache4Args a, int split, cudaStream_t stream) {
 
 template <int HD, int G, bool kBf16>
 cudaError_t pick_cache4(SdpaCache4Args a, cudaStream_t stream) {
-    const int nr = a.lq * static_cast<long long>(a.kv_group) <= 8 ? 1 : 2;
-    a.row_tiles = static_cast<int>((static_cast<long long>(a.lq) * a.kv_group + 8 * nr - 1) / (8 * nr));
+    const long long rows = static_cast<long long>(a.lq) * a.kv_group;
+    const int nr = rows <= 8 ? 1 : 2, sms = sm_count();
+    a.row_tiles = static_cast<int>((rows + 8 * nr - 1) / (8 * nr));
     const long long units = static_cast<long long>(a.batch) * a.c.kv_heads * a.row_tiles;
+    // sixteens of keys that there are for the longest sequence
     const long long seen = a.window > 0 ? static_cast<long long>(a.window) + a.sinks + a.lq - 1 : a.c.rows;
     const long long steps = ((seen < a.c.rows ? seen : a.c.rows) + 15) / 16;
-    int split = 1;
-    while (split < 8 && units * split * 2 <= 3 * sm_count() && steps >= 8 * split) split *= 2;
-    return nr == 1 ? go_cache4<HD, G, kBf16, 4, 1, 3, 3>(a, split, stream) : go_cache4<HD, G, kBf16, 4, 2, 3, 2>(a, split, stream);
+    auto least = [](long long x, long long y) { return static_cast<int>(x < y ? x : y); };
+    // Few heads over long caches: eight warps to a CTA, two CTAs to an SM and the keys of a head over all CTAs there is room for, with two steps
+    // to a warp (8 heads over 32768 keys: sixteen CTAs 27.4 us, eight 33.5, sixteen of four warps 34.2; 32 heads over 4000 keys: eight CTAs 9.6,
+    // sixteen of four warps 11.3).
+    if (nr == 1 && units * 8 <= 2 * sms && steps >= 128) {
+        const int split = least(least(kC4MaxSplit, 2 * sms / units), steps / 16);
+        return go_cache4<HD, G, kBf16, 8, 1, 3, 2>(a, split < 1 ? 1 : split, stream);
+    }
+    // Else four warps, and three and a half rounds of CTAs, so that the last one costs little (256 heads over up to 32768 keys: over six CTAs
+    // 238 us, over eight 249, over four 254, over two 290), but one step to a warp at least (8 heads over 777 keys: over eight 4.1, over
+    // sixteen 4.4, over six 4.7).
+    constexpr int kOne = HD == 64 || G == 1 ? 4 : 3, kTwo = HD == 64 ? 4 : 2;           // CTAs of an SM: what registers allow
+    const int slots = sms * (nr == 1 ? kOne : kTwo);
+    int split = nr == 2 && units >= slots ? 1 : least(8, (7ll * slots / 2 + units - 1) / units);       // (509 x 2 rows, 16 heads of 64: whole 134, over two 144)
+    split = least(split, (steps + 3) / 4);
+    if (split < 1) split = 1;
+    return nr == 1 ? go_cache4<HD, G, kBf16, 4, 1, 3, kOne>(a, split, stream) : go_cache4<HD, G, kBf16, 4, 2, 3, kTwo>(a, split, stream);
 }
 
 }  // namespace
