@@ -118,9 +118,19 @@ __device__ __forceinline__ void norm_gains(const void* gain, int is_f32, int c, 
     if (gain == nullptr) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = 1.0f;
-    } else if (is_f32) {
+    } else if (is_f32 && kShift) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = !kShift || (c + i >= 0 && c + i < cols) ? reinterpret_cast<const float*>(gain)[c + i] : 0.0f;
+        for (int i = 0; i < 8; ++i) g[i] = c + i >= 0 && c + i < cols ? reinterpret_cast<const float*>(gain)[c + i] : 0.0f;
+    } else if (is_f32) {
+        // (two loads: eight of them, predicated off for gains of 16 bits, are instructions all the same)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(gain) + c + i);
+            g[i] = v.x;
+            g[i + 1] = v.y;
+            g[i + 2] = v.z;
+            g[i + 3] = v.w;
+        }
     } else if (kShift) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = c + i >= 0 && c + i < cols ? layer_ld16<kBf16>(gain, c + i) : 0.0f;

@@ -13,93 +13,163 @@
 namespace bdattn {
 namespace {
 
-// NaN where a row's sum of squares is not finite (its root would make zeros of finite values).
+// NaN where a row's sum of squares is not finite (its root would make zeros of finite values); a row of zeros stays one with an
+// eps of 0 too.
 __device__ __forceinline__ float sandwich_root(float ss, const SandwichNormArgs& a) {
-    return ss <= FLT_MAX ? rsqrtf(ss / static_cast<float>(a.cols) + a.eps) : __uint_as_float(0x7fffffffu);
+    const float v = ss / static_cast<float>(a.cols) + a.eps;
+    return !(ss <= FLT_MAX) ? __uint_as_float(0x7fffffffu) : v > 0.0f ? rsqrtf(v) : 0.0f;
+}
+
+// Two FP32 values to an instruction: the kernel is short of issue slots (16384 x 5120 131 us without).
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+    asm("{.reg .b64 x, y; mov.b64 x, {%0, %1}; mov.b64 y, {%2, %3}; mul.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}" : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+// c += a * b
+__device__ __forceinline__ void fma2(float& c0, float& c1, float a0, float a1, float b0, float b1) {
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%0, %1}; fma.rn.f32x2 z, x, y, z; mov.b64 {%0, %1}, z;}"
+        : "+f"(c0), "+f"(c1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+// Sum, and maximum where it is wanted, over the CTA (at most 32 warps); red: 64 floats, 16-byte aligned.
+template <bool kMax>
+__device__ __forceinline__ void sandwich_meet(float& s, float& m, float* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (kMax) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    }
+    const int warps = static_cast<int>(blockDim.x) >> 5;
+    if (warps == 1) return;
+    if ((threadIdx.x & 31) == 0) {
+        red[threadIdx.x >> 5] = s;
+        if (kMax) red[32 + (threadIdx.x >> 5)] = m;
+    }
+    __syncthreads();
+    s = 0.0f;
+    for (int w = 0; w < warps; w += 4) {          // the same order in every thread
+        const float4 v = *reinterpret_cast<const float4*>(red + w);
+        s += v.x;
+        if (w + 1 < warps) s += v.y;
+        if (w + 2 < warps) s += v.z;
+        if (w + 3 < warps) s += v.w;
+        if (kMax) {
+            const float4 t = *reinterpret_cast<const float4*>(red + 32 + w);
+            m = fmaxf(m, t.x);
+            if (w + 1 < warps) m = fmaxf(m, t.y);
+            if (w + 2 < warps) m = fmaxf(m, t.z);
+            if (w + 3 < warps) m = fmaxf(m, t.w);
+        }
+    }
 }
 
 // As add_rmsnorm_kernel: a row to a team of kTeam lanes or, with kTeam = 0, to a CTA, kV pieces of eight values to a thread, in
 // registers between the one read and the one write; the next row is on its way while this one is reduced.
-template <bool kBf16, int kV, int kTeam, bool kShift>
-__global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) sandwich_norm_kernel(const __grid_constant__ SandwichNormArgs a) {
-    __shared__ float red[2][64];
+template <bool kBf16, bool kFp8, int kV, int kTeam, bool kShift>
+__global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512, kTeam > 0 ? 1 : kV == 2 ? 2 : 1) sandwich_norm_kernel(const __grid_constant__ SandwichNormArgs a) {
+    __shared__ __align__(16) float red[2][64];
     constexpr int kSide = kTeam > 0 ? 128 / (kTeam > 0 ? kTeam : 1) : 1;       // rows side by side
     const int team = kTeam > 0 ? kTeam : static_cast<int>(blockDim.x);
     const int me = kTeam > 0 ? static_cast<int>(threadIdx.x) & (kTeam - 1) : static_cast<int>(threadIdx.x);
     if (a.one_wave) dependents_may_launch();
     wait_for_prior_grid();
-    auto shift_of = [&](long long row) { return kShift ? static_cast<int>((a.shift + row * a.ldx) & 7) : 0; };
-    auto fetch = [&](const void* base, long long ld, long long row, uint4 (&v)[kV]) {
-        const uint16_t* const at = reinterpret_cast<const uint16_t*>(base) + row * ld;
+    // (rows and their step are below 2^31 and 2^24)
+    const uint32_t rows = static_cast<uint32_t>(a.rows), step = gridDim.x * kSide;
+    uint32_t row = blockIdx.x * kSide + (kTeam > 0 ? threadIdx.x / (kTeam > 0 ? kTeam : 1) : 0);
+    auto shift_of = [&](uint32_t row) { return kShift ? static_cast<int>((a.shift + row * static_cast<uint32_t>(a.ldx)) & 7) : 0; };
+    auto fetch = [&](const uint16_t* at, uint32_t row, uint4 (&v)[kV]) {
         const int s = shift_of(row);
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
             const int c = (me + i * team) * 8 - s;
             v[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (row < a.rows && c < a.cols) v[i] = norm_load<kShift>(at, c, a.cols);
+            if (row < rows && c < a.cols) v[i] = norm_load<kShift>(at, c, a.cols);
         }
     };
-    auto reduce = [&](float& ss, float& top, float* const where) {
+    auto reduce = [&](auto max, float& ss, float& top, float* const where) {
+        constexpr bool kMax = decltype(max)::value;
         if constexpr (kTeam > 0) {
 #pragma unroll
             for (int o = kTeam / 2; o > 0; o >>= 1) {
                 ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (kMax) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             }
         } else {
-            block_sum_max(ss, top, where);
+            sandwich_meet<kMax>(ss, top, where);
         }
     };
     uint4 x[kV], r[kV];
-    const long long step = static_cast<long long>(gridDim.x) * kSide;
-    long long row = static_cast<long long>(blockIdx.x) * kSide + (kTeam > 0 ? threadIdx.x / (kTeam > 0 ? kTeam : 1) : 0);
-    fetch(a.x, a.ldx, row, x);
-    fetch(a.residual, a.ldr, row, r);
+    // rows by pointers that go on by the same number of bytes
+    const uint16_t* xr = reinterpret_cast<const uint16_t*>(a.x) + row * a.ldx;
+    const uint16_t* rr = reinterpret_cast<const uint16_t*>(a.residual) + row * a.ldr;
+    uint16_t* ror = reinterpret_cast<uint16_t*>(a.residual_out) + row * a.ldro;
+    uint8_t* outr = reinterpret_cast<uint8_t*>(a.out) + row * a.ldo * (kFp8 ? 1 : 2);
+    fetch(xr, row, x);
+    fetch(rr, row, r);
     // (all rows of a CTA's turn together: the teams of a warp meet in its shuffles)
-    for (long long base = static_cast<long long>(blockIdx.x) * kSide; base < a.rows; base += step, row += step) {
-        const bool exists = kTeam == 0 || row < a.rows;
+    for (uint32_t base = blockIdx.x * kSide; base < rows; base += step) {
+        const bool exists = kTeam == 0 || row < rows;
         const int s = shift_of(row);
         const uint16_t* const gate = a.gate == nullptr ? nullptr
-            : reinterpret_cast<const uint16_t*>(a.gate) +
-              static_cast<int>(min(row, static_cast<long long>(a.rows) - 1)) / a.gate_rows * a.ldg;
+            : reinterpret_cast<const uint16_t*>(a.gate) + min(row, rows - 1) / static_cast<uint32_t>(a.gate_rows) * a.ldg;
         float y[kV][8];
-        float ss = 0.0f, top = 0.0f;
+        float ss = 0.0f, ss1 = 0.0f, top = 0.0f;
+        // x times what stands behind its norm, while its squares are added up
 #pragma unroll
         for (int v = 0; v < kV; ++v) {
+            const int c = (me + v * team) * 8 - s;
             norm_wide<kBf16>(x[v], y[v]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(y[v][i], y[v][i], ss);
+            for (int i = 0; i < 8; i += 2) fma2(ss, ss1, y[v][i], y[v][i + 1], y[v][i], y[v][i + 1]);
+            if (exists && c < a.cols) {
+                float t[8];
+                if (a.post_gain != nullptr) {
+                    norm_gains<kBf16, kShift>(a.post_gain, a.gain_is_f32, c, a.cols, t);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) mul2(y[v][i], y[v][i + 1], t[i], t[i + 1]);
+                }
+                if (gate != nullptr) {
+                    norm_gains<kBf16, kShift>(gate, 0, c, a.cols, t);
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) mul2(y[v][i], y[v][i + 1], t[i], t[i + 1]);
+                }
+            }
         }
-        fetch(a.x, a.ldx, row + step, x);
-        reduce(ss, top, red[0]);
+        ss += ss1;
+        xr += step * a.ldx;
+        fetch(xr, row + step, x);
+        reduce(std::false_type{}, ss, top, red[0]);
         const float inv_x = sandwich_root(ss, a);
-        ss = top = 0.0f;
+        ss = ss1 = top = 0.0f;
 #pragma unroll
         for (int v = 0; v < kV; ++v) {
             const int c = (me + v * team) * 8 - s;
             if (exists && c < a.cols) {
                 float t[8];
-                norm_gains<kBf16, kShift>(a.post_gain, a.gain_is_f32, c, a.cols, t);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[v][i] *= inv_x * t[i];
-                if (gate != nullptr) {
-                    norm_gains<kBf16, kShift>(gate, 0, c, a.cols, t);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[v][i] *= t[i];
-                }
                 norm_wide<kBf16>(r[v], t);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[v][i] = fmaf(a.residual_scale, t[i], y[v][i]);
-                    // (a piece's places off the row have values of the vectors, not of the row)
-                    if (kShift && (c + i < 0 || c + i >= a.cols)) y[v][i] = 0.0f;
-                    ss = fmaf(y[v][i], y[v][i], ss);
+                for (int i = 0; i < 8; i += 2) {
+                    mul2(t[i], t[i + 1], a.residual_scale, a.residual_scale);
+                    fma2(t[i], t[i + 1], y[v][i], y[v][i + 1], inv_x, inv_x);
+                    y[v][i] = t[i];
+                    y[v][i + 1] = t[i + 1];
+                    if (kShift) {
+                        // (a piece's places off the row are not the row's, whatever the root is)
+                        if (c + i < 0 || c + i >= a.cols) y[v][i] = 0.0f;
+                        if (c + i + 1 < 0 || c + i + 1 >= a.cols) y[v][i + 1] = 0.0f;
+                    }
+                    fma2(ss, ss1, y[v][i], y[v][i + 1], y[v][i], y[v][i + 1]);
                 }
-                norm_store<kBf16, kShift>(reinterpret_cast<uint16_t*>(a.residual_out) + row * a.ldro, c, a.cols, y[v]);
+                norm_store<kBf16, kShift>(ror, c, a.cols, y[v]);
             }
         }
-        const long long now = row;
-        fetch(a.residual, a.ldr, row + step, r);
+        ss += ss1;
+        const uint32_t now = row;
+        row += step;
+        rr += step * a.ldr;
+        ror += step * a.ldro;
+        uint8_t* const out = outr;
+        outr += step * a.ldo * (kFp8 ? 1 : 2);
+        fetch(rr, row, r);
         if (a.out == nullptr) {
             if (kTeam == 0) __syncthreads();       // (the next row's sums go where this one's were read)
             continue;
@@ -108,18 +178,21 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) sandwi
         for (int v = 0; v < kV; ++v) {
             const int c = (me + v * team) * 8 - s;
             if (exists && c < a.cols) {
-                float g[8];
-                norm_gains<kBf16, kShift>(a.gain, a.gain_is_f32, c, a.cols, g);
+                if (a.gain != nullptr) {
+                    float g[8];
+                    norm_gains<kBf16, kShift>(a.gain, a.gain_is_f32, c, a.cols, g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[v][i] *= g[i];
-                    top = fmaxf(top, fabsf(y[v][i]));
+                    for (int i = 0; i < 8; i += 2) mul2(y[v][i], y[v][i + 1], g[i], g[i + 1]);
+                }
+                if (kFp8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(y[v][i]));
                 }
             }
         }
-        reduce(ss, top, red[1]);
+        reduce(std::integral_constant<bool, kFp8>{}, ss, top, red[1]);
         float inv = sandwich_root(ss, a);
-        if (a.out_scale != nullptr) {
+        if constexpr (kFp8) {
             const RowScale rs = row_scale(ss, top, inv);
             if (exists && me == 0) a.out_scale[now] = rs.scale;
             inv = rs.factor;
@@ -136,9 +209,9 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512) sandwi
             const int c = (me + v * team) * 8 - s;
             if (exists && c < a.cols) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[v][i] *= inv;
-                if (a.out_scale != nullptr) norm_store_e4m3<kShift>(reinterpret_cast<uint8_t*>(a.out) + now * a.ldo, c, a.cols, y[v]);
-                else norm_store<kBf16, kShift>(reinterpret_cast<uint16_t*>(a.out) + now * a.ldo, c, a.cols, y[v]);
+                for (int i = 0; i < 8; i += 2) mul2(y[v][i], y[v][i + 1], inv, inv);
+                if constexpr (kFp8) norm_store_e4m3<kShift>(out, c, a.cols, y[v]);
+                else norm_store<kBf16, kShift>(out, c, a.cols, y[v]);
             }
         }
     }
@@ -187,7 +260,7 @@ __global__ void __launch_bounds__(1024) sandwich_norm_any_kernel(const __grid_co
     }
 }
 
-template <bool kBf16>
+template <bool kBf16, bool kFp8>
 cudaError_t launch_sandwich(SandwichNormArgs a, cudaStream_t stream) {
     // Elements that a tensor's rows lie off their vectors of eight: the same for all of them, as in launch_norm.
     auto off = [](const void* p, int bytes) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) / bytes % 8); };
@@ -211,13 +284,16 @@ cudaError_t launch_sandwich(SandwichNormArgs a, cudaStream_t stream) {
         constexpr bool kS = decltype(shift)::value;
         const int pieces = kS ? (a.cols + 14) / 8 : a.cols / 8;
         auto threads = [&](int v) { return ((pieces + v - 1) / v + 31) / 32 * 32; };
-        if (pieces <= 8) return go(sandwich_norm_kernel<kBf16, 1, 8, kS>, 16, 128);
-        if (pieces <= 32) return go(sandwich_norm_kernel<kBf16, 1, 32, kS>, 4, 128);
-        if (a.rows <= sm_count() && pieces <= 1024) return go(sandwich_norm_kernel<kBf16, 1, 0, kS>, 1, threads(1));
-        if (pieces <= 64) return go(sandwich_norm_kernel<kBf16, 2, 32, kS>, 4, 128);
-        if (pieces <= 128) return go(sandwich_norm_kernel<kBf16, 4, 32, kS>, 4, 128);
-        if (pieces <= 512) return go(sandwich_norm_kernel<kBf16, 2, 0, kS>, 1, threads(2));
-        return go(sandwich_norm_kernel<kBf16, 4, 0, kS>, 1, threads(4));
+        if (pieces <= 8) return go(sandwich_norm_kernel<kBf16, kFp8, 1, 8, kS>, 16, 128);
+        if (pieces <= 32) return go(sandwich_norm_kernel<kBf16, kFp8, 1, 32, kS>, 4, 128);
+        // Few rows: a piece to a thread, the shortest chain.  More: two to a thread in 64 registers, which are twice as many warps as the
+        // compiler would leave (16384 x 5120, 8-bit output, 157 us without the bound, 149 with it, 275 with one piece; 4332 x 2240 27.9, 21.5,
+        // 24.5; both ahead of the arithmetic in pairs).
+        if (a.rows <= sm_count() && pieces <= 1024) return go(sandwich_norm_kernel<kBf16, kFp8, 1, 0, kS>, 1, threads(1));
+        if (pieces <= 64) return go(sandwich_norm_kernel<kBf16, kFp8, 2, 32, kS>, 4, 128);
+        if (pieces <= 128) return go(sandwich_norm_kernel<kBf16, kFp8, 4, 32, kS>, 4, 128);
+        if (pieces <= 1024) return go(sandwich_norm_kernel<kBf16, kFp8, 2, 0, kS>, 1, threads(2));
+        return go(sandwich_norm_kernel<kBf16, kFp8, 4, 0, kS>, 1, threads(4));
     };
     if (same && a.cols <= 16384 - 14) return zero ? pick(std::false_type{}) : pick(std::true_type{});
     const int threads = a.cols < 1024 ? (a.cols + 31) / 32 * 32 : 1024;
@@ -227,7 +303,8 @@ cudaError_t launch_sandwich(SandwichNormArgs a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_sandwich_norm(const SandwichNormArgs& a, bool bf16, cudaStream_t stream) {
-    return bf16 ? launch_sandwich<true>(a, stream) : launch_sandwich<false>(a, stream);
+    if (a.out_scale != nullptr) return bf16 ? launch_sandwich<true, true>(a, stream) : launch_sandwich<false, true>(a, stream);
+    return bf16 ? launch_sandwich<true, false>(a, stream) : launch_sandwich<false, false>(a, stream);
 }
 
 }  // namespace bdattn

@@ -170,6 +170,16 @@ def test_epsilon_and_magnitudes(bd, eps, size):
         check(call(bd, x, r, eps=eps, out_dtype=out), x, r, eps=eps)
 
 
+def test_rows_of_zeros_without_an_epsilon(bd):
+    x, r = randn(1, 3, 640), randn(2, 3, 640)
+    x[1], x[2], r[2] = 0, 0, 0
+    for cols in (640, 333):
+        h, out, _ = call(bd, x[:, :cols], r[:, :cols], eps=0.0, out_dtype=torch.bfloat16)
+        assert (h[1] == r[1, :cols]).all() and (h[2] == 0).all() and (out[2] == 0).all() and torch.isfinite(out).all()
+        h, q, scale = call(bd, x[:, :cols], r[:, :cols], eps=0.0, out_dtype=E4M3)
+        assert scale[2] == 0 and (q[2].float() == 0).all() and torch.isfinite(scale).all()
+
+
 def test_no_rows_streams_and_repeats(bd):
     x = torch.empty(0, 64, device="cuda", dtype=torch.bfloat16)
     bd.sandwich_norm_fwd(x, torch.empty_like(x), torch.empty_like(x), out=torch.empty_like(x))
