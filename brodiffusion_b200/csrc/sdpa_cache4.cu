@@ -325,6 +325,19 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                 }
             }
         }
+        // the power of two goes to the steps or to the weights, whichever are fewer
+        constexpr bool kLiftSteps = 2 * G < 4 * NR;
+        float lifted_step[2][G];
+        if (kLiftSteps) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int gi = 0; gi < G; ++gi) lifted_step[h][gi] = layer_pair<kBf16>(vp[h][gi]).x * v_lift;
+            }
+        }
+        // (code of its own where pairs are not finite: as branches of one, its instructions are issued all the same)
+        auto weigh = [&](auto is_odd) {
+            constexpr bool kOdd = decltype(is_odd)::value;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
             float top[2] = {fmaxf(s[nr][0], s[nr][2]), fmaxf(s[nr][1], s[nr][3])};
@@ -355,7 +368,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 p[e] = fast_exp2((s[nr][e] - ref[nr][e & 1]) * sl2[nr][e & 1]);
-                lifted[e] = p[e] * v_lift;
+                if (!kLiftSteps) lifted[e] = p[e] * v_lift;
                 l[nr][e & 1] += p[e];
             }
 #pragma unroll
@@ -368,11 +381,11 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int e = 2 * h + c;
-                        w[e] = lifted[e] * v.x;
-                        if (!odd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
+                        w[e] = kLiftSteps ? p[e] * lifted_step[h][gi] : lifted[e] * v.x;
+                        if (!kOdd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
                     }
                 }
-                if (odd) {               // (zero times what is not finite: of a row that the query does not see)
+                if (kOdd) {              // (zero times what is not finite: of a row that the query does not see)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float2 v = layer_pair<kBf16>(vp[e >> 1][gi]);
@@ -399,6 +412,9 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                 }
             }
         }
+        };
+        if (odd) weigh(std::true_type{});
+        else weigh(std::false_type{});
     }
     // the warps' sums, whole: over the lanes' keys, the lows and the powers of two put in
 #pragma unroll
