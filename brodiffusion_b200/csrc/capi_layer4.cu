@@ -155,7 +155,7 @@ int bdattn_w4_pack(const void* codes, long long codes_ld, const void* scales, lo
     const char* op = "bdattn_w4_pack";
     if (require_sm100(op)) return -1;
     if (!is_group(group)) return fail("%s: group must be 32, 64 or 128 (got %d)", op, group);
-    if (N < 1 || K < 1 || K % 8 != 0) return fail("%s: N must be >= 1 and K a multiple of 8 (got %d and %d)", op, N, K);
+    if (N < 1 || K < 1 || K % 8 != 0 || K > (1 << 30)) return fail("%s: N must be >= 1 and K a multiple of 8 up to 2^30 (got %d and %d)", op, N, K);
     if (codes == nullptr || scales == nullptr || packed == nullptr) return fail("%s: codes/scales/packed is null", op);
     bdattn::W4PackArgs a;
     const long long groups = (static_cast<long long>(K) + group - 1) / group;
@@ -183,7 +183,8 @@ int bdattn_linear_w4_fwd(const bdattn_linear_w4_params* p, bdattn_stream_t strea
     if (p->act < BDATTN_ACT_NONE || p->act > BDATTN_ACT_SILU) return fail("%s: unknown activation %d", op, p->act);
     if (p->M < 0 || p->N < 1 || p->K < 1 || p->K % 8 != 0)
         return fail("%s: M must be >= 0, N >= 1 and K a multiple of 8 (got %d, %d, %d)", op, p->M, p->N, p->K);
-    if (p->M > 8 * 65535) return fail("%s: more than 524280 rows (got %d)", op, p->M);
+    // (a tile's columns go on past the last one; eight rows are a pass in the grid's second dimension)
+    if (p->K > (1 << 30) || p->M > 8 * 65535) return fail("%s: more than 2^30 columns or 524280 rows (got %d and %d)", op, p->K, p->M);
     if (p->M == 0) return 0;
     if (p->x == nullptr || p->w == nullptr || p->y == nullptr) return fail("%s: x/w/y is null", op);
     bdattn::GemmProblem g;

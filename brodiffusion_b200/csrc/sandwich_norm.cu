@@ -5,7 +5,7 @@
 //   out = y rounded, or  a = max|y| / 448,  out = e4m3(y / a),  out_scale = a, or nothing
 // x and residual are read once, both sums of squares are of unrounded values.  Bound by memory from a few hundred
 // rows on (6 bytes an element for the stream and 1 or 2 for the output), by two meetings of a row's threads below: the second
-// sum needs the first one's root.
+// sum needs the first one's root.  16384 x 5120 to 8 bits 104.5 us (5.6 TB/s), 4332 x 2240 in 16 bits 17.9 (4.3 TB/s), one row 2.4.
 #include <type_traits>
 
 #include "norm_rows.cuh"
@@ -288,7 +288,7 @@ cudaError_t launch_sandwich(SandwichNormArgs a, cudaStream_t stream) {
         if (pieces <= 32) return go(sandwich_norm_kernel<kBf16, kFp8, 1, 32, kS>, 4, 128);
         // Few rows: a piece to a thread, the shortest chain.  More: two to a thread in 64 registers, which are twice as many warps as the
         // compiler would leave (16384 x 5120, 8-bit output, 157 us without the bound, 149 with it, 275 with one piece; 4332 x 2240 27.9, 21.5,
-        // 24.5; both ahead of the arithmetic in pairs).
+        // 24.5; all with single FP32 values to an instruction, with pairs of them 104.5 and 17.9).
         if (a.rows <= sm_count() && pieces <= 1024) return go(sandwich_norm_kernel<kBf16, kFp8, 1, 0, kS>, 1, threads(1));
         if (pieces <= 64) return go(sandwich_norm_kernel<kBf16, kFp8, 2, 32, kS>, 4, 128);
         if (pieces <= 128) return go(sandwich_norm_kernel<kBf16, kFp8, 4, 32, kS>, 4, 128);

@@ -2,15 +2,19 @@
 //   s_ij = scale * sum_g step_K[j, g] (sum_{c in g} q_ic u_jc) + low_K[j, g] (sum_{c in g} q_ic)
 //   o_i  = (sum_j p_ij step_V[j, g] (u_j - 8) + sum_j p_ij (low_V[j, g] + 8 step_V[j, g])) / sum_j p_ij,   p_ij = exp(s_ij - max)
 // (with u as it is, both sums would be some ten times the output of many keys, and the roundings of the first in proportion: fp16
-// outputs of 8000 keys were off by 5.3e-4, with u - 8 by 2.4e-4, of which 2.1e-4 are the outputs' own).
+// outputs of 8000 keys were off by 5.3e-4, with u - 8 by 2.8e-4, of which 2.1e-4 are the outputs' own).
 // The codes enter mma.sync as exact FP16 integers (four_bit.cuh); steps and lows are applied to FP32 scores and to the
-// FP32 weights ahead of their one rounding, to FP16.  What a call costs is reading the visible rows once, 4 + 32 / group bits
-// a value: the query heads that share a K/V head, and the new tokens, are the (eight or sixteen) columns of a product whose rows are
-// sixteen keys, or sixteen columns of V.  A warp takes sixteen keys at a time, straight from memory to registers, with the next
-// sixteen on their way, and has a running maximum, sum and accumulator of its own; these meet in shared memory, then in
-// distributed shared memory, where every CTA of a head's cluster finishes its share of the rows.
+// FP32 weights ahead of their one rounding, to FP16.  The query heads that share a K/V head, and the new tokens, are the (eight or
+// sixteen) columns of a product whose rows are sixteen keys, or sixteen columns of V.  A warp takes sixteen keys at a time through a
+// ring in shared memory of its own (cp.async: straight to registers 285 us of 32 sequences of up to 32768 keys, the ring 257 at the same
+// arithmetic) and has a running maximum, sum and accumulator of its own; these meet in shared memory, then in distributed
+// shared memory, where every CTA of a head's cluster finishes its share of the rows.
+// What a call has to do is read the visible rows once, 4 + 32 / group bits a value.  What bounds it is issue, some 400 instructions to sixteen
+// keys of a warp: of 32 sequences of up to 32768 keys (241 us), reading alone took 136 us when the whole took 247, arithmetic alone 244.
 #include "four_bit.cuh"
 #include "sdpa_window.cuh"
+
+#include <atomic>
 
 namespace bdattn {
 namespace {
@@ -148,7 +152,8 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         for (int gi = 0; gi < G; ++gi) mine = q == gi ? sum[gi] : mine;
         qs[nr][0] = __uint_as_float(__float_as_uint(mine) & 0xffffe000u);
         qs[nr][1] = mine - qs[nr][0];
-        const float down = pow2(-up) * (0x1p24f * a.scale * 1.4426950408889634f);
+        // (kept normal and finite: times the infinities and zeros that a difference of scores may be, it has to stay what it is)
+        const float down = fminf(fmaxf(pow2(-up) * (0x1p24f * a.scale * 1.4426950408889634f), FLT_MIN), FLT_MAX);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int from = (2 * q + h) * 4;
@@ -339,79 +344,79 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         auto weigh = [&](auto is_odd) {
             constexpr bool kOdd = decltype(is_odd)::value;
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-            float top[2] = {fmaxf(s[nr][0], s[nr][2]), fmaxf(s[nr][1], s[nr][3])};
-            // a new largest score is rare after the first steps
-            if (__any_sync(0xffffffffu, top[0] > m[nr][0] || top[1] > m[nr][1])) {
+            for (int nr = 0; nr < NR; ++nr) {
+                float top[2] = {fmaxf(s[nr][0], s[nr][2]), fmaxf(s[nr][1], s[nr][3])};
+                // a new largest score is rare after the first steps
+                if (__any_sync(0xffffffffu, top[0] > m[nr][0] || top[1] > m[nr][1])) {
 #pragma unroll
-                for (int x = 4; x < 32; x *= 2) {
-                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], x));
-                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], x));
+                    for (int x = 4; x < 32; x *= 2) {
+                        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], x));
+                        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], x));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float now = fmaxf(m[nr][h], top[h]);
+                        const float alpha = now == -INFINITY ? 1.0f : fast_exp2((m[nr][h] - now) * sl2[nr][h]);
+                        m[nr][h] = now;
+                        ref[nr][h] = now == -INFINITY ? 0.0f : now;
+                        l[nr][h] *= alpha;
+#pragma unroll
+                        for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] *= alpha;
+#pragma unroll
+                        for (int i = 0; i < 2 * S; ++i) {
+                            o[nr][i][h] *= alpha;
+                            o[nr][i][2 + h] *= alpha;
+                        }
+                    }
+                }
+                float p[4], lifted[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = fast_exp2((s[nr][e] - ref[nr][e & 1]) * sl2[nr][e & 1]);
+                    if (!kLiftSteps) lifted[e] = p[e] * v_lift;
+                    l[nr][e & 1] += p[e];
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float now = fmaxf(m[nr][h], top[h]);
-                    const float alpha = now == -INFINITY ? 1.0f : fast_exp2((m[nr][h] - now) * sl2[nr][h]);
-                    m[nr][h] = now;
-                    ref[nr][h] = now == -INFINITY ? 0.0f : now;
-                    l[nr][h] *= alpha;
+                for (int gi = 0; gi < G; ++gi) {
+                    float w[4];
 #pragma unroll
-                    for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] *= alpha;
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 v = layer_pair<kBf16>(vp[h][gi]);
+                        const float mid = fmaf(8.0f, v.x, v.y);
 #pragma unroll
-                    for (int i = 0; i < 2 * S; ++i) {
-                        o[nr][i][h] *= alpha;
-                        o[nr][i][2 + h] *= alpha;
+                        for (int c = 0; c < 2; ++c) {
+                            const int e = 2 * h + c;
+                            w[e] = kLiftSteps ? p[e] * lifted_step[h][gi] : lifted[e] * v.x;
+                            if (!kOdd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
+                        }
+                    }
+                    if (kOdd) {              // (zero times what is not finite: of a row that the query does not see)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 v = layer_pair<kBf16>(vp[e >> 1][gi]);
+                            if (p[e] == 0.0f) w[e] = 0.0f;
+                            else lo[nr][gi][e & 1] = fmaf(p[e], fmaf(8.0f, v.x, v.y), lo[nr][gi][e & 1]);
+                        }
+                    }
+                    const uint32_t b0 = c4_transpose8(pack2<false>(w[0], w[1])), b1 = c4_transpose8(pack2<false>(w[2], w[3]));
+#pragma unroll
+                    for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
+                        // four columns of two keys: the halves of a word of each
+                        const uint32_t sel = (i & 1) ? sel_high : sel_low;
+                        const uint32_t w0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), w1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
+                        uint32_t u0[4], u1[4];
+                        codes8(w0, u0);
+                        codes8(w1, u1);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            u0[e] = (e & 1) ? less_eight<true>(u0[e]) : less_eight<false>(u0[e]);
+                            u1[e] = (e & 1) ? less_eight<true>(u1[e]) : less_eight<false>(u1[e]);
+                        }
+                        mma16<false>(o[nr][2 * i], u0[0], u0[2], u1[0], u1[2], b0, b1);
+                        mma16<false>(o[nr][2 * i + 1], u0[1], u0[3], u1[1], u1[3], b0, b1);
                     }
                 }
             }
-            float p[4], lifted[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[e] = fast_exp2((s[nr][e] - ref[nr][e & 1]) * sl2[nr][e & 1]);
-                if (!kLiftSteps) lifted[e] = p[e] * v_lift;
-                l[nr][e & 1] += p[e];
-            }
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) {
-                float w[4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float2 v = layer_pair<kBf16>(vp[h][gi]);
-                    const float mid = fmaf(8.0f, v.x, v.y);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int e = 2 * h + c;
-                        w[e] = kLiftSteps ? p[e] * lifted_step[h][gi] : lifted[e] * v.x;
-                        if (!kOdd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
-                    }
-                }
-                if (kOdd) {              // (zero times what is not finite: of a row that the query does not see)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v = layer_pair<kBf16>(vp[e >> 1][gi]);
-                        if (p[e] == 0.0f) w[e] = 0.0f;
-                        else lo[nr][gi][e & 1] = fmaf(p[e], fmaf(8.0f, v.x, v.y), lo[nr][gi][e & 1]);
-                    }
-                }
-                const uint32_t b0 = c4_transpose8(pack2<false>(w[0], w[1])), b1 = c4_transpose8(pack2<false>(w[2], w[3]));
-#pragma unroll
-                for (int i = gi * kPer; i < (gi + 1) * kPer; ++i) {
-                    // four columns of two keys: the halves of a word of each
-                    const uint32_t sel = (i & 1) ? sel_high : sel_low;
-                    const uint32_t w0 = __byte_perm(vw[0][i / 2], vw[1][i / 2], sel), w1 = __byte_perm(vw[2][i / 2], vw[3][i / 2], sel);
-                    uint32_t u0[4], u1[4];
-                    codes8(w0, u0);
-                    codes8(w1, u1);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        u0[e] = (e & 1) ? less_eight<true>(u0[e]) : less_eight<false>(u0[e]);
-                        u1[e] = (e & 1) ? less_eight<true>(u1[e]) : less_eight<false>(u1[e]);
-                    }
-                    mma16<false>(o[nr][2 * i], u0[0], u0[2], u1[0], u1[2], b0, b1);
-                    mma16<false>(o[nr][2 * i + 1], u0[1], u0[3], u1[1], u1[3], b0, b1);
-                }
-            }
-        }
         };
         if (odd) weigh(std::true_type{});
         else weigh(std::false_type{});
@@ -511,9 +516,21 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 template <int HD, int G, bool kBf16, int W, int NR, int D, int kCtas>
 cudaError_t go_cache4(SdpaCache4Args a, int split, cudaStream_t stream) {
     using C = Cache4Cfg<HD, G, W, NR, D>;
-    const auto kern = a.key_mask != nullptr ? sdpa_cache4_kernel<HD, G, kBf16, true, W, NR, D, kCtas> : sdpa_cache4_kernel<HD, G, kBf16, false, W, NR, D, kCtas>;
+    const auto masked = sdpa_cache4_kernel<HD, G, kBf16, true, W, NR, D, kCtas>, plain = sdpa_cache4_kernel<HD, G, kBf16, false, W, NR, D, kCtas>;
+    const auto kern = a.key_mask != nullptr ? masked : plain;
     cudaError_t e = set_max_smem_once(kern, C::kSmem);
-    if (e == cudaSuccess && split > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && split > 8) {
+        // clusters of more than eight CTAs are allowed once for each device, and again where that has no bit
+        static std::atomic<unsigned long long> allowed{0};
+        int dev = 0;
+        e = cudaGetDevice(&dev);
+        const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+        if (e == cudaSuccess && (allowed.load() & bit) == 0) {
+            e = cudaFuncSetAttribute(masked, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(plain, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e == cudaSuccess) allowed.fetch_or(bit);
+        }
+    }
     if (e != cudaSuccess) return e;
     a.split = split;
     const dim3 grid(static_cast<unsigned>(split * a.c.kv_heads * a.row_tiles), static_cast<unsigned>(a.batch));
@@ -534,11 +551,10 @@ cudaError_t pick_cache4(SdpaCache4Args a, cudaStream_t stream) {
     // to a warp (8 heads over 32768 keys: sixteen CTAs 27.4 us, eight 33.5, sixteen of four warps 34.2; 32 heads over 4000 keys: eight CTAs 9.6,
     // sixteen of four warps 11.3).
     if (nr == 1 && units * 8 <= 2 * sms && steps >= 128) {
-        const int split = least(least(kC4MaxSplit, 2 * sms / units), steps / 16);
-        return go_cache4<HD, G, kBf16, 8, 1, 3, 2>(a, split < 1 ? 1 : split, stream);
+        return go_cache4<HD, G, kBf16, 8, 1, 3, 2>(a, least(least(kC4MaxSplit, 2 * sms / units), steps / 16), stream);
     }
     // Else four warps, and three and a half rounds of CTAs, so that the last one costs little (256 heads over up to 32768 keys: over six CTAs
-    // 238 us, over eight 249, over four 254, over two 290), but one step to a warp at least (8 heads over 777 keys: over eight 4.1, over
+    // 232 us, over eight 239, over four 245, over three 250), but one step to a warp at least (8 heads over 777 keys: over eight 4.1, over
     // sixteen 4.4, over six 4.7).
     constexpr int kOne = HD == 64 || G == 1 ? 4 : 3, kTwo = HD == 64 ? 4 : 2;           // CTAs of an SM: what registers allow
     const int slots = sms * (nr == 1 ? kOne : kTwo);

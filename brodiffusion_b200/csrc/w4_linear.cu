@@ -255,15 +255,15 @@ template <bool kBf16, int kGroups>
 cudaError_t pick_w4(W4Args a, cudaStream_t stream) {
     const int sms = sm_count(), tiles = (a.p.N - 1) / 16 + 1, pairs = (tiles + 1) / 2, kt = a.k_tiles;
     // the fewest CTAs to a cluster with which a warp has no more than `most` K tiles, if `ctas` such clusters fit `room` CTAs; or 0
-    auto split = [&](int ctas, long long room, int warps, int most) {
-        for (int p = 1; p <= kW4MaxParts && p * static_cast<long long>(ctas) <= room; ++p)
+    auto split = [&](long long ctas, long long room, int warps, int most) {
+        for (int p = 1; p <= kW4MaxParts && p * ctas <= room; ++p)
             if ((kt - 1) / (warps * p) + 1 <= most) return p;
         return 0;
     };
     // as many as there is room for with two K tiles to a warp
-    auto spread = [&](int ctas, long long room, int warps) {
+    auto spread = [&](long long ctas, long long room, int warps) {
         int p = 1;
-        while (p < kW4MaxParts && (p * 2) * static_cast<long long>(ctas) <= room && kt >= warps * p * 4) p *= 2;
+        while (p < kW4MaxParts && p * 2 * ctas <= room && kt >= warps * p * 4) p *= 2;
         return p;
     };
     if (a.p.M <= 8) {
@@ -278,13 +278,11 @@ cudaError_t pick_w4(W4Args a, cudaStream_t stream) {
     if (a.p.M <= 16) {
         if ((a.parts = split(tiles, sms, 8, 2)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 2, 1>(a, stream);
         if ((a.parts = split(tiles, 2ll * sms, 8, 3)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 1, 2>(a, stream);
-    }
-    if (a.p.M <= 16) {
         a.parts = spread(pairs, 3ll * sms, 4);
         return go_w4_few<kBf16, kGroups, 4, 2, 2, 1, 3>(a, stream);
     }
     // more rows: sixteen a pass, which read W from the L2 after the first (48 rows x 10240 x 2560 19.3 us, with four warps to a CTA 31)
-    a.parts = spread(pairs * ((a.p.M - 1) / 16 + 1), 2ll * sms, 8);
+    a.parts = spread(pairs * ((a.p.M - 1) / 16 + 1ll), 2ll * sms, 8);
     return go_w4_few<kBf16, kGroups, 8, 2, 2, 1, 2>(a, stream);
 }
 

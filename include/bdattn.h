@@ -622,8 +622,9 @@ int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_para
 
 /* ------------------------------------------- the same layer in 4 bits
  * Values in groups of 32, 64 or 128 of a row, each with a step and a lowest value of the activations' type (a
- * pair: step, then low):  x = low + step * u,  u in 0..15.  No operator rounds a value that it reads: codes meet the other
- * operand as integers, steps and lows are applied to FP32 sums.
+ * pair: step, then low):  x = low + step * u,  u in 0..15.  Products round no value
+ * that they read: codes meet the other operand as integers, steps and lows are applied to FP32 sums.  Attention rounds its weights
+ * times the steps once, to FP16.
  *
  * bdattn_sandwich_norm_fwd: what stands between two blocks of a layer with norms on both sides of each,
  *   b = x * rsqrt(mean(x^2) + eps) * post_gain,
@@ -665,10 +666,10 @@ int bdattn_sandwich_norm_fwd(const bdattn_sandwich_norm_params* p, bdattn_stream
  *   Y[m, n] = residual[m, n] + gate[n] * act(sum_k X[m, k] W[n, k] + bias[n]),
  * W packed by bdattn_w4_pack (once, at load) into bdattn_w4_bytes(N, K, group) bytes, 16-byte aligned: tiles of 16 rows x 128
  * columns, codes in the order of the kernel's lanes, pairs behind them.  X (M, K), Y, residual (M, N), bias and gate (N) of
- * dtype BF16 / F16, the pairs of the weights too; bias, gate and residual may be NULL; residual may be Y (same ld).  K and x_ld
- * are multiples of 8, X is 16-byte aligned; any N.  Meant for up to 64 rows, which read W once; more rows
- * read it again for each 64.  A row of X with a value that is not finite (BF16: of 2^63 and more) comes out not finite; BF16 values below 2^-57 may count as
- * zeros.
+ * dtype BF16 / F16, the pairs of the weights too; bias, gate and residual may be NULL; residual may be Y (same ld).  K (up to
+ * 2^30) and x_ld are multiples of 8, X is 16-byte aligned; any N; up to 524280 rows.  Y may not overlap X.  Meant for few rows: up to 16
+ * read W once, more read it again (from the L2, if it fits) for each 16.  A row of X with a value that is not finite (BF16: of 2^63
+ * and more) comes out not finite; BF16 values below 2^-57 may count as zeros.
  * bdattn_w4_pack: codes (N, K / 2 bytes, row stride codes_ld bytes) hold two columns a byte, the even one in the low half;
  * scales (N, ceil(K / group), 2) the pairs, row stride scales_ld values; a last group may be short. */
 typedef struct bdattn_linear_w4_params {
@@ -697,18 +698,21 @@ int bdattn_linear_w4_fwd(const bdattn_linear_w4_params* p, bdattn_stream_t strea
 /* A cache of K and V in 4 bits: (batch, num_kv_heads, rows, head_dim / 2) bytes of codes and (batch, num_kv_heads, rows,
  * head_dim / group, 2) pairs of dtype, for K and V each, rows of a head dense.  A group of a new row x is held as
  *   low = min x,  step = (max x - min x) / 15 rounded to dtype,  u = round((x - low) / step) up to 15 (0 where step is 0);
- * a group with a value that is not finite has NaN for both and is NaN.  Steps below 2^-126 count as 0.  The
+ * a group with a value that is not finite, or a range beyond FP32's largest value, has NaN for both and is NaN.  Steps below 2^-126 count as 0.  The
  * codes of a row lie in the order of the attention kernel's lanes (bdattn_cache4_read gives the values back); rows can be
- * moved, copied and left out as they are.  head_dim 64 or 128, group 32, 64 or 128 up to it; codes 16-byte aligned with
+ * moved, copied and left out as they are.  Up to 65535 items, 32767 heads and 2^30 rows, head_dim 64 or 128, group 32, 64 or 128 up to it; codes 16-byte aligned with
  * strides that are multiples of 16, scales aligned to a row's pairs.
  *
  * bdattn_cache4_append: row i of the r->rows new ones of item b goes to place n - r->rows + i, n = kv_len[b] (kv_len NULL: all
  * rows of the cache): kv_len counts the new rows already, as for the attention behind it.  A place before the
  * first row is not written.  bdattn_cache4_read: the same places back as low + step * u, rounded once (to the largest finite
- * value where a rounded step takes it beyond); zeros from before the first row.  k, v (batch, r->rows, num_kv_heads * head_dim) of dtype, 16-byte aligned with strides that are multiples of 8.
+ * value where a rounded step takes it beyond); zeros from before the first row.  k, v (batch, r->rows, num_kv_heads * head_dim) of
+ * dtype, 16-byte aligned with strides that are multiples of 8.
  *
  * bdattn_sdpa_cache4_fwd: bdattn_sdpa_window_fwd over such a cache: the same rule of what is seen, the same treatment of
- * kv_len, key_mask and rows that nobody sees (they may hold anything).  One query segment. */
+ * kv_len, key_mask and rows that nobody sees (they may hold anything).  Where a row's largest |q| times the scale is 2^117 or more, its scores may be too
+ * small by what it is beyond that.  One query segment; o may be q (same strides).  For up to some tens of new tokens:
+ * from there on bdattn_cache4_read and bdattn_sdpa_window_fwd take less time. */
 typedef struct bdattn_cache4 {
     int dtype;
     int batch;

@@ -96,6 +96,16 @@ def test_groups_of_one_value_and_values_that_are_not_finite(bd, dtype):
         assert int(torch.isnan(got).sum()) == 3 * 32 and (got[0, 0, :32] == 3).all() and (got[0, 1] == 0).all()
 
 
+def test_a_range_beyond_fp32_counts_as_not_finite(bd):
+    x = randn(1, 1, 2, 64)
+    x[0, 0, 3], x[0, 0, 5] = 3e38, -3e38
+    x[0, 1, 3], x[0, 1, 40] = 3e38, -3e38                  # (not in one group)
+    c = garbage(bd, 1, 1, 2, 64, 32, torch.bfloat16)
+    bd.cache4_append(x, x, c)
+    for got in read(bd, c, 2):
+        assert torch.isnan(got[0, 0, :32]).all() and torch.isfinite(got[0, 0, 32:]).all() and torch.isfinite(got[0, 1]).all()
+
+
 def test_ties_and_the_ends_of_the_types(bd):
     """Quotients on the border between two codes go to the even one; the largest finite values stay finite."""
     x = torch.zeros(1, 3, 64, device="cuda", dtype=torch.float16)
@@ -293,6 +303,24 @@ def test_magnitudes_of_queries_and_keys(bd, dtype, q_size, k_size):
     c = garbage(bd, 1, 1, 400, 128, 64, dtype)
     bd.cache4_append(k, v, c)
     check(run(bd, q, c, 2), q, k, v, 2, 1, 64)
+
+
+@pytest.mark.parametrize("q_size,scale", [(1e37, 0.0), (1e-30, 1e-30), (1.0, 1e-38)])
+def test_factors_beyond_fp32(bd, q_size, scale):
+    """The factor of the scores passes FP32's ends: the largest score takes all, or all seen keys count alike; hidden ones count for
+    nothing."""
+    q, k, v = randn(1, 1, 3, 128, scale=q_size), randn(2, 1, 100, 128), randn(3, 1, 100, 128)
+    c = garbage(bd, 1, 1, 100, 128, 64, torch.bfloat16)
+    bd.cache4_append(k, v, c)
+    out = torch.empty_like(q)
+    bd.sdpa_cache4_fwd(q, c, out, 1, softmax_scale=scale)
+    kh, vh = held(k, 64)[0], held(v, 64)[0]
+    for i in range(3):
+        n = 98 + i
+        want = vh[(kh[:n] @ q[0, i].double()).argmax()] if scale == 0 else vh[:n].mean(0)
+        # (a weight times a step and the output are rounded once each, and 2^-11 is the more for the FP32 sums)
+        bound = 2.0 ** -8 * want.abs() + 2.0 ** -11 * vh[:n].abs().amax(0)
+        assert ((out[0, i].double() - want).abs() <= bound).all()
 
 
 def test_queries_of_zeros_and_a_scale(bd):

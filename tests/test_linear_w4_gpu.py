@@ -208,7 +208,7 @@ def test_refusals(bd):
     assert bd.w4_bytes(0, 8, 32) == bd.w4_bytes(8, 0, 32) == bd.w4_bytes(8, 8, 33) == 0
     p = bd.LinearW4Params(dtype=bd.BF16, M=3, N=n, K=k, group=group, x=x.data_ptr(), w=packed.data_ptr(), y=y.data_ptr(), act=9)
     for field, value, reason in (("act", 9, "activation"), ("K", 132, "multiple of 8"), ("x_ld", 132, "multiple of 8"), ("x", 0, "null"),
-                                 ("y_ld", 8, "row stride"), ("w", packed.data_ptr() + 8, "aligned"), ("M", 600000, "rows"), ("M", -1, ">= 0")):
+                                 ("y_ld", 8, "row stride"), ("w", packed.data_ptr() + 8, "aligned"), ("M", 600000, "rows"), ("K", (1 << 30) + 8, "2^30"), ("M", -1, ">= 0")):
         q = bd.LinearW4Params.from_buffer_copy(p)
         q.act = 0
         setattr(q, field, value)
