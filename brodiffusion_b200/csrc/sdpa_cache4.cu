@@ -10,7 +10,7 @@
 // arithmetic) and has a running maximum, sum and accumulator of its own; these meet in shared memory, then in distributed
 // shared memory, where every CTA of a head's cluster finishes its share of the rows.
 // What a call has to do is read the visible rows once, 4 + 32 / group bits a value.  What bounds it is issue, some 400 instructions to sixteen
-// keys of a warp: of 32 sequences of up to 32768 keys (241 us), reading alone took 136 us when the whole took 247, arithmetic alone 244.
+// keys of a warp: of 32 sequences of up to 32768 keys (231 us), reading alone took 136 us when the whole took 247, arithmetic alone 244.
 #include "four_bit.cuh"
 #include "sdpa_window.cuh"
 
@@ -553,14 +553,20 @@ cudaError_t pick_cache4(SdpaCache4Args a, cudaStream_t stream) {
     if (nr == 1 && units * 8 <= 2 * sms && steps >= 128) {
         return go_cache4<HD, G, kBf16, 8, 1, 3, 2>(a, least(least(kC4MaxSplit, 2 * sms / units), steps / 16), stream);
     }
-    // Else four warps, and three and a half rounds of CTAs, so that the last one costs little (256 heads over up to 32768 keys: over six CTAs
-    // 232 us, over eight 239, over four 245, over three 250), but one step to a warp at least (8 heads over 777 keys: over eight 4.1, over
-    // sixteen 4.4, over six 4.7).
+    // Else four warps.  SMs come in pairs, the CTAs of a cluster find their places within some of them: where there is more than one round, a
+    // cluster is all the CTAs of a pair of SMs, or a part that divides them, so that no place stays empty (256 heads over up to 32768 keys,
+    // three CTAs to an SM: over six 232 us, over five 240, seven 241, eight 238; keys all alike 303, 330, 336, 332), and the smallest such part with
+    // two and a half rounds (512 heads over up to 8192 keys: over three 129, over six 137; 256 heads: over three 252).  Eight, where all run at
+    // once, but one step to a warp at least (8 heads over 777 keys: over eight 4.1, over sixteen 4.4, over six 4.7).
     constexpr int kOne = HD == 64 || G == 1 ? 4 : 3, kTwo = HD == 64 ? 4 : 2;           // CTAs of an SM: what registers allow
-    const int slots = sms * (nr == 1 ? kOne : kTwo);
-    int split = nr == 2 && units >= slots ? 1 : least(8, (7ll * slots / 2 + units - 1) / units);       // (509 x 2 rows, 16 heads of 64: whole 134, over two 144)
+    const int ctas = nr == 1 ? kOne : kTwo, slots = sms * ctas;
+    int split = 8;
+    if (units * 8 > slots) {
+        split = 1;
+        while (split < 2 * ctas && (2 * ctas % split != 0 || 2 * units * split < 5ll * slots)) ++split;
+    }
+    if (nr == 2 && units >= slots) split = 1;          // (509 x 2 rows, 16 heads of 64: whole 134, over two 144)
     split = least(split, (steps + 3) / 4);
-    if (split < 1) split = 1;
     return nr == 1 ? go_cache4<HD, G, kBf16, 4, 1, 3, kOne>(a, split, stream) : go_cache4<HD, G, kBf16, 4, 2, 3, kTwo>(a, split, stream);
 }
 
