@@ -22,7 +22,7 @@ __all__ = [
     "ROPE_INTERLEAVED", "ROPE_HALF_SPLIT", "SdpaParams", "NormRopeJob", "sdpa_fwd",
     "rmsnorm_rope", "linear_attn_relu_fwd", "rope_tables_flux", "rope_tables_qwen", "RopeSegment", "device_status", "last_error",
     "E4M3", "AddRmsNormParams", "add_rmsnorm_fwd", "WindowParams", "sdpa_window_fwd", "LinearActParams",
-    "linear_act_fwd", "SandwichNormParams", "sandwich_norm_fwd", "LinearW4Params", "w4_bytes", "w4_pack", "linear_w4_fwd",
+    "linear_act_fwd", "SandwichNormParams", "sandwich_norm_fwd", "LinearW4Params", "w4_bytes", "w4_pack", "w4_unpack", "linear_w4_fwd",
     "Cache4", "Cache4Params", "Cache4Rows", "SdpaCache4Params", "cache4_append", "cache4_read", "sdpa_cache4_fwd",
 ]
 
@@ -298,6 +298,7 @@ def lib():
         L.bdattn_w4_bytes.argtypes = [C.c_int] * 3
         L.bdattn_w4_pack.argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                      C.c_void_p]
+        L.bdattn_w4_unpack.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]
         L.bdattn_linear_w4_fwd.argtypes = [C.POINTER(LinearW4Params), C.c_void_p]
         L.bdattn_cache4_append.argtypes = [C.POINTER(Cache4Params), C.POINTER(Cache4Rows), C.c_void_p]
         L.bdattn_cache4_read.argtypes = [C.POINTER(Cache4Params), C.POINTER(Cache4Rows), C.c_void_p]
@@ -816,6 +817,11 @@ def w4_pack(codes, scales, packed, *, group, stream=None):
     """``bdattn_w4_pack``: codes (N, K / 2) uint8, two columns a byte with the even one in the low half, and scales
     (N, ceil(K / group), 2), the (step, low) pairs of w = low + step * code, into packed (``w4_bytes`` uint8)."""
     (_binding or _load_binding()).w4_pack(codes, scales, packed, group, None if stream is None else stream.cuda_stream)
+
+
+def w4_unpack(packed, w, *, group, stream=None):
+    """``bdattn_w4_unpack``: the packed matrix back as w (N, K), of the pairs' type, each value rounded once."""
+    (_binding or _load_binding()).w4_unpack(packed, w, group, None if stream is None else stream.cuda_stream)
 
 
 def linear_w4_fwd(x, w, bias, y, *, group, act="none", gate=None, residual=None, stream=None):

@@ -345,6 +345,20 @@ PyObject* w4_pack(PyObject* const* a) {
                                stream_of(a[4])));
 }
 
+// (packed, w, group, stream)
+PyObject* w4_unpack(PyObject* const* a) {
+    const at::Tensor &packed = tensor(a[0], "packed"), &w = tensor(a[1], "w");
+    const int group = integer(a[2]);
+    typed(&packed, at::kByte, "packed");
+    const Matrix mw(w, "w");
+    if (packed.dim() != 1 || static_cast<size_t>(packed.size(0)) != bdattn_w4_bytes(mw.rows, mw.cols, group) || (packed.size(0) > 1 && packed.stride(0) != 1) ||
+        packed.size(0) == 0)
+        refuse("packed must be dense, of w4_bytes(rows of w, columns of w, group) bytes");
+    const int dtype = code(w, "w");
+    on_gpu({&packed, &w});
+    return done(bdattn_w4_unpack(packed.data_ptr(), mw.data, mw.ld, mw.rows, mw.cols, group, dtype, stream_of(a[3])));
+}
+
 // (x, w, bias, y, group, act, gate, residual, stream)
 PyObject* linear_w4(PyObject* const* a) {
     const at::Tensor &x = tensor(a[0], "x"), &w = tensor(a[1], "w"), &y = tensor(a[3], "y");
@@ -538,6 +552,7 @@ PyMethodDef methods[] = {
     {"sdpa_window", fast(entry<sdpa_window, 12>), METH_FASTCALL, "bdattn_sdpa_window_fwd"},
     {"sandwich_norm", fast(entry<sandwich_norm, 11>), METH_FASTCALL, "bdattn_sandwich_norm_fwd"},
     {"w4_pack", fast(entry<w4_pack, 5>), METH_FASTCALL, "bdattn_w4_pack"},
+    {"w4_unpack", fast(entry<w4_unpack, 4>), METH_FASTCALL, "bdattn_w4_unpack"},
     {"linear_w4", fast(entry<linear_w4, 9>), METH_FASTCALL, "bdattn_linear_w4_fwd"},
     {"cache4_append", fast(entry<cache4_rows<true>, 8>), METH_FASTCALL, "bdattn_cache4_append"},
     {"cache4_read", fast(entry<cache4_rows<false>, 8>), METH_FASTCALL, "bdattn_cache4_read"},

@@ -174,6 +174,28 @@ int bdattn_w4_pack(const void* codes, long long codes_ld, const void* scales, lo
     return e != cudaSuccess ? cuda_fail(op, e) : 0;
 }
 
+int bdattn_w4_unpack(const void* packed, void* w, long long w_ld, int N, int K, int group, int dtype, bdattn_stream_t stream) {
+    const char* op = "bdattn_w4_unpack";
+    if (require_sm100(op)) return -1;
+    if (!is_16bit(dtype)) return fail("%s: dtype must be BF16 or F16 (got %d)", op, dtype);
+    if (!is_group(group)) return fail("%s: group must be 32, 64 or 128 (got %d)", op, group);
+    if (N < 1 || K < 1 || K % 8 != 0 || K > (1 << 30)) return fail("%s: N must be >= 1 and K a multiple of 8 up to 2^30 (got %d and %d)", op, N, K);
+    if (packed == nullptr || w == nullptr) return fail("%s: packed/w is null", op);
+    bdattn::W4UnpackArgs a;
+    a.ld = w_ld != 0 ? w_ld : K;
+    if (a.ld < K) return fail("%s: a row stride is smaller than a row", op);
+    if (a.ld % 8 != 0 || !aligned16(packed) || !aligned16(w))
+        return fail("%s: packed and w must be 16-byte aligned, the row stride of w a multiple of 8 (got %lld)", op, a.ld);
+    a.packed = static_cast<const uint8_t*>(packed);
+    a.w = static_cast<uint16_t*>(w);
+    a.N = N;
+    a.K = K;
+    a.group = group;
+    a.k_tiles = (K - 1) / 128 + 1;
+    const cudaError_t e = bdattn::launch_w4_unpack(a, dtype == BDATTN_BF16, reinterpret_cast<cudaStream_t>(stream));
+    return e != cudaSuccess ? cuda_fail(op, e) : 0;
+}
+
 int bdattn_linear_w4_fwd(const bdattn_linear_w4_params* p, bdattn_stream_t stream) {
     const char* op = "bdattn_linear_w4_fwd";
     if (p == nullptr) return fail("%s: params is null", op);

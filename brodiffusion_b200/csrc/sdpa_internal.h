@@ -286,7 +286,14 @@ struct W4PackArgs {
     long long codes_ld, scales_ld;
 };
 cudaError_t launch_w4_linear(const GemmProblem& p, const void* x, long long ldx, const void* w, int group, bool bf16, cudaStream_t stream);
+struct W4UnpackArgs {
+    const uint8_t* packed;
+    uint16_t* w;               // (N, K) of 16 bits
+    long long ld;
+    int N, K, group, k_tiles;
+};
 cudaError_t launch_w4_pack(const W4PackArgs& a, cudaStream_t stream);
+cudaError_t launch_w4_unpack(const W4UnpackArgs& a, bool bf16, cudaStream_t stream);
 
 // A cache in 4 bits: rows of heads behind one another, strides of batch items and heads in bytes (codes) and 16-bit units.
 struct Cache4Dev {

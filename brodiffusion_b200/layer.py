@@ -18,7 +18,7 @@ captured call would write the same rows again: of the calls above only the atten
 ``FourBitLayer`` is such a layer with a norm on both sides of each block, served with weights and cache in 4 bits:
 
     rows             <- add_rmsnorm_fwd   (16 bits, the stream's first norm)
-    Q, K, V          <- linear_w4_fwd
+    Q, K, V          <- linear_w4_fwd     (a few rows), or w4_unpack and linear_act_fwd (many); so all products
     Q, K             <- rmsnorm_rope
     cache            <- cache4_append     (to the places that the lengths on the device say)
     attention        <- sdpa_cache4_fwd   (a few new tokens), or cache4_read and sdpa_window_fwd (a prompt)
@@ -158,6 +158,9 @@ class FourBitLayer:
     # New tokens of a sequence from which on the cache is read back to 16 bits for the attention of whole prompts: that kernel takes
     # 128 rows at a time (2 x 509 rows of 16 heads over 8009 keys: 145 us from the 4 bits).
     PROMPT = 32
+    # Rows from which on a matrix goes back to 16 bits ahead of its product, a workspace of the call's (10240 x 2560: 64 rows 29.5 us in 4 bits,
+    # 21.7 so, 32 rows 18.2 and 21.6; 1536 rows 606 and 70).
+    MANY = 64
 
     def __init__(self, weights, num_heads, num_kv_heads, head_dim, *, window=0, sinks=0, act="gelu_tanh", eps=1e-6, group=64,
                  residual_scale=1.0):
@@ -170,7 +173,12 @@ class FourBitLayer:
     def _product(self, x, name, bias=None, **kw):
         import torch
         y = torch.empty(len(x), self.widths[name], device=x.device, dtype=x.dtype)
-        bd.linear_w4_fwd(x, self.packed[name], bias, y, group=self.group, **kw)
+        if len(x) < self.MANY:
+            bd.linear_w4_fwd(x, self.packed[name], bias, y, group=self.group, **kw)
+        else:
+            w = torch.empty(self.widths[name], x.shape[1], device=x.device, dtype=x.dtype)
+            bd.w4_unpack(self.packed[name], w, group=self.group)
+            bd.linear_act_fwd(x, w, bias, y, **kw)
         return y
 
     def forward(self, stream, cache, cos, sin):

@@ -668,10 +668,13 @@ int bdattn_sandwich_norm_fwd(const bdattn_sandwich_norm_params* p, bdattn_stream
  * columns, codes in the order of the kernel's lanes, pairs behind them.  X (M, K), Y, residual (M, N), bias and gate (N) of
  * dtype BF16 / F16, the pairs of the weights too; bias, gate and residual may be NULL; residual may be Y (same ld).  K (up to
  * 2^30) and x_ld are multiples of 8, X is 16-byte aligned; any N; up to 524280 rows.  Y may not overlap X.  Meant for few rows: up to 16
- * read W once, more read it again (from the L2, if it fits) for each 16.  A row of X with a value that is not finite (BF16: of 2^63
+ * read W once, more read it again (from the L2, if it fits) for each 16; for prompts bdattn_w4_unpack and a product in 16 bits take
+ * less time.  A row of X with a value that is not finite (BF16: of 2^63
  * and more) comes out not finite; BF16 values below 2^-57 may count as zeros.
  * bdattn_w4_pack: codes (N, K / 2 bytes, row stride codes_ld bytes) hold two columns a byte, the even one in the low half;
- * scales (N, ceil(K / group), 2) the pairs, row stride scales_ld values; a last group may be short. */
+ * scales (N, ceil(K / group), 2) the pairs, row stride scales_ld values; a last group may be short.
+ * bdattn_w4_unpack: the matrix (N, K) back in 16 bits, low + step * u rounded once to dtype, that of the pairs (to the largest finite value
+ * where it lies beyond), for bdattn_linear_act_fwd on many rows.  w 16-byte aligned, w_ld (0 => K) a multiple of 8. */
 typedef struct bdattn_linear_w4_params {
     int dtype;
     int M;                 /* 0: nothing is done */
@@ -693,6 +696,7 @@ typedef struct bdattn_linear_w4_params {
 size_t bdattn_w4_bytes(int N, int K, int group);
 int bdattn_w4_pack(const void* codes, long long codes_ld, const void* scales, long long scales_ld, void* packed, int N, int K,
                    int group, bdattn_stream_t stream);
+int bdattn_w4_unpack(const void* packed, void* w, long long w_ld, int N, int K, int group, int dtype, bdattn_stream_t stream);
 int bdattn_linear_w4_fwd(const bdattn_linear_w4_params* p, bdattn_stream_t stream);
 
 /* A cache of K and V in 4 bits: (batch, num_kv_heads, rows, head_dim / 2) bytes of codes and (batch, num_kv_heads, rows,

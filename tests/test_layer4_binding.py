@@ -71,6 +71,9 @@ def test_shapes_that_do_not_fit_are_refused_before_any_launch():
                  lambda: bd.w4_pack(z(32, 32, dtype=torch.uint8), z(32, 2, 2).float(), w, group=32),
                  lambda: bd.w4_pack(z(32, 32, dtype=torch.uint8), z(32, 2, 2), w[1:], group=32),
                  lambda: bd.w4_pack(z(32, 32, dtype=torch.uint8), z(1, 2, 2).expand(32, 2, 2), w, group=32),
+                 lambda: bd.w4_unpack(w[1:], z(32, 64), group=32), lambda: bd.w4_unpack(w, z(32, 64), group=64),
+                 lambda: bd.w4_unpack(w, z(32, 136), group=32), lambda: bd.w4_unpack(w, z(32, 64).int(), group=32),
+                 lambda: bd.w4_unpack(w, z(1, 64).expand(32, 64), group=32),
                  lambda: bd.cache4_append(k, k[:, :2], c), lambda: bd.cache4_append(k[:1], k[:1], c), lambda: bd.cache4_append(q, q, c),
                  lambda: bd.cache4_append(k.half(), k.half(), c), lambda: bd.cache4_append(k, k, c, kv_len=z(2)),
                  lambda: bd.cache4_append(k, k, c, kv_len=z(3, dtype=torch.int32)),
@@ -92,7 +95,7 @@ def test_shapes_that_do_not_fit_are_refused_before_any_launch():
     # tensors of the host are refused before the library sees their addresses
     for call in (lambda: bd.sandwich_norm_fwd(x, x, x), lambda: bd.linear_w4_fwd(x, w, None, y, group=32), lambda: bd.cache4_append(k, k, c),
                  lambda: bd.cache4_read(c, k, k), lambda: bd.sdpa_cache4_fwd(q, c, q, 4),
-                 lambda: bd.w4_pack(z(32, 32, dtype=torch.uint8), z(32, 2, 2), w, group=32)):
+                 lambda: bd.w4_pack(z(32, 32, dtype=torch.uint8), z(32, 2, 2), w, group=32), lambda: bd.w4_unpack(w, z(32, 64), group=32)):
         with pytest.raises(bd.BdattnError, match="GPU"):
             call()
 
@@ -103,11 +106,12 @@ def test_a_view_of_the_first_rows():
     assert c.rows == 16 and f.rows == 5 and f.k_codes.data_ptr() == c.k_codes.data_ptr() and f.v_scales.shape == (2, 2, 5, 2, 2)
 
 
-CALLS = ["add_rmsnorm_fwd", "linear_w4_fwd", "rmsnorm_rope", "cache4_append", "cache4_read", "sdpa_cache4_fwd", "sdpa_window_fwd", "sandwich_norm_fwd"]
+CALLS = ["add_rmsnorm_fwd", "linear_w4_fwd", "rmsnorm_rope", "cache4_append", "cache4_read", "sdpa_cache4_fwd", "sdpa_window_fwd", "sandwich_norm_fwd",
+         "w4_unpack", "linear_act_fwd"]
 
 
 @pytest.mark.parametrize("new", [2, 40])
-@pytest.mark.parametrize("refused", range(11))
+@pytest.mark.parametrize("refused", range(16))
 def test_a_refused_call_leaves_the_cache_as_it_was(monkeypatch, refused, new):
     D, nh, nkv, hd, F, B = 64, 2, 1, 64, 128, 3
     monkeypatch.setattr(LY, "quantise_rows4", lambda w, group: None)
@@ -130,7 +134,8 @@ def test_a_refused_call_leaves_the_cache_as_it_was(monkeypatch, refused, new):
         monkeypatch.setattr(bd, name, stand_in(name))
     cos = torch.zeros(64, hd // 2)
     x = z(B, new, D)
-    calls = 11 if new < L.PROMPT else 12
+    assert 2 < L.PROMPT <= 40 and 2 * B < L.MANY <= 40 * B
+    calls = 11 if new == 2 else 16
     if refused < calls:
         with pytest.raises(bd.BdattnError, match="refused"):
             L.forward(x, kv, cos, cos)
@@ -138,9 +143,10 @@ def test_a_refused_call_leaves_the_cache_as_it_was(monkeypatch, refused, new):
     made[:] = ["no more"] * 20
     L.forward(x, kv, cos, cos)
     assert kv.filled == [5 + new, new, 9 + new] and lengths.tolist() == kv.filled
-    assert made[20:] == ["add_rmsnorm_fwd", "linear_w4_fwd", "rmsnorm_rope", "rmsnorm_rope", "cache4_append"] + \
-        (["sdpa_cache4_fwd"] if new < L.PROMPT else ["cache4_read", "sdpa_window_fwd"]) + \
-        ["linear_w4_fwd", "sandwich_norm_fwd", "linear_w4_fwd", "linear_w4_fwd", "sandwich_norm_fwd"]
+    product = ["linear_w4_fwd"] if new == 2 else ["w4_unpack", "linear_act_fwd"]
+    assert made[20:] == ["add_rmsnorm_fwd", *product, "rmsnorm_rope", "rmsnorm_rope", "cache4_append"] + \
+        (["sdpa_cache4_fwd"] if new == 2 else ["cache4_read", "sdpa_window_fwd"]) + \
+        [*product, "sandwich_norm_fwd", *product, *product, "sandwich_norm_fwd"]
 
 
 # These kernels run before the kernel ahead of them has ended, and may not read what it writes through the read-only path.

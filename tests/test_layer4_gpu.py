@@ -82,6 +82,19 @@ def test_the_layers_quantiser(bd):
         assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1e-4 * cols ** 0.5).all()
 
 
+def test_products_of_many_rows_against_those_of_few(bd, monkeypatch):
+    """Matrices back in 16 bits, each value rounded once more (2^-9 of it, as the steps between are), against the 4 bits themselves."""
+    D, nh, nkv, hd, F, n = 640, 6, 2, 128, 1288, 100
+    w, g = weights(5, D, nh, nkv, hd, F, 0)
+    L = LY.FourBitLayer(w, nh, nkv, hd, group=32)
+    cos, sin = tables(128, hd)
+    x = torch.randn(1, n, D, device="cuda", generator=g).bfloat16()
+    many = L.forward(x.clone(), LY.KvCache4(1, n, nkv, hd, 64, x.dtype), cos, sin)
+    monkeypatch.setattr(LY.FourBitLayer, "MANY", 10 ** 9)
+    few = L.forward(x.clone(), LY.KvCache4(1, n, nkv, hd, 64, x.dtype), cos, sin)
+    assert not torch.equal(many, few) and far(many, few) < BOUND
+
+
 def test_chunks_and_single_tokens_continue_a_prompt(bd):
     D, nh, nkv, hd, F, n = 640, 6, 2, 128, 1280, 150
     w, g = weights(3, D, nh, nkv, hd, F, 0)

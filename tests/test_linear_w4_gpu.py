@@ -179,6 +179,45 @@ def test_no_rows_streams_repeats_and_capture(bd):
     check(y, x, codes, scales, group)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 128), (17, 136), (100, 648), (1291, 1368), (33, 10240)])
+def test_the_matrix_back_in_16_bits(bd, n, k, group, dtype):
+    """Bit for bit: each value rounded once, to the largest finite one where it lies beyond; what is not the matrix's is left."""
+    codes, scales = weights(n + k, n, k, group, dtype)
+    most = torch.finfo(dtype).max
+    scales[0, 0, 0], scales[0, 0, 1] = most / 8, most / 2
+    codes[0, :8] = torch.arange(8, 16, device="cuda")
+    if n > 1:
+        scales[1, 0] = float("nan")
+    wide = torch.full((n + 2, k + 16), 7.0, device="cuda", dtype=dtype)
+    bd.w4_unpack(pack(bd, codes, scales, group), wide[1:n + 1, 8:k + 8], group=group)
+    got, want = wide[1:n + 1, 8:k + 8].clone(), values(codes, scales, group).clamp(-most, most).to(dtype)
+    assert ((got == want) | (torch.isnan(got) & torch.isnan(want))).all()
+    assert int(torch.isnan(got).sum()) == (min(group, k) if n > 1 else 0)
+    wide[1:n + 1, 8:k + 8] = 7.0
+    assert (wide == 7.0).all() and bd.device_status() == 0
+
+
+def test_refusals_of_the_matrix_back(bd):
+    codes, scales = weights(3, 20, 128, 32, torch.bfloat16)
+    packed, w = pack(bd, codes, scales, 32), torch.zeros(20, 128, device="cuda", dtype=torch.bfloat16)
+    for call in (lambda: bd.w4_unpack(packed[:-1], w, group=32), lambda: bd.w4_unpack(packed, w, group=64), lambda: bd.w4_unpack(packed, w, group=16),
+                 lambda: bd.w4_unpack(packed, w.repeat(1, 2), group=32), lambda: bd.w4_unpack(packed, w.float(), group=32),
+                 lambda: bd.w4_unpack(packed, w[:1].expand(20, 128), group=32), lambda: bd.w4_unpack(packed, w.t().contiguous().t(), group=32),
+                 lambda: bd.w4_unpack(packed.view(torch.int8), w, group=32), lambda: bd.w4_unpack(packed, w.cpu(), group=32)):
+        with pytest.raises(bd.BdattnError):
+            call()
+    L = bd.lib()
+    good = dict(packed=packed.data_ptr(), w=w.data_ptr(), ld=128, N=20, K=128, group=32, dtype=bd.BF16)
+    for field, value, reason in (("packed", 0, "null"), ("w", 0, "null"), ("w", w.data_ptr() + 8, "aligned"), ("ld", 120, "row stride"), ("ld", 132, "multiple of 8"),
+                                 ("N", 0, "N must"), ("K", 132, "multiple of 8"), ("K", (1 << 30) + 8, "2^30"), ("group", 48, "group"), ("dtype", bd.F32, "dtype")):
+        c = dict(good, **{field: value})
+        assert L.bdattn_w4_unpack(c["packed"], c["w"], c["ld"], c["N"], c["K"], c["group"], c["dtype"], None) == -1
+        assert reason in bd.last_error(), (field, bd.last_error())
+    assert (w == 0).all()
+
+
 def test_refusals(bd):
     n, k, group = 32, 128, 32
     codes, scales = weights(15, n, k, group, torch.bfloat16)
