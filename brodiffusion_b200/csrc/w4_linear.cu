@@ -317,15 +317,19 @@ cudaError_t pick_w4(W4Args a, cudaStream_t stream) {
         a.parts = spread(pairs, 5ll * sms, 4);
         return go_w4_few<kBf16, kGroups, 4, 2, 1, 1, 5>(a, stream);
     }
-    if (a.p.M <= 16) {
-        if ((a.parts = split(tiles, sms, 8, 2)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 2, 1>(a, stream);
-        if ((a.parts = split(tiles, 2ll * sms, 8, 3)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 1, 2>(a, stream);
-        a.parts = spread(pairs, 3ll * sms, 4);
-        return go_w4_few<kBf16, kGroups, 4, 2, 2, 1, 3>(a, stream);
+    // More rows: sixteen a pass, which read W from the L2 after the first; the same rules, of all passes' CTAs.  Few tiles as above (13 x 1291 x 1368
+    // 3.2 us, 40 rows 4.2, two row tiles to a CTA 5.1).  Else four warps, three CTAs to an SM (16 x 2560 x 10240 over four 9.9, eight warps over three
+    // 10.8; 12 x 10240 x 2560 9.1, 11.8; 32 x 5120 x 5120 15.0, 17.5), but eight where several passes' CTAs of them all run at once (48 x 2560 x 10240
+    // 19.3, 22.2) or those of four do not (48 x 5120 x 5120 20.8, 24.6).
+    const long long passes = (a.p.M - 1) / 16 + 1;
+    if ((a.parts = split(tiles * passes, sms, 8, 2)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 2, 1>(a, stream);
+    if ((a.parts = split(tiles * passes, 2ll * sms, 8, 3)) != 0) return go_w4_few<kBf16, kGroups, 8, 1, 2, 1, 2>(a, stream);
+    if (passes > 1 && (pairs * passes <= 2ll * sms || pairs * passes > 3ll * sms)) {
+        a.parts = spread(pairs * passes, 2ll * sms, 8);
+        return go_w4_few<kBf16, kGroups, 8, 2, 2, 1, 2>(a, stream);
     }
-    // more rows: sixteen a pass, which read W from the L2 after the first (48 rows x 10240 x 2560 19.3 us, with four warps to a CTA 31)
-    a.parts = spread(pairs * ((a.p.M - 1) / 16 + 1ll), 2ll * sms, 8);
-    return go_w4_few<kBf16, kGroups, 8, 2, 2, 1, 2>(a, stream);
+    a.parts = spread(pairs * passes, 3ll * sms, 4);
+    return go_w4_few<kBf16, kGroups, 4, 2, 2, 1, 3>(a, stream);
 }
 
 }  // namespace
