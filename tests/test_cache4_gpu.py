@@ -9,6 +9,10 @@ Tolerance of the attention, for o = sum p v with v = (low + 8 step) + step (u - 
   - the sums of n keys in FP32, n / 64 of them one behind the other: (n / 64 + 64) 2^-23;
   - the output is rounded once."""
 import math
+import os
+import subprocess
+import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -397,6 +401,75 @@ def test_the_same_call_gives_the_same_bits_on_any_stream_and_captured(bd):
         check(out, q, k, v, 4, 2, 32)
         k1.copy_(randn(6, 2, 4, 256))
         n += 4
+
+
+@pytest.mark.parametrize("lq,hd,window", [(1, 128, 0), (3, 64, 40), (70, 64, 0)])
+def test_the_output_in_the_queries_place(bd, lq, hd, window):
+    q, k, v = randn(1, 2, lq, 4 * hd), randn(2, 2, 3000, 2 * hd), randn(3, 2, 3000, 2 * hd)
+    c = garbage(bd, 2, 2, 3000, hd, 32, torch.bfloat16)
+    bd.cache4_append(k, v, c)
+    apart = run(bd, q, c, 4, window=window)
+    bd.sdpa_cache4_fwd(q, c, q, 4, window=window)
+    assert torch.equal(q, apart)
+
+
+def test_calls_at_once(bd):
+    """Two host threads with a stream and tensors of their own each: the bits of calls one behind the other."""
+    def work(i, stream):
+        heads, hd = (4, 128) if i else (8, 64)
+        q, k, v = randn(i, 3, 2, heads * hd), randn(i + 2, 3, 5000, heads * hd // 2), randn(i + 4, 3, 5000, heads * hd // 2)
+        packed = torch.randint(0, 100, (bd.w4_bytes(1291, heads * hd, 64),), device="cuda", dtype=torch.uint8, generator=torch.Generator("cuda").manual_seed(i))
+        x, res = q.view(6, -1), randn(i + 6, 6, heads * hd)
+        c = garbage(bd, 3, heads // 2, 5000, hd, 64, torch.bfloat16)
+        out = []
+        stream.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            bd.cache4_append(k, v, c, stream=stream)
+            with torch.cuda.stream(stream):
+                o, y, r = torch.empty_like(q), torch.empty(6, 1291, device="cuda", dtype=torch.bfloat16), torch.empty_like(res)
+            bd.sdpa_cache4_fwd(q, c, o, heads, stream=stream)
+            bd.linear_w4_fwd(x, packed, None, y, group=64, stream=stream)
+            bd.sandwich_norm_fwd(x, res, r, stream=stream)
+            out.append((o, y, r))
+        stream.synchronize()
+        return out
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    alone = [work(i, s)[0] for i, s in enumerate(streams)]
+    with ThreadPoolExecutor(2) as pool:
+        together = [f.result() for f in [pool.submit(work, i, s) for i, s in enumerate(streams)]]
+    for one, many in zip(alone, together):
+        for got in many:
+            for a, b in zip(one, got):
+                assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+CAPTURED_FIRST = """
+import torch, brodiffusion_b200 as bd
+r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+q, k, x = r(1, 1, 1024), r(1, 32768, 1024), r(40, 1024)
+c = bd.Cache4.empty(1, 8, 32768, 128, 32, torch.bfloat16)
+w = torch.zeros(bd.w4_bytes(5000, 1024, 32), device="cuda", dtype=torch.uint8)
+o, y, m, t = torch.empty_like(q), torch.empty(40, 5000, device="cuda", dtype=torch.bfloat16), r(5000, 1024), torch.empty_like(x)
+calls = lambda: (bd.cache4_append(k, k, c), bd.sdpa_cache4_fwd(q, c, o, 8), bd.linear_w4_fwd(x, w, None, y, group=32), bd.w4_unpack(w, m, group=32),
+                 bd.sandwich_norm_fwd(x, x, t))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    calls()
+g.replay()
+torch.cuda.synchronize()
+first = [a.clone() for a in (o, y, m, t)]
+calls()
+assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(first, (o, y, m, t))) and bd.device_status() == 0
+print("captured first")
+"""
+
+
+def test_a_processs_first_calls_are_captured():
+    """What a launch looks up once (limits of shared memory, clusters of more than eight CTAs) is no obstacle to a capture."""
+    res = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], capture_output=True, text=True, timeout=300,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert res.returncode == 0 and "captured first" in res.stdout, res.stderr[-2000:]
 
 
 def test_refusals(bd):
