@@ -53,11 +53,25 @@ __device__ __forceinline__ uint32_t extreme2(uint32_t a, uint32_t b) {
     return r;
 }
 
-// a / b rounded to the nearest, by Markstein's correction of a * (1 / b); inv is 1 / b rounded to the nearest, the quotient neither
-// huge nor tiny.
-__device__ __forceinline__ float quotient(float a, float b, float inv) {
-    const float q = a * inv;
-    return fmaf(fmaf(-q, b, a), inv, q);
+// Two FP32 values to an instruction, of the kind that keeps what is below the normal range (the library is compiled to flush it).
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+// a * b + c
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 z, x, y, z; mov.b64 {%0, %1}, z;}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
+// a / b rounded to the nearest, by Markstein's correction of a * (1 / b); minus_b is -b, inv is 1 / b rounded to the nearest, the
+// quotients neither huge nor tiny.  (What is left of a is below the normal range where b is below 2^-102.)
+__device__ __forceinline__ float2 quotients(float2 a, float minus_b, float inv) {
+    const float2 i = make_float2(inv, inv), q = fma2(a, i, make_float2(0.0f, 0.0f));
+    return fma2(fma2(q, make_float2(minus_b, minus_b), a), i, q);
 }
 
 template <bool kBf16, int HD, int kGroup>
@@ -86,7 +100,8 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4RowsArgs
             hi2 = extreme2<kBf16, true>(hi2, __shfl_xor_sync(0xffffffffu, hi2, o));
         }
         const float low = layer_pair<kBf16>(extreme2<kBf16, false>(lo2, lo2 >> 16)).x, high = layer_pair<kBf16>(extreme2<kBf16, true>(hi2, hi2 >> 16)).x;
-        uint32_t pair = pack2<kBf16>(quotient(high - low, 15.0f, 1.0f / 15.0f), low);
+        const float2 minus = make_float2(-1.0f, -1.0f), low2 = make_float2(low, low);
+        uint32_t pair = pack2<kBf16>(quotients(fma2(low2, minus, make_float2(high, high)), -15.0f, 1.0f / 15.0f).x, low);
         float step = layer_pair<kBf16>(pair).x;
         // (a value that is not finite has made one of both so)
         if (!(step <= FLT_MAX && fabsf(low) <= FLT_MAX)) {
@@ -103,15 +118,12 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4RowsArgs
             const uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
 #pragma unroll
             for (int e = 3; e >= 0; --e) {
-                const float2 f = layer_pair<kBf16>(w[e]);
+                float2 u = quotients(fma2(low2, minus, layer_pair<kBf16>(w[e])), -step, inv);
                 // (only steps below FP16's smallest normal are so much smaller than a fifteenth of the range that a code could be 16)
-                float u[2] = {quotient(f.x - low, step, inv), quotient(f.y - low, step, inv)};
-                if (!kBf16) {
-                    u[0] = fminf(u[0], 15.0f);
-                    u[1] = fminf(u[1], 15.0f);
-                }
-                codes = codes * 16 + __float_as_uint(u[1] + kRound);
-                codes = codes * 16 + __float_as_uint(u[0] + kRound);
+                if (!kBf16) u = make_float2(fminf(u.x, 15.0f), fminf(u.y, 15.0f));
+                u = add2(u, make_float2(kRound, kRound));
+                codes = codes * 16 + __float_as_uint(u.y);
+                codes = codes * 16 + __float_as_uint(u.x);
             }
             codes -= kRest;
         }
