@@ -316,11 +316,12 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         }
         // a new largest step of V is rare after the first keys
         if (__any_sync(0xffffffffu, careful >= v_most)) {
-            const int e = static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(careful)) >> 23) - 127 - 14;
+            // (at least -126, so that the power and the one that takes it back are both normal)
+            const int e = max(-126, static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(careful)) >> 23) - 127 - 14);
             const float f = v_exp < e - 126 ? 0.0f : pow2(v_exp - e);
             v_exp = e;
-            v_lift = pow2(min(127, -v_exp));
-            v_most = e < 112 ? pow2(max(-126, e + 15)) : INFINITY;
+            v_lift = pow2(-v_exp);
+            v_most = e < 112 ? pow2(e + 15) : INFINITY;
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
