@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         const bool whole = (step < whole_sinks || (step >= whole_first && step < whole_end)) && live == 0xffffffffu;
         float careful = 0.0f;            // the largest step of V of this lane's keys
         bool odd = false;                // some of their pairs are not finite, and not all queries may see them
+        uint32_t hidden = 0;             // of the scores, by bits
         if (!whole) {
             const int begin = step < sink_steps ? 0 : span.win_begin, end = step < sink_steps ? span.sink_end : span.win_end;
 #pragma unroll
@@ -291,7 +292,10 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const bool seen = on && key <= pos[nr][c] && (a.window == 0 || pos[nr][c] - key < a.window || key < a.sinks);
-                        if (!seen) s[nr][2 * h + c] = -INFINITY;
+                        if (!seen) {
+                            s[nr][2 * h + c] = -INFINITY;
+                            hidden |= 1u << (nr * 4 + 2 * h + c);
+                        }
                     }
                 }
                 // what hidden rows hold counts for nothing (nor does a step that is not finite below, where some rows may not see it)
@@ -391,11 +395,11 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                             if (!kOdd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
                         }
                     }
-                    if (kOdd) {              // (zero times what is not finite: of a row that the query does not see)
+                    if (kOdd) {              // (what a query does not see is left out; zero times what it does see is NaN where that is not finite)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float2 v = layer_pair<kBf16>(vp[e >> 1][gi]);
-                            if (p[e] == 0.0f) w[e] = 0.0f;
+                            if ((hidden >> (nr * 4 + e)) & 1u) w[e] = 0.0f;
                             else lo[nr][gi][e & 1] = fmaf(p[e], fmaf(8.0f, v.x, v.y), lo[nr][gi][e & 1]);
                         }
                     }

@@ -1,4 +1,4 @@
-"""Attention over the 4-bit cache where the steps of V are beyond what FP16 holds."""
+"""Attention over the 4-bit cache where the steps of V are beyond what FP16 holds, or not finite."""
 import math
 
 import pytest
@@ -37,3 +37,20 @@ def test_tiny_values(bd, size, mix, lq, hd, group):
         tol = UNIT[q.dtype] * ref.abs() + (2.0 ** -11 + 2.0 ** -17) * (p @ (step * (vc - 8).abs())) + 2.0 ** -11 * (p @ ((vd - 8 * step).abs() + 8 * step)) + 3 * n * 2.0 ** -126
         err = (out[0, :, h * hd:(h + 1) * hd].double() - ref).abs()
         assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("at", [3, 20, 58])
+@pytest.mark.parametrize("lq", [1, 5])
+def test_a_visible_row_that_is_not_finite_reaches_the_output_whatever_its_weight(bd, at, lq):
+    """0 times NaN is NaN, whether or not all queries see all of the sixteen keys that the row lies among."""
+    hd, n = 64, 60
+    q = randn(1, 1, lq, hd).abs() + 1
+    k, v = randn(2, 1, n, hd), randn(3, 1, n, hd)
+    k[0, at], v[0, at, :32] = -1000.0, float("nan")          # a score of -8000 and less
+    out = attend(bd, q, k, v, 1, 1, 32)
+    for i in range(lq):
+        sees = n - lq + i >= at
+        assert torch.isnan(out[0, i, :32]).all() == sees and torch.isfinite(out[0, i, 32:]).all(), (i, sees)
+    mask = torch.ones(n, device="cuda")
+    mask[at] = 0
+    assert torch.isfinite(attend(bd, q, k, v, 1, 1, 32, key_mask=mask)).all()
