@@ -20,6 +20,7 @@ namespace bdattn {
 namespace {
 
 constexpr int kC4MaxSplit = 16;
+constexpr float kC4MostLift = 0x1p126f;
 
 __device__ __forceinline__ uint32_t c4_transpose8(uint32_t v) {
     uint32_t r;
@@ -32,8 +33,14 @@ __device__ __forceinline__ void c4_store_cluster(uint32_t addr, float4 v) {
 __device__ __forceinline__ void c4_store_cluster(uint32_t addr, float2 v) {
     asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
 }
-// 2^e for e in [-126, 127]
+// 2^e for e in [-126, 127], and e of a normal number's power of two
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+__device__ __forceinline__ int exponent(float f) { return static_cast<int>(__float_as_uint(f) >> 23) - 127; }
+// a / b, powers of two; 0 below FP32's normal range
+__device__ __forceinline__ float pow2_ratio(float a, float b) {
+    const int e = exponent(a) - exponent(b);
+    return e < -126 ? 0.0f : pow2(min(e, 127));
+}
 
 template <int HD, int G, int W, int NR, int D>
 struct Cache4Cfg {
@@ -41,7 +48,7 @@ struct Cache4Cfg {
     static constexpr int kCodes = 16 * HD / 2, kScales = 16 * 4 * G, kStep = 2 * (kCodes + kScales);      // bytes of sixteen keys
     static constexpr int kRing = W * D * kStep, kSums = W * kRows * kLd * 4;                              // (the sums lie in the ring's place)
     static constexpr int kFirst = kRing > kSums ? kRing : kSums;
-    static constexpr int kSmem = kFirst + (kMergeRows * (kLd + 2) + W * kRows * 2) * 4;
+    static constexpr int kSmem = kFirst + (kMergeRows * (kLd + 2) + W * kRows * (2 + G)) * 4;
 };
 
 // Global to shared memory, 4, 8 or 16 bytes.
@@ -74,6 +81,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     float* const o_cta = reinterpret_cast<float*>(c4_smem + C::kFirst);     // [kMergeRows][kLd]
     float2* const ml_warp = reinterpret_cast<float2*>(o_cta + C::kMergeRows * C::kLd);     // [W][kRows]
     float2* const ml_cta = ml_warp + W * kRows;                             // [kMergeRows]
+    float2* const lifts = ml_cta + C::kMergeRows;                           // [W][NR][G][4], pairs of rows
 
     const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int split = a.split, part = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -205,8 +213,28 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < 2 * S; ++i) o[nr][i][0] = o[nr][i][1] = o[nr][i][2] = o[nr][i][3] = 0.0f;
     }
-    int v_exp = -1000;           // the steps of V count 2^-v_exp each: the largest so far is in [2^14, 2^15) then
-    float v_lift = 0.0f, v_most = 0.0f;          // 2^-v_exp; the step from which on it is another
+    // The weights times the steps of V, which FP16 has to hold, are lifted by powers of two to where the largest is some 2^11, for every query row by
+    // what it sees, and by what counts of that, alone: a key that it does not see, or that has next to no weight, may have steps 2^100 times as large.
+    // One lift serves all groups of a row while the largest of each is 2^2 or more by it; then (uneven) each has its own, in shared memory.
+    // What FP16 loses below its normal range is 2^-19 of the largest a key then, at most.  (One lift for all rows, by the largest step that any of them might
+    // see, took 1 to 6 % less: 32 sequences of up to 32768 keys 248 us, this way 254, groups of 128 83.0 and 83.5.)
+    float lift[NR][2], fades[NR][2];      // (fades: scores from here on make 2^-8 and less of what a row has so far)
+    float v_most = INFINITY;              // steps from here on might be too large
+    bool uneven = false;
+    uint32_t dead = 0;                    // groups that had nothing but steps of 0 when their lift was chosen
+    float2* const own = lifts + warp * NR * G * 4 + q;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        lift[nr][0] = lift[nr][1] = kC4MostLift;
+        fades[nr][0] = fades[nr][1] = -INFINITY;
+    }
+    auto scale_o = [&](int nr, int gi, int c, float f) {
+#pragma unroll
+        for (int i = 2 * gi * kPer; i < 2 * (gi + 1) * kPer; ++i) {
+            o[nr][i][c] *= f;
+            o[nr][i][2 + c] *= f;
+        }
+    };
     const int stride = W * split;
     int step = part * W + warp, slot = 0;
 #pragma unroll
@@ -214,7 +242,11 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
         if (step + i * stride < steps) fetch(step + i * stride, i);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    for (; step < steps; step += stride) {
+    // (two loops: what looks at the groups' own lifts is in the second alone, to which a warp goes for good when it has some; in one it cost 3 %)
+    auto walk = [&](auto is_by_groups) {
+    constexpr bool kByGroups = decltype(is_by_groups)::value;
+    bool leave = false;
+    for (; step < steps && !leave; step += stride) {
         asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
         __syncwarp();            // all lanes' copies are there, and all lanes have read the slot that is filled next
         if (step + (D - 1) * stride < steps) fetch(step + (D - 1) * stride, slot == 0 ? D - 1 : slot - 1);
@@ -318,68 +350,132 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             }
             careful = fmaxf(0.0f, layer_pair<kBf16>(top).x);
         }
-        // a new largest step of V is rare after the first keys
-        if (__any_sync(0xffffffffu, careful >= v_most)) {
-            // (at least -126, so that the power and the one that takes it back are both normal)
-            const int e = max(-126, static_cast<int>(__reduce_max_sync(0xffffffffu, __float_as_uint(careful)) >> 23) - 127 - 14);
-            const float f = v_exp < e - 126 ? 0.0f : pow2(v_exp - e);
-            v_exp = e;
-            v_lift = pow2(-v_exp);
-            v_most = e < 112 ? pow2(e + 15) : INFINITY;
+        // a step of V that might be too large, were its weight 1, is rare
+        bool special = odd || (kByGroups && uneven) || __any_sync(0xffffffffu, careful >= v_most);
+        if (kByGroups && dead != 0) {
+            bool some = false;
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
+            for (int i = 0; i < 2 * G; ++i) some = some || (((dead >> (i % G)) & 1u) != 0 && layer_pair<kBf16>(vp[i / G][i % G]).x != 0.0f);
+            special = __any_sync(0xffffffffu, some) || special;
+        }
 #pragma unroll
-                for (int i = 0; i < 2 * S; ++i) {
+        for (int nr = 0; nr < NR; ++nr) {
+            float top[2] = {fmaxf(s[nr][0], s[nr][2]), fmaxf(s[nr][1], s[nr][3])};
+            // a new largest score is rare after the first steps
+            if (__any_sync(0xffffffffu, top[0] > m[nr][0] || top[1] > m[nr][1])) {
+                special = __any_sync(0xffffffffu, top[0] > fades[nr][0] || top[1] > fades[nr][1]) || special;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) o[nr][i][x] *= f;
+                for (int x = 4; x < 32; x *= 2) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], x));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], x));
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float now = fmaxf(m[nr][h], top[h]);
+                    const float alpha = now == -INFINITY ? 1.0f : fast_exp2((m[nr][h] - now) * sl2[nr][h]);
+                    m[nr][h] = now;
+                    ref[nr][h] = now == -INFINITY ? 0.0f : now;
+                    l[nr][h] *= alpha;
+#pragma unroll
+                    for (int gi = 0; gi < G; ++gi) {
+                        lo[nr][gi][h] *= alpha;
+                        scale_o(nr, gi, h, alpha);
+                    }
                 }
             }
         }
-        // the power of two goes to the steps or to the weights, whichever are fewer
-        constexpr bool kLiftSteps = 2 * G < 4 * NR;
-        float lifted_step[2][G];
-        if (kLiftSteps) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int gi = 0; gi < G; ++gi) lifted_step[h][gi] = layer_pair<kBf16>(vp[h][gi]).x * v_lift;
-            }
-        }
-        // (code of its own where pairs are not finite: as branches of one, its instructions are issued all the same)
-        auto weigh = [&](auto is_odd) {
-            constexpr bool kOdd = decltype(is_odd)::value;
+        // (code of its own where lifts are looked at, or pairs are not finite: as branches of one, its instructions are issued all the same)
+        auto weigh = [&](auto is_special) {
+            constexpr bool kSpecial = decltype(is_special)::value;
+            float p[NR][4], by[NR][kSpecial ? G : 1][2];
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-                float top[2] = {fmaxf(s[nr][0], s[nr][2]), fmaxf(s[nr][1], s[nr][3])};
-                // a new largest score is rare after the first steps
-                if (__any_sync(0xffffffffu, top[0] > m[nr][0] || top[1] > m[nr][1])) {
 #pragma unroll
-                    for (int x = 4; x < 32; x *= 2) {
-                        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], x));
-                        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], x));
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    p[nr][e] = fast_exp2((s[nr][e] - ref[nr][e & 1]) * sl2[nr][e & 1]);
+                    l[nr][e & 1] += p[nr][e];
+                }
+                by[nr][0][0] = lift[nr][0];
+                by[nr][0][1] = lift[nr][1];
+            }
+            if constexpr (kSpecial) {
+                float highest = 0.0f;
+                bool apart = false;
+                dead = 0;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float now = fmaxf(m[nr][h], top[h]);
-                        const float alpha = now == -INFINITY ? 1.0f : fast_exp2((m[nr][h] - now) * sl2[nr][h]);
-                        m[nr][h] = now;
-                        ref[nr][h] = now == -INFINITY ? 0.0f : now;
-                        l[nr][h] *= alpha;
+                for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
-                        for (int gi = 0; gi < G; ++gi) lo[nr][gi][h] *= alpha;
+                    for (int c = 0; c < 2; ++c) {
+                        // (2^up: what the row has faded by)
+                        const int up = static_cast<int>(fminf(fmaxf((m[nr][c] - fades[nr][c]) * sl2[nr][c] + 8.0f, 0.0f), 252.0f));
+                        const float up0 = pow2(up / 2), up1 = pow2(up - up / 2);
+                        float most[G], least = kC4MostLift, any = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 2 * S; ++i) {
-                            o[nr][i][h] *= alpha;
-                            o[nr][i][2 + h] *= alpha;
+                        for (int gi = 0; gi < G; ++gi) {
+                            // what has faded comes up again, where there is something
+                            bool nothing = fades[nr][c] == -INFINITY;
+                            if constexpr (kByGroups) {
+                                nothing = true;
+#pragma unroll
+                                for (int i = 2 * gi * kPer; i < 2 * (gi + 1) * kPer; ++i) nothing = nothing && o[nr][i][c] == 0.0f && o[nr][i][2 + c] == 0.0f;
+                                nothing = (~__ballot_sync(0xffffffffu, nothing) & (0x11111111u << q)) == 0;
+                            }
+                            const float was = kByGroups && uneven ? reinterpret_cast<const float*>(own + (nr * G + gi) * 4)[c] : lift[nr][c];
+                            float now = nothing ? kC4MostLift : fminf(was * up0 * up1, kC4MostLift);
+                            // the largest of these sixteen keys goes to 2^11 where it is too large
+                            float t = fmaxf(fmaxf(0.0f, p[nr][c] * layer_pair<kBf16>(vp[0][gi]).x), p[nr][2 + c] * layer_pair<kBf16>(vp[1][gi]).x);
+#pragma unroll
+                            for (int x = 4; x < 32; x *= 2) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+                            most[gi] = t = fminf(t, FLT_MAX);
+                            if (t * now >= 0x1p15f) now = pow2(11 - exponent(t));
+                            if (!nothing) scale_o(nr, gi, c, pow2_ratio(now, was));
+                            by[nr][gi][c] = now;
+                            any = fmaxf(any, t);
+                            least = fminf(least, now);
+                        }
+                        fades[nr][c] = m[nr][c] == -INFINITY ? -INFINITY : m[nr][c] + 8.0f / sl2[nr][c];
+                        lift[nr][c] = least;
+                        if (m[nr][c] != -INFINITY) highest = fmaxf(highest, least);
+#pragma unroll
+                        for (int gi = 0; gi < G; ++gi) {
+                            const float now = by[nr][gi][c];
+                            const bool none = any > 0.0f && most[gi] == 0.0f;
+                            if (none) dead |= 1u << gi;
+                            apart = apart || !(now == least || (none ? now == kC4MostLift || now * 0x1p-64f <= least : most[gi] * least >= 4.0f));
                         }
                     }
                 }
-                float p[4], lifted[4];
+                if constexpr (G > 1) {
+                    dead = __reduce_or_sync(0xffffffffu, dead);
+                    __syncwarp();            // (all lanes have read their rows' lifts)
+                    uneven = __any_sync(0xffffffffu, apart);
+                    leave = !kByGroups && (uneven || dead != 0);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[e] = fast_exp2((s[nr][e] - ref[nr][e & 1]) * sl2[nr][e & 1]);
-                    if (!kLiftSteps) lifted[e] = p[e] * v_lift;
-                    l[nr][e & 1] += p[e];
+                    for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+                        for (int gi = 0; gi < G; ++gi) {
+                            if (uneven) {
+                                if (g == 0) own[(nr * G + gi) * 4] = make_float2(by[nr][gi][0], by[nr][gi][1]);
+                            } else {
+#pragma unroll
+                                for (int c = 0; c < 2; ++c) {
+                                    scale_o(nr, gi, c, pow2_ratio(lift[nr][c], by[nr][gi][c]));
+                                    by[nr][gi][c] = lift[nr][c];
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                const uint32_t high = __reduce_max_sync(0xffffffffu, __float_as_uint(highest));
+                v_most = high == 0 ? INFINITY : pow2(min(127, 15 - exponent(__uint_as_float(high))));
+            }
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                float lifted[4];
+                if (!kSpecial) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) lifted[e] = p[nr][e] * lift[nr][e & 1];
                 }
 #pragma unroll
                 for (int gi = 0; gi < G; ++gi) {
@@ -391,16 +487,16 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             const int e = 2 * h + c;
-                            w[e] = kLiftSteps ? p[e] * lifted_step[h][gi] : lifted[e] * v.x;
-                            if (!kOdd) lo[nr][gi][c] = fmaf(p[e], mid, lo[nr][gi][c]);
+                            w[e] = (kSpecial ? p[nr][e] * by[nr][kSpecial ? gi : 0][c] : lifted[e]) * v.x;
+                            if (!kSpecial) lo[nr][gi][c] = fmaf(p[nr][e], mid, lo[nr][gi][c]);
                         }
                     }
-                    if (kOdd) {              // (what a query does not see is left out; zero times what it does see is NaN where that is not finite)
+                    if (kSpecial) {              // (what a query does not see is left out; zero times what it does see is NaN where that is not finite)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float2 v = layer_pair<kBf16>(vp[e >> 1][gi]);
                             if ((hidden >> (nr * 4 + e)) & 1u) w[e] = 0.0f;
-                            else lo[nr][gi][e & 1] = fmaf(p[e], fmaf(8.0f, v.x, v.y), lo[nr][gi][e & 1]);
+                            else lo[nr][gi][e & 1] = fmaf(p[nr][e], fmaf(8.0f, v.x, v.y), lo[nr][gi][e & 1]);
                         }
                     }
                     const uint32_t b0 = c4_transpose8(pack2<false>(w[0], w[1])), b1 = c4_transpose8(pack2<false>(w[2], w[3]));
@@ -423,9 +519,12 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
                 }
             }
         };
-        if (odd) weigh(std::true_type{});
+        if (__builtin_expect(special, 0)) weigh(std::true_type{});
         else weigh(std::false_type{});
     }
+    };
+    walk(std::false_type{});
+    if constexpr (G > 1) walk(std::true_type{});
     // the warps' sums, whole: over the lanes' keys, the lows and the powers of two put in
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -439,7 +538,6 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
             }
         }
     }
-    const float v_down = pow2(max(-126, v_exp));
     float* const mine = o_warp + warp * kRows * C::kLd;
     __syncthreads();
 #pragma unroll
@@ -452,9 +550,10 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 const float low = lo[nr][s / kPer][h];
+                const float down = pow2(-exponent(uneven ? reinterpret_cast<const float*>(own + (nr * G + s / kPer) * 4)[h] : lift[nr][h]));
                 *reinterpret_cast<float4*>(mine + r * C::kLd + 32 * s + 4 * g) =
-                    make_float4(fmaf(o[nr][2 * s][h] * 0x1p24f, v_down, low), fmaf(o[nr][2 * s + 1][h] * 0x1p20f, v_down, low),
-                                fmaf(o[nr][2 * s][2 + h] * 0x1p24f, v_down, low), fmaf(o[nr][2 * s + 1][2 + h] * 0x1p20f, v_down, low));
+                    make_float4(fmaf(o[nr][2 * s][h] * 0x1p24f, down, low), fmaf(o[nr][2 * s + 1][h] * 0x1p20f, down, low),
+                                fmaf(o[nr][2 * s][2 + h] * 0x1p24f, down, low), fmaf(o[nr][2 * s + 1][2 + h] * 0x1p20f, down, low));
             }
         }
     }
