@@ -662,7 +662,7 @@ cudaError_t pick_cache4(SdpaCache4Args a, cudaStream_t stream) {
     // three CTAs to an SM: over six 232 us, over five 240, seven 241, eight 238; keys all alike 303, 330, 336, 332), and the smallest such part with
     // two and a half rounds (512 heads over up to 8192 keys: over three 129, over six 137; 256 heads: over three 252).  Eight, where all run at
     // once, but one step to a warp at least (8 heads over 777 keys: over eight 4.1, over sixteen 4.4, over six 4.7).
-    constexpr int kOne = HD == 64 || G == 1 ? 4 : 3, kTwo = HD == 64 ? 4 : 2;           // CTAs of an SM: what registers allow
+    constexpr int kOne = HD == 64 || G == 1 ? 4 : 3, kTwo = HD == 64 ? (G == 1 ? 4 : 3) : 2;           // CTAs of an SM: what registers allow
     const int ctas = nr == 1 ? kOne : kTwo, slots = sms * ctas;
     int split = 8;
     if (units * 8 > slots) {
