@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(W * 32, kCtas) w4_few_kernel(const __grid_cons
 #pragma unroll
         for (int gi = 0; gi < kGroups; ++gi) {
             constexpr int kPer = 4 / kGroups;
-            // sums of X over the group's columns, in the places of their rows of C: a product with ones
+            // sums of X over the group's columns, in the places of their rows of C: a product with ones, at 2^32 times their size, so
+            // that no sum of values below 2^64 is beyond FP32
             float xs[NR][4];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
@@ -101,19 +102,19 @@ __global__ void __launch_bounds__(W * 32, kCtas) w4_few_kernel(const __grid_cons
                 for (int s = gi * kPer; s < (gi + 1) * kPer; ++s) {
                     uint4& v = xv[i][s][r];
                     if constexpr (kBf16) {
-                        // 2^64, and 2^60 where the codes are sixteen times theirs: exact, beyond FP32 from |x| = 2^63 on
+                        // 2^64, and 2^60 where the codes are sixteen times theirs: exact, infinite from |x| = 2^64 on
                         v.x = times_pow2(v.x, 0x5f805f80u);
                         v.y = times_pow2(v.y, 0x5f805f80u);
                         v.z = times_pow2(v.z, 0x5d805d80u);
                         v.w = times_pow2(v.w, 0x5d805d80u);
                     }
-                    constexpr uint32_t kOne = kBf16 ? 0x3f803f80u : 0x3c003c00u, kOdd = kBf16 ? 0x41804180u : kOne;
+                    constexpr uint32_t kOne = kBf16 ? 0x2f802f80u : 0x3c003c00u, kOdd = kBf16 ? 0x31803180u : kOne;
                     mma16<kBf16>(xs[r], kOne, kOne, kOne, kOne, v.x, v.y);
                     mma16<kBf16>(xs[r], kOdd, kOdd, kOdd, kOdd, v.z, v.w);
                 }
                 if constexpr (kBf16) {
-                    xs[r][0] *= 0x1p-64f;
-                    xs[r][1] *= 0x1p-64f;
+                    xs[r][0] *= 0x1p-32f;
+                    xs[r][1] *= 0x1p-32f;
                 }
             }
 #pragma unroll

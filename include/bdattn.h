@@ -669,7 +669,7 @@ int bdattn_sandwich_norm_fwd(const bdattn_sandwich_norm_params* p, bdattn_stream
  * dtype BF16 / F16, the pairs of the weights too; bias, gate and residual may be NULL; residual may be Y (same ld).  K (up to
  * 2^30) and x_ld are multiples of 8, X is 16-byte aligned; any N; up to 524280 rows.  Y may not overlap X.  Meant for few rows: up to 16
  * read W once, more read it again (from the L2, if it fits) for each 16; for prompts bdattn_w4_unpack and a product in 16 bits take
- * less time.  A row of X with a value that is not finite (BF16: of 2^63
+ * less time.  A row of X with a value that is not finite (BF16: of 2^64
  * and more) comes out not finite; BF16 values below 2^-57 may count as zeros.
  * bdattn_w4_pack: codes (N, K / 2 bytes, row stride codes_ld bytes) hold two columns a byte, the even one in the low half;
  * scales (N, ceil(K / group), 2) the pairs, row stride scales_ld values; a last group may be short.
