@@ -138,13 +138,14 @@ __global__ void __launch_bounds__(W * 32, kCtas) w4_few_kernel(const __grid_cons
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    // (BF16: the codes' units go to the sums, since a step times them may be beyond FP32; that costs up to 3 %)
                     float2 sl = layer_pair<kBf16>(sv[i][t][h][gi]);
-                    sl.x *= kBf16 ? 0x1p69f : 0x1p24f;
+                    if (!kBf16) sl.x *= 0x1p24f;
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float f = kBf16 ? d[r][2 * h + c] + e[r][2 * h + c] : fmaf(e[r][2 * h + c], 0.0625f, d[r][2 * h + c]);
+                            const float f = kBf16 ? (d[r][2 * h + c] + e[r][2 * h + c]) * 0x1p69f : fmaf(e[r][2 * h + c], 0.0625f, d[r][2 * h + c]);
                             y[t][r][2 * h + c] = fmaf(f, sl.x, fmaf(xs[r][c], sl.y, y[t][r][2 * h + c]));
                         }
                     }

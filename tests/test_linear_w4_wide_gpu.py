@@ -43,6 +43,21 @@ def test_sums_of_large_activations(bd, size, m, group):
     check(run(bd, x, pack(bd, codes, scales, group), n, group), x, codes, scales, group)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 11])
+@pytest.mark.parametrize("size", [2.0 ** 57, 2.0 ** 62, 2.0 ** 100, 2.0 ** -100])
+def test_steps_of_any_size(bd, size, m, group):
+    """(and rows of X that are zero, which stay zero)"""
+    n, k = 40, 512
+    codes = exact_codes(n, k)
+    scales = torch.stack([randn(1, n, k // group, dtype=torch.float32) * size, randn(2, n, k // group, dtype=torch.float32) * size], -1).bfloat16()
+    x = randn(3, m, k)
+    x[0, :256] = 0
+    packed = pack(bd, codes, scales, group)
+    check(run(bd, x, packed, n, group), x, codes, scales, group)
+    assert (run(bd, torch.zeros_like(x), packed, n, group) == 0).all()
+
+
 CAPTURED_FIRST = """
 import torch, brodiffusion_b200 as bd
 r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
