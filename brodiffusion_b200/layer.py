@@ -193,6 +193,9 @@ class FourBitLayer:
             return stream
         if max(cache.filled) + L > min(cache.rows.rows, cos.shape[0]):
             raise bd.BdattnError(f"{L} new tokens do not fit the cache or the RoPE tables")
+        for name in ("gate1", "gate2"):
+            if name in w and w[name].dim() == 2 and (len(w[name]) < 1 or B % len(w[name])):
+                raise bd.BdattnError(f"{name} must have a vector for each batch / n sequences ({len(w[name])} for {B})")
         rows = stream.view(B * L, D)
         x = torch.empty_like(rows)
         bd.add_rmsnorm_fwd(rows, x, w["norm1"], eps=self.eps)

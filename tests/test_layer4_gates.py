@@ -1,0 +1,41 @@
+"""What a layer with weights and cache in 4 bits refuses ahead of its first call (no GPU)."""
+import pytest
+import torch
+
+import brodiffusion_b200 as bd
+from brodiffusion_b200 import layer as LY
+
+BF16 = torch.bfloat16
+D, NH, NKV, HD, F = 64, 2, 1, 64, 128
+
+
+def z(*shape, dtype=BF16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def layer(monkeypatch, **more):
+    monkeypatch.setattr(LY, "quantise_rows4", lambda w, group: None)
+    f = torch.float32
+    w = dict(norm1=z(D, dtype=f), norm2=z(D, dtype=f), post1=z(D, dtype=f), post2=z(D, dtype=f), wqkv=z((NH + 2 * NKV) * HD, D),
+             wo=z(D, NH * HD), w_up=z(F, D), w_down=z(D, F), **more)
+    return LY.FourBitLayer(w, NH, NKV, HD)
+
+
+def nothing_is_called(monkeypatch):
+    def call(*a, **kw):
+        raise AssertionError("a call was made")
+    for name in ("add_rmsnorm_fwd", "linear_w4_fwd", "rmsnorm_rope", "cache4_append", "cache4_read", "sdpa_cache4_fwd", "sdpa_window_fwd",
+                 "sandwich_norm_fwd", "w4_unpack", "linear_act_fwd"):
+        monkeypatch.setattr(bd, name, call)
+
+
+@pytest.mark.parametrize("which", ["gate1", "gate2"])
+@pytest.mark.parametrize("B,n,L", [(3, 2, 2), (3, 2, 1), (2, 4, 2), (2, 4, 4), (1, 3, 3)])
+def test_gates_that_do_not_divide_the_sequences(monkeypatch, which, B, n, L):
+    """n vectors are for B / n sequences each: rows alone would let a vector end inside a sequence."""
+    layer4 = layer(monkeypatch, **{"gate1": z(D), "gate2": z(D), which: z(n, D)})
+    nothing_is_called(monkeypatch)
+    kv = LY.KvCache4(B, 16, NKV, HD, 32, BF16, device="cpu")
+    with pytest.raises(bd.BdattnError, match="gate"):
+        layer4.forward(z(B, L, D), kv, z(16, HD // 2), z(16, HD // 2))
+    assert kv.filled == [0] * B and kv.lengths.tolist() == [0] * B
