@@ -164,7 +164,11 @@ class FourBitLayer:
 
     def __init__(self, weights, num_heads, num_kv_heads, head_dim, *, window=0, sinks=0, act="gelu_tanh", eps=1e-6, group=64,
                  residual_scale=1.0):
+        import torch
         self.w = {n: t for n, t in weights.items() if n not in ("wqkv", "wo", "w_up", "w_down")}
+        self.dtype = weights["wqkv"].dtype   # (of the steps and lows, which the packed bytes do not say)
+        if self.dtype not in (torch.bfloat16, torch.float16) or any(weights[n].dtype != self.dtype for n in ("wo", "w_up", "w_down")):
+            raise bd.BdattnError("wqkv, wo, w_up and w_down must be of one 16-bit dtype")
         self.nh, self.nkv, self.hd = num_heads, num_kv_heads, head_dim
         self.window, self.sinks, self.act, self.eps, self.group, self.scale = window, sinks, act, eps, group, residual_scale
         self.widths = {n: weights[n].shape[0] for n in ("wqkv", "wo", "w_up", "w_down")}
@@ -189,6 +193,8 @@ class FourBitLayer:
         w, nh, nkv, hd = self.w, self.nh, self.nkv, self.hd
         if B != len(cache.filled) or not stream.is_contiguous():
             raise bd.BdattnError("stream must be dense, with a sequence for every one of the cache")
+        if stream.dtype != self.dtype:
+            raise bd.BdattnError(f"stream must have the weights' dtype ({self.dtype}, got {stream.dtype})")
         if L == 0:
             return stream
         if max(cache.filled) + L > min(cache.rows.rows, cos.shape[0]):

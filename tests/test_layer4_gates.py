@@ -39,3 +39,26 @@ def test_gates_that_do_not_divide_the_sequences(monkeypatch, which, B, n, L):
     with pytest.raises(bd.BdattnError, match="gate"):
         layer4.forward(z(B, L, D), kv, z(16, HD // 2), z(16, HD // 2))
     assert kv.filled == [0] * B and kv.lengths.tolist() == [0] * B
+
+
+@pytest.mark.parametrize("odd", ["wqkv", "wo", "w_up", "w_down"])
+def test_matrices_of_several_types(monkeypatch, odd):
+    """Packed weights do not say of which type their pairs are."""
+    monkeypatch.setattr(LY, "quantise_rows4", lambda w, group: None)
+    w = dict(norm1=z(D), norm2=z(D), post1=z(D), post2=z(D), wqkv=z((NH + 2 * NKV) * HD, D), wo=z(D, NH * HD), w_up=z(F, D), w_down=z(D, F))
+    LY.FourBitLayer(w, NH, NKV, HD)
+    with pytest.raises(bd.BdattnError, match="dtype"):
+        LY.FourBitLayer({**w, odd: w[odd].half()}, NH, NKV, HD)
+    with pytest.raises(bd.BdattnError, match="dtype"):
+        LY.FourBitLayer({**w, **{n: w[n].float() for n in ("wqkv", "wo", "w_up", "w_down")}}, NH, NKV, HD)
+
+
+@pytest.mark.parametrize("L", [1, 40])
+def test_a_stream_of_another_type_than_the_weights(monkeypatch, L):
+    """(gains in FP32 fit both)"""
+    layer4 = layer(monkeypatch)
+    nothing_is_called(monkeypatch)
+    kv = LY.KvCache4(2, 64, NKV, HD, 32, torch.float16, device="cpu")
+    with pytest.raises(bd.BdattnError, match="dtype"):
+        layer4.forward(z(2, L, D, dtype=torch.float16), kv, z(64, HD // 2), z(64, HD // 2))
+    assert kv.filled == [0, 0] and kv.lengths.tolist() == [0, 0]
