@@ -155,8 +155,13 @@ class FourBitLayer:
     """``weights`` as for ``CausalLayer``, and post1, post2 (D), the gains behind the two blocks; optionally gate1, gate2 (D)
     or (n, D), a vector for each batch / n sequences.  ``group``: columns of W to a step and a low."""
 
-    # New tokens of a sequence from which on the cache is read back to 16 bits for the attention of whole prompts: that kernel takes
-    # 128 rows at a time (2 x 509 rows of 16 heads over 8009 keys: 145 us from the 4 bits).
+    # The attention reads 16-bit rows, read back from the cache, from PROMPT new tokens of a sequence and 64 rows of heads to a K/V head on: it takes 128 of
+    # those at a time, the kernel over 4 bits sixteen.  Heads of 128, groups of 32, 8 K/V heads, us from the 4 bits and by way of 16:
+    #   24 heads, 8 tokens over 1000 / 8000 / 32768 keys 12.0, 26.6, 72 and 12.5, 22.7, 75, of 32 sequences of 8192 259 and 448;
+    #   32 tokens 15.0, 43, 133 and 14.4, 37, 127, of 32 sequences 722 and 720; 64 tokens 26, 82, 223 and 17, 57, 207, of 32 sequences 1352 and 721;
+    #   8 heads, 8 sequences of 8000: 32 tokens 84 and 122, 64 tokens 162 and 157.
+    # With a window only what it shows is read back, where all sequences are as long (32 sequences of 8192, window 1024: 16 tokens 88 and 104, 32 tokens
+    # 162 and 133, with all rows read back 344).
     PROMPT = 32
     # Rows from which on a matrix goes back to 16 bits ahead of its product, a workspace of the call's (10240 x 2560: 64 rows 29.5 us in 4 bits,
     # 21.7 so, 32 rows 18.2 and 21.6; 1536 rows 606 and 70).
@@ -214,24 +219,31 @@ class FourBitLayer:
         cache.lengths += L
         try:
             bd.cache4_append(k, v, cache.rows, kv_len=cache.lengths)
-            self._behind_the_cache(rows, x, q, cache, max(cache.filled) + L)
+            self._behind_the_cache(rows, x, q, cache, min(cache.filled) + L, max(cache.filled) + L)
         except BaseException:
             cache.lengths -= L               # the rows behind the lengths are nobody's
             raise
         cache.filled[:] = [n + L for n in cache.filled]
         return stream
 
-    def _behind_the_cache(self, rows, x, q, cache, most):
-        """Attention over the first ``most`` rows of the cache (no row behind the longest sequence is looked at) and what follows."""
+    def _behind_the_cache(self, rows, x, q, cache, least, most):
+        """Attention over the first ``most`` rows of the cache (no row behind the longest sequence is looked at; the shortest has ``least``) and
+        what follows."""
         import torch
         w, held = self.w, cache.rows.first(most)
         att = torch.empty(q.shape, device=q.device, dtype=q.dtype)
         seen = dict(window=self.window, sinks=self.sinks, kv_len=cache.lengths)
-        if q.shape[1] < self.PROMPT:
+        new = q.shape[1]
+        if new < self.PROMPT or new * self.nh < 64 * self.nkv:
             bd.sdpa_cache4_fwd(q, held, att, self.nh, **seen)
         else:
+            tail, first, places = self.window + new - 1, 0, {}
+            if 0 < self.window and self.sinks + tail <= least:           # the first rows that stay visible, and the last that any new token sees
+                first, most, places = self.sinks, self.sinks + tail, dict(kv_len=seen.pop("kv_len"))
             k, v = (torch.empty(q.shape[0], most, self.nkv * self.hd, device=q.device, dtype=q.dtype) for _ in range(2))
-            bd.cache4_read(held, k, v)
+            if first > 0:
+                bd.cache4_read(held.first(first), k[:, :first], v[:, :first])
+            bd.cache4_read(held, k[:, first:], v[:, first:], **places)
             bd.sdpa_window_fwd(q, k, v, att, self.nh, num_kv_heads=self.nkv, **seen)
         behind = dict(residual_scale=self.scale, eps=self.eps)
         branch = self._product(att.view(len(rows), -1), "wo")

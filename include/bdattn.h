@@ -715,8 +715,9 @@ int bdattn_linear_w4_fwd(const bdattn_linear_w4_params* p, bdattn_stream_t strea
  *
  * bdattn_sdpa_cache4_fwd: bdattn_sdpa_window_fwd over such a cache: the same rule of what is seen, the same treatment of
  * kv_len, key_mask and rows that nobody sees (they may hold anything).  Where a row's largest |q| times the scale is 2^117 or more, its scores may be too
- * small by what it is beyond that.  One query segment; o may be q (same strides).  For up to some tens of new tokens:
- * from there on bdattn_cache4_read and bdattn_sdpa_window_fwd take less time. */
+ * small by what it is beyond that.  One query segment; o may be q (same strides).  For few new tokens: from some
+ * 100 to 200 rows (tokens times query heads to a K/V head) on, bdattn_cache4_read and bdattn_sdpa_window_fwd take less time, with a window where
+ * no more is read back than it shows (the last window + q_rows - 1 rows, and the sinks ahead of them). */
 typedef struct bdattn_cache4 {
     int dtype;
     int batch;
