@@ -163,8 +163,9 @@ class FourBitLayer:
     # With a window only what it shows is read back, where all sequences are as long (32 sequences of 8192, window 1024: 16 tokens 88 and 104, 32 tokens
     # 162 and 133, with all rows read back 344).
     PROMPT = 32
-    # Rows from which on a matrix goes back to 16 bits ahead of its product, a workspace of the call's (10240 x 2560: 64 rows 29.5 us in 4 bits,
-    # 21.7 so, 32 rows 18.2 and 21.6; 1536 rows 606 and 70).
+    # Rows from which on a matrix goes back to 16 bits ahead of its product, a workspace of the call's, and half as many more for one of less
+    # than 2^23 values (us in 4 bits and so, groups of 32: 10240 x 2560, 32 rows 21.2 and 22.3, 48 rows 28 and 23, 1536 rows 606 and 70; 5120 x 5120, 32 rows 20.5 and
+    # 24.7, 64 rows 33 and 25; 2560 x 2560, 64 rows 12.1 and 14.2, 96 rows 16.0 and 14.4; 1280 x 1280, 64 rows 5.8 and 8.0, 128 rows 7.8 and 7.6).
     MANY = 64
 
     def __init__(self, weights, num_heads, num_kv_heads, head_dim, *, window=0, sinks=0, act="gelu_tanh", eps=1e-6, group=64,
@@ -182,7 +183,7 @@ class FourBitLayer:
     def _product(self, x, name, bias=None, **kw):
         import torch
         y = torch.empty(len(x), self.widths[name], device=x.device, dtype=x.dtype)
-        if len(x) < self.MANY:
+        if len(x) < (self.MANY if self.widths[name] * x.shape[1] >= 1 << 23 else self.MANY * 3 // 2):
             bd.linear_w4_fwd(x, self.packed[name], bias, y, group=self.group, **kw)
         else:
             w = torch.empty(self.widths[name], x.shape[1], device=x.device, dtype=x.dtype)

@@ -62,3 +62,15 @@ def test_a_stream_of_another_type_than_the_weights(monkeypatch, L):
     with pytest.raises(bd.BdattnError, match="dtype"):
         layer4.forward(z(2, L, D, dtype=torch.float16), kv, z(64, HD // 2), z(64, HD // 2))
     assert kv.filled == [0, 0] and kv.lengths.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("D,F,rows,many", [(64, 128, 95, False), (64, 128, 96, True), (2048, 4096, 63, False), (2048, 4096, 64, True), (2040, 4096, 64, False)])
+def test_matrices_that_go_back_to_16_bits(monkeypatch, D, F, rows, many):
+    """Small ones half as many rows later."""
+    monkeypatch.setattr(LY, "quantise_rows4", lambda w, group: None)
+    w = dict(norm1=z(D), norm2=z(D), post1=z(D), post2=z(D), wqkv=z(3 * HD, D), wo=z(D, HD), w_up=z(F, D), w_down=z(D, F))
+    made = []
+    for name in ("linear_w4_fwd", "w4_unpack", "linear_act_fwd"):
+        monkeypatch.setattr(bd, name, lambda *a, name=name, **kw: made.append(name))
+    y = LY.FourBitLayer(w, 1, 1, HD)._product(z(rows, D), "w_up")
+    assert y.shape == (rows, F) and made == (["w4_unpack", "linear_act_fwd"] if many else ["linear_w4_fwd"])
