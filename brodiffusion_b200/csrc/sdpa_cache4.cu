@@ -48,7 +48,7 @@ struct Cache4Cfg {
     static constexpr int kCodes = 16 * HD / 2, kScales = 16 * 4 * G, kStep = 2 * (kCodes + kScales);      // bytes of sixteen keys
     static constexpr int kRing = W * D * kStep, kSums = W * kRows * kLd * 4;                              // (the sums lie in the ring's place)
     static constexpr int kFirst = kRing > kSums ? kRing : kSums;
-    static constexpr int kSmem = kFirst + (kMergeRows * (kLd + 2) + W * kRows * (2 + G)) * 4;
+    static constexpr int kSmem = kFirst + (kMergeRows * (kLd + 2) + W * kRows * (2 + (G > 1 ? G : 0))) * 4;
 };
 
 // Global to shared memory, 4, 8 or 16 bytes.
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     float* const o_cta = reinterpret_cast<float*>(c4_smem + C::kFirst);     // [kMergeRows][kLd]
     float2* const ml_warp = reinterpret_cast<float2*>(o_cta + C::kMergeRows * C::kLd);     // [W][kRows]
     float2* const ml_cta = ml_warp + W * kRows;                             // [kMergeRows]
-    float2* const lifts = ml_cta + C::kMergeRows;                           // [W][NR][G][4], pairs of rows
+    float2* const lifts = ml_cta + C::kMergeRows;                           // [W][NR][G][4], pairs of rows (with more than one group)
 
     const int warp = warp_index(), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int split = a.split, part = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;

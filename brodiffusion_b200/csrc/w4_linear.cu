@@ -294,7 +294,9 @@ cudaError_t go_w4_few(const W4Args& a, cudaStream_t stream) {
 // warp's K tiles in registers (1368 x 1291, one row 2.3 us, two row tiles to a CTA 2.7; 2560 x 1280 2.5 and 2.7).  More:
 // two row tiles to a CTA of eight warps, two or three CTAs to an SM (2560 x 2560 over three CTAs 2.9, over two 3.9, whole 4.1; 10240 x 2560
 // whole 5.8, over two 8.3), and of four warps, five CTAs to an SM, for the rest (5120 x 5120 over four 6.0, over two CTAs of eight warps
-// 6.8; 20480 x 5120 15.3, 15.6).
+// 6.8; 20480 x 5120 15.3, 15.6): that is where rows of W are longer than 24 K tiles and the second form finds room for clusters (10240 rows of 2560,
+// 2944, 3328, 5120 columns 6.4, 7.0, 8.0, 10.4 us by the first, 6.9, 6.9, 8.0, 9.8 by the second; 13824 rows, which leave it none, 6.5, 7.0, 8.1, 10.7 and
+// 8.9, 10.2, 11.4, 15.9).
 template <bool kBf16, int kGroups>
 cudaError_t pick_w4(W4Args a, cudaStream_t stream) {
     const int sms = sm_count(), tiles = (a.p.N - 1) / 16 + 1, pairs = (tiles + 1) / 2, kt = a.k_tiles;
@@ -315,7 +317,7 @@ cudaError_t pick_w4(W4Args a, cudaStream_t stream) {
         if ((a.parts = split(pairs, 2ll * sms, 8, 1)) != 0 || (a.parts = split(pairs, sms, 8, 2)) != 0)
             return go_w4_few<kBf16, kGroups, 8, 2, 1, 1, 2>(a, stream);
         a.parts = 1;
-        if (pairs <= 3 * sms && kt <= 24) return go_w4_few<kBf16, kGroups, 8, 2, 1, 1, 3>(a, stream);
+        if (pairs <= 3 * sms && (kt <= 24 || 2 * pairs > 5 * sms)) return go_w4_few<kBf16, kGroups, 8, 2, 1, 1, 3>(a, stream);
         a.parts = spread(pairs, 5ll * sms, 4);
         return go_w4_few<kBf16, kGroups, 4, 2, 1, 1, 5>(a, stream);
     }

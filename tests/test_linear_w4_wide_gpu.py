@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("n,k,ms", [(10230, 2560, (1, 8, 12, 16)), (5111, 5120, (1, 8, 32, 48)), (2551, 2568, (1, 7, 24)), (2551, 10240, (1, 8, 12, 16, 32, 48)),
-                                    (5111, 5000, (5, 13)), (20471, 1032, (1, 20)), (1291, 10240, (3, 40)), (4711, 1928, (8, 9)), (5111, 1288, (24,))])
+                                    (5111, 5000, (5, 13)), (13810, 4104, (1, 8)), (20471, 1032, (1, 20)), (1291, 10240, (3, 40)), (4711, 1928, (8, 9)), (5111, 1288, (24,))])
 def test_sizes_of_large_layers(bd, n, k, ms, group, dtype):
     codes, scales = weights(n + k, n, k, group, dtype)
     packed = pack(bd, codes, scales, group)
