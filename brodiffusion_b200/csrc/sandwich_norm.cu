@@ -5,7 +5,7 @@
 //   out = y rounded, or  a = max|y| / 448,  out = e4m3(y / a),  out_scale = a, or nothing
 // x and residual are read once, both sums of squares are of unrounded values.  Bound by memory from a few hundred
 // rows on (6 bytes an element for the stream and 1 or 2 for the output), by two meetings of a row's threads below: the second
-// sum needs the first one's root.  16384 x 5120 to 8 bits 104.5 us (5.6 TB/s), 4332 x 2240 in 16 bits 17.9 (4.3 TB/s), one row 2.4.
+// sum needs the first one's root.  16384 x 5120 to 8 bits 105 to 117 us by the GPU (5.0 to 5.6 TB/s), 4332 x 2240 in 16 bits 17.9 (4.3 TB/s), one row 2.4.
 #include <type_traits>
 
 #include "norm_rows.cuh"
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kTeam > 0 ? 128 : kV == 1 ? 1024 : 512, kTeam 
 }
 
 // Rows wider than the registers of a CTA, and tensors that are off 16 bytes by different numbers of elements: an element at a
-// time, read three times (the second and third from the L2).
+// time, read three times (the second and third from the L2).  4096 x 20480 557 us, its bytes 102; 4096 x 5120 188, 31 by the kernel above.
 template <bool kBf16>
 __global__ void __launch_bounds__(1024) sandwich_norm_any_kernel(const __grid_constant__ SandwichNormArgs a) {
     __shared__ float red[2][64];
@@ -295,7 +295,7 @@ cudaError_t launch_sandwich(SandwichNormArgs a, cudaStream_t stream) {
         if (pieces <= 1024) return go(sandwich_norm_kernel<kBf16, kFp8, 2, 0, kS>, 1, threads(2));
         return go(sandwich_norm_kernel<kBf16, kFp8, 4, 0, kS>, 1, threads(4));
     };
-    if (same && a.cols <= 16384 - 14) return zero ? pick(std::false_type{}) : pick(std::true_type{});
+    if (same && a.cols <= (zero ? 16384 : 16384 - 14)) return zero ? pick(std::false_type{}) : pick(std::true_type{});
     const int threads = a.cols < 1024 ? (a.cols + 31) / 32 * 32 : 1024;
     return launch_dependent(sandwich_norm_any_kernel<kBf16>, dim3(static_cast<unsigned>(a.rows)), dim3(threads), 0, stream, a);
 }

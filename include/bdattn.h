@@ -632,8 +632,8 @@ int bdattn_sdpa_window_fwd(const bdattn_sdpa_params* p, const bdattn_window_para
  *   y = h * rsqrt(mean(h^2) + eps) * gain,  out and out_scale from y as in bdattn_add_rmsnorm_fwd.
  * x is the block's output, residual the stream; gate: `gates` vectors of cols values, of which row r has number
  * r / (rows / gates) (batch items with a modulation each); post_gain, gain, gate and out may be NULL (out: the last block;
- * gain goes with out).  Both norms are of unrounded values.  A sum of squares that is not finite in FP32 gives NaN, rows of
- * zeros stay zeros with an eps of 0 too.
+ * gain goes with out).  Both norms are of unrounded values; x * post_gain * gate has to be within FP32's range.  A sum of squares
+ * that is not finite in FP32 gives NaN, rows of zeros stay zeros with an eps of 0 too.
  * residual_out may be residual or x, out may be x or residual where its dtype is theirs (same ld).  Sizes, strides and
  * alignments as for bdattn_add_rmsnorm_fwd. */
 typedef struct bdattn_sandwich_norm_params {
