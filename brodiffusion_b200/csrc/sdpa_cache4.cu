@@ -10,7 +10,7 @@
 // arithmetic) and has a running maximum, sum and accumulator of its own; these meet in shared memory, then in distributed
 // shared memory, where every CTA of a head's cluster finishes its share of the rows.
 // What a call has to do is read the visible rows once, 4 + 32 / group bits a value.  What bounds it is issue, some 400 instructions to sixteen
-// keys of a warp: of 32 sequences of up to 32768 keys (231 us), reading alone took 136 us when the whole took 247, arithmetic alone 244.
+// keys of a warp: of 32 sequences of up to 32768 keys (237 us), reading alone took 136 us when the whole took 247, arithmetic alone 244.
 #include "four_bit.cuh"
 #include "sdpa_window.cuh"
 
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(W * 32, kCtas) sdpa_cache4_kernel(const __grid
     // what it sees, and by what counts of that, alone: a key that it does not see, or that has next to no weight, may have steps 2^100 times as large.
     // One lift serves all groups of a row while the largest of each is 2^2 or more by it; then (uneven) each has its own, in shared memory.
     // What FP16 loses below its normal range is 2^-19 of the largest a key then, at most.  (One lift for all rows, by the largest step that any of them might
-    // see, took 1 to 6 % less: 32 sequences of up to 32768 keys 248 us, this way 254, groups of 128 83.0 and 83.5.)
+    // see, took up to 6 % less: 32 sequences of up to 32768 keys 231 us, this way 237, of 8192 in groups of 128 83.2 and 83.8.)
     float lift[NR][2], fades[NR][2];      // (fades: scores from here on make 2^-8 and less of what a row has so far)
     float v_most = INFINITY;              // steps from here on might be too large
     bool uneven = false;

@@ -50,5 +50,6 @@ def test_rows_that_are_read_back(bd, monkeypatch, window, sinks, new, filled, ro
     assert asked == rows
     by_codes, asked = stream(bd, monkeypatch, L, x, filled, 10 ** 9, nkv, hd, 600)
     assert asked == []
-    # the caches are the same to the bit, so what differs is K and V in 16 bits: 2^-9 of each, as the steps between are rounded
+    # the caches are the same to the bit, so what differs is K and V in 16 bits, 0.0016 rms of each, and the roundings of the steps behind
+    # (eight of them, of as much: 0.0046, twice that)
     assert far(by_rows, by_codes) < 0.01 < BOUND
