@@ -9,7 +9,7 @@
 // ring in shared memory of its own (cp.async: straight to registers 285 us of 32 sequences of up to 32768 keys, the ring 257 at the same
 // arithmetic) and has a running maximum, sum and accumulator of its own; these meet in shared memory, then in distributed
 // shared memory, where every CTA of a head's cluster finishes its share of the rows.
-// What a call has to do is read the visible rows once, 4 + 32 / group bits a value.  What bounds it is issue, some 400 instructions to sixteen
+// What a call has to do is read the visible rows once, 4 + 32 / group bits a value.  What bounds it is issue, some 450 instructions to sixteen
 // keys of a warp: of 32 sequences of up to 32768 keys (237 us), reading alone took 136 us when the whole took 247, arithmetic alone 244.
 #include "four_bit.cuh"
 #include "sdpa_window.cuh"
